@@ -19,6 +19,7 @@ _i64 = ctypes.c_int64
 _i32 = ctypes.c_int
 _f32 = ctypes.c_float
 _size_t = ctypes.c_size_t
+_i64p = ctypes.POINTER(ctypes.c_int64)
 
 # name -> (restype, argtypes); mirrors include/dsa_b200.h
 SIGNATURES = {
@@ -67,6 +68,9 @@ SIGNATURES = {
                              _c_void_p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32,
                              _i64, _i32, _i64, _f32, _c_void_p, _c_void_p, _i32, _i32, _i32,
                              _c_void_p, _f32, _c_void_p, _c_void_p, _size_t, _c_void_p]),
+    "dsa_window_attn_fwd": (_i32, [_c_void_p, _i64p, _c_void_p, _i64p, _c_void_p, _i64p,
+                                   _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64,
+                                   _i64, _i32, _i32, _i32, _i64, _i64, _f32, _c_void_p]),
 }
 
 _LIB = None

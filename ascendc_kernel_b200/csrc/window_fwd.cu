@@ -1,0 +1,583 @@
+// Attention with a sliding window and a few first tokens that stay visible,
+// forward, for sm_100a.
+//
+//   s_j = scale q.k_j over the keys a row sees (window_common.cuh)
+//   out = sum_j e^(s_j) v_j / (sum_j e^(s_j) + e^(sink_h)),  lse = log of the divisor
+// A row that sees no key and has no sink gets out = 0 and lse = -inf.
+//
+// One pass over the keys with a running reference (maximum) and sum in fp32.
+// Per CTA (one per SM, persistent, 384 threads), a work item is two 128-row
+// tiles (consecutive tokens, all heads of a group) that share every key chunk of
+// up to 128 keys:
+//   warp 0      TMA: q tiles, K and V chunks into a ring of slots (one slot a
+//               chunk when K and V are the same tensor).
+//   warp 1      tcgen05 issuer: S = Q K^T, then O += P V with P read from TMEM.
+//               Per chunk PV(c) of a tile, then S(c+1) of the same tile into the
+//               columns PV(c) read: one tile's products run under the other
+//               tile's softmax.
+//   warps 4..11 softmax: a warpgroup per tile, a thread per row: no exchange
+//               between threads for the row's maximum and sum.
+// P is rounded to the operands' 16-bit type for the second product (its sum is
+// taken before the rounding, in fp32): a relative 2^-9 (2^-12 for fp16) a term,
+// the size of the output's own rounding. The reference moves, and O is rescaled,
+// only when a row's maximum exceeds it by more than 2^8, so P stays within fp16.
+// TMEM per tile w: S/P columns [256w, 256w+128), O columns [256w+128, 256w+128+D).
+#include "host_util.h"
+#include "window_common.cuh"
+#include "window_host.h"
+
+namespace dsa {
+namespace win {
+
+constexpr int kThreads = 384;
+// The launch holds 384 x 168 registers; the softmax warpgroups, whose threads keep
+// a chunk's 128 scores, take 208 each and the warpgroup of TMA and MMA keeps 88:
+// 128 x 88 + 256 x 208 = 384 x 168.
+constexpr int kRegsAux = 88;
+constexpr int kRegsSoftmax = 208;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kRescaleLog2 = 8.0f;
+constexpr int kChunkBlks = 4;  // blocks of a chunk
+
+template <int D>
+struct FwdCfg {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTileBytes = kRows * D * 2;
+  static constexpr int kSlots = D == 128 ? 4 : 6;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffKV = 2 * kTileBytes;
+  static constexpr int kOffBar = kOffKV + kSlots * kTileBytes;
+  static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 2 + 2 + 2 + 2 + 1;
+  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
+};
+
+struct FwdParams {
+  Shape s;
+  int tt;               // tokens of a tile
+  int tiles;            // token tiles per (batch, kv head)
+  int items_per_head;   // pairs of them
+  int64_t total_items;
+  float scale_log2;
+  const float* sink;    // [h] or null
+  uint16_t* out;        // [batch, m, h, D]
+  float* lse;           // [batch, m, h] or null
+  int shared;           // K and V are one tensor
+  unsigned int* err;
+};
+
+struct Item {
+  int b, kvh, kv_len;
+  int t0[2], t1[2];  // tokens of each tile, empty when t1 <= t0
+  Range r;
+  int chunks;
+};
+
+__device__ __forceinline__ Item make_item(const FwdParams& p, int64_t item) {
+  Item it;
+  const int64_t bh = item / p.items_per_head;
+  const int pair = static_cast<int>(item - bh * p.items_per_head);
+  it.b = static_cast<int>(bh / p.s.hk);
+  it.kvh = static_cast<int>(bh - static_cast<int64_t>(it.b) * p.s.hk);
+  it.kv_len = kv_len_of(p.s, it.b);
+  for (int w = 0; w < 2; ++w) {
+    it.t0[w] = min((2 * pair + w) * p.tt, p.s.m);
+    it.t1[w] = min((2 * pair + w + 1) * p.tt, p.s.m);
+  }
+  it.r = key_range(p.s, it.t0[0], max(it.t1[0], it.t1[1]), it.kv_len);
+  it.chunks = (it.r.nblk + kChunkBlks - 1) / kChunkBlks;
+  return it;
+}
+
+__device__ __forceinline__ int chunk_blocks(const Item& it, int c) {
+  return min(kChunkBlks, it.r.nblk - c * kChunkBlks);
+}
+
+// Whether any row of tile w sees a key of chunk c.
+__device__ __forceinline__ bool tile_active(const FwdParams& p, const Item& it, int w, int c) {
+  if (it.t1[w] <= it.t0[w]) return false;
+  const int off = p.s.n - p.s.m;
+  const int hi = min(it.t1[w] + off, it.kv_len);
+  const int lo = it.t0[w] + off - p.s.window + 1;
+  const int nb = chunk_blocks(it, c);
+  bool any = false;
+  for (int i = 0; i < nb; ++i) {
+    const int k = it.r.key(c * kChunkBlks + i);
+    const bool first = c * kChunkBlks + i < it.r.nfb;
+    any = any || (k < hi && (first || k + kBlk > lo || k < p.s.n_first));
+  }
+  return any;
+}
+
+// First and last active chunk of tile w (last = -1 when none).
+__device__ __forceinline__ void active_span(const FwdParams& p, const Item& it, int w, int* first,
+                                            int* last) {
+  int f = 0, l = it.chunks - 1;
+  while (l >= 0 && !tile_active(p, it, w, l)) --l;
+  while (f <= l && !tile_active(p, it, w, f)) ++f;
+  *first = f;
+  *last = l;
+}
+
+__device__ __forceinline__ void tmem_st_x16_nowait(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16};\n"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+        "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+        "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                      const __grid_constant__ CUtensorMap tm_v, const FwdParams p) {
+  using C = FwdCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* q_full = bars;                  // [2] TMA -> MMA
+  uint64_t* q_empty = q_full + 2;           // [2] last S of the tile done -> TMA
+  uint64_t* kv_full = q_empty + 2;          // [kSlots]
+  uint64_t* kv_empty = kv_full + C::kSlots; // [kSlots]
+  uint64_t* s_full = kv_empty + C::kSlots;  // [2] S of a chunk in TMEM
+  uint64_t* p_full = s_full + 2;            // [2] P written (128 arrivals)
+  uint64_t* o_done = p_full + 2;            // [2] PV of a chunk completed
+  uint64_t* o_empty = o_done + 2;           // [2] O read by the epilogue (128 arrivals)
+  uint64_t* drain_bar = o_empty + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int per = p.shared ? 1 : 2;  // slots of a chunk
+
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&q_full[w], 1);
+      mbar_init(&q_empty[w], 1);
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], 128);
+      mbar_init(&o_done[w], 1);
+      mbar_init(&o_empty[w], 128);
+    }
+    for (int s = 0; s < C::kSlots; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp < 4) {
+    set_max_regs_dec<kRegsAux>();
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int seq = 0;
+      int uses[2] = {0, 0};
+      bool ok = true;
+      auto load_slot = [&](const Item& it, const CUtensorMap* tm, int c) -> bool {
+        const int s = seq % C::kSlots;
+        if (!mbar_wait(&kv_empty[s], ((seq / C::kSlots) & 1) ^ 1, abort_flag, p.err,
+                       DSA_DEVERR_WIN_WAIT))
+          return false;
+        const int nb = chunk_blocks(it, c);
+        uint8_t* dst = smem + C::kOffKV + s * C::kTileBytes;
+        mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(nb * kBlk * D * 2));
+        for (int i = 0; i < nb; ++i) {
+          const int key = it.r.key(c * kChunkBlks + i);
+#pragma unroll
+          for (int half = 0; half < C::kHalves; ++half)
+            tma_load_4d(dst + half * kBoxBytes + i * kBlk * 128, tm, half * 64, key, it.kvh, it.b,
+                        &kv_full[s]);
+        }
+        ++seq;
+        return true;
+      };
+      for (int64_t item = blockIdx.x; ok && item < p.total_items; item += gridDim.x) {
+        const Item it = make_item(p, item);
+        for (int w = 0; w < 2 && ok; ++w) {
+          int f, l;
+          active_span(p, it, w, &f, &l);
+          if (l < 0) continue;
+          if (!mbar_wait(&q_empty[w], (uses[w] & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) {
+            ok = false;
+            break;
+          }
+          uint8_t* qs = smem + C::kOffQ + w * C::kTileBytes;
+          mbar_arrive_expect_tx(&q_full[w],
+                                static_cast<uint32_t>(p.tt * p.s.g * D * 2));
+#pragma unroll
+          for (int half = 0; half < C::kHalves; ++half)
+            tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0[w], it.b,
+                        &q_full[w]);
+          ++uses[w];
+        }
+        for (int c = 0; c < it.chunks && ok; ++c) {
+          ok = load_slot(it, &tm_k, c);
+          if (ok && !p.shared) ok = load_slot(it, &tm_v, c);
+        }
+      }
+      // copies in flight land before the CTA's shared memory goes away
+      for (int i = (seq > C::kSlots ? seq - C::kSlots : 0); i < seq; ++i)
+        mbar_drain(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
+      for (int w = 0; w < 2; ++w)
+        if (uses[w] > 0) mbar_drain(&q_full[w], (uses[w] - 1) & 1);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      constexpr uint32_t idesc_o = make_idesc<T>(128, D, 1);
+      const uint64_t dq = make_smem_desc(smem_u32(smem + C::kOffQ), 16u, 1024u, kLayoutSW128);
+      const uint64_t dk = make_smem_desc(smem_u32(smem + C::kOffKV), 16u, 1024u, kLayoutSW128);
+      const uint32_t hi = static_cast<uint32_t>(dk >> 32);
+      const uint32_t q_lo = static_cast<uint32_t>(dq);
+      const uint32_t k_lo = static_cast<uint32_t>(dk);
+      const uint32_t v_lo = static_cast<uint32_t>(make_smem_desc(
+          smem_u32(smem + C::kOffKV), static_cast<uint32_t>(kBoxBytes), 1024u, kLayoutSW128));
+      int seq = 0;             // slot number of the item's first chunk
+      int gs[2] = {0, 0};      // S products issued per tile
+      int gp[2] = {0, 0};      // PV products issued per tile
+      int uses[2] = {0, 0};    // items per tile
+      int first[2] = {0, 0}, last[2] = {-1, -1};
+      bool ok = true;
+      auto issue_s = [&](int w, int c, int slot, int nb) -> bool {
+        // the S/P columns are free once the tile's previous PV product completed
+        if (gp[w] >= 1 && !mbar_wait(&o_done[w], (gp[w] - 1) & 1, abort_flag, p.err,
+                                     DSA_DEVERR_WIN_WAIT))
+          return false;
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(w * 256);
+        const uint32_t qa = q_lo + static_cast<uint32_t>(w * (C::kTileBytes >> 4));
+        const uint32_t kb = k_lo + static_cast<uint32_t>(slot * (C::kTileBytes >> 4));
+        const uint32_t idesc_s = make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(nb * kBlk / 8) << 17);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t o = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+          umma_bf16(d, desc_from_words(qa + o, hi), desc_from_words(kb + o, hi), idesc_s,
+                    k > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[w]);
+        if (c == last[w]) umma_commit(&q_empty[w]);
+        ++gs[w];
+        return true;
+      };
+      auto issue_pv = [&](int w, int c, int slot, int nb) -> bool {
+        if (!mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) return false;
+        if (c == first[w] && uses[w] > 1 &&
+            !mbar_wait(&o_empty[w], (uses[w] - 2) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
+          return false;
+        tc_fence_after();
+        const uint32_t sp = tmem + static_cast<uint32_t>(w * 256);
+        const uint32_t vb = v_lo + static_cast<uint32_t>(slot * (C::kTileBytes >> 4));
+        for (int st = 0; st < nb * 2; ++st)  // 16 keys a step, 8 TMEM columns of P
+          umma_bf16_tmem_a(sp + 128u, sp + static_cast<uint32_t>(st * 8),
+                           desc_from_words(vb + static_cast<uint32_t>(st * 128), hi), idesc_o,
+                           (c > first[w] || st > 0) ? 1u : 0u);
+        umma_commit(&o_done[w]);
+        ++gp[w];
+        return true;
+      };
+      auto wait_slot = [&](int i) -> bool {
+        return mbar_wait(&kv_full[i % C::kSlots], (i / C::kSlots) & 1, abort_flag, p.err,
+                         DSA_DEVERR_WIN_WAIT);
+      };
+      // V rows at or past kv_len may hold anything, and 0 x NaN is NaN: they are
+      // cleared before the product that reads them (at most 31 rows of a block)
+      auto clear_tail = [&](const Item& it, int c, int slot, int nb) {
+        uint8_t* base = smem + C::kOffKV + slot * C::kTileBytes;
+        bool wrote = false;
+        for (int i = 0; i < nb; ++i) {
+          const int key = it.r.key(c * kChunkBlks + i);
+          for (int r = max(it.kv_len - key, 0); r < kBlk; ++r) {
+            wrote = true;
+            for (int x = 0; x < C::kHalves * 8; ++x)
+              st_shared_v4(smem_u32(base + (x >> 3) * kBoxBytes + (i * kBlk + r) * 128 + (x & 7) * 16),
+                           0u, 0u, 0u, 0u);
+          }
+        }
+        if (wrote) fence_proxy_async_smem();
+      };
+      for (int64_t item = blockIdx.x; ok && item < p.total_items; item += gridDim.x) {
+        const Item it = make_item(p, item);
+        for (int w = 0; w < 2 && ok; ++w) {
+          active_span(p, it, w, &first[w], &last[w]);
+          if (last[w] < 0) continue;
+          ok = mbar_wait(&q_full[w], uses[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+          ++uses[w];
+        }
+        if (!ok) break;
+        auto k_slot = [&](int c) { return seq + c * per; };
+        auto v_slot = [&](int c) { return seq + c * per + per - 1; };
+        if (it.chunks > 0) {
+          const int nb = chunk_blocks(it, 0);
+          ok = wait_slot(k_slot(0));
+          for (int w = 0; w < 2 && ok; ++w)
+            if (tile_active(p, it, w, 0)) ok = issue_s(w, 0, k_slot(0) % C::kSlots, nb);
+          if (ok && !p.shared) umma_commit(&kv_empty[k_slot(0) % C::kSlots]);
+        }
+        for (int c = 0; c < it.chunks && ok; ++c) {
+          const int nb = chunk_blocks(it, c);
+          const bool more = c + 1 < it.chunks;
+          const int nbn = more ? chunk_blocks(it, c + 1) : 0;
+          const int sv = v_slot(c) % C::kSlots;
+          ok = wait_slot(v_slot(c));
+          if (ok && p.s.kv_lens != nullptr) clear_tail(it, c, sv, nb);
+          if (ok && more) ok = wait_slot(k_slot(c + 1));
+          for (int w = 0; w < 2 && ok; ++w) {
+            if (tile_active(p, it, w, c)) ok = issue_pv(w, c, sv, nb);
+            if (ok && more && tile_active(p, it, w, c + 1))
+              ok = issue_s(w, c + 1, k_slot(c + 1) % C::kSlots, nbn);
+          }
+          if (!ok) break;
+          umma_commit(&kv_empty[sv]);
+          if (more && !p.shared) umma_commit(&kv_empty[k_slot(c + 1) % C::kSlots]);
+        }
+        seq += it.chunks * per;
+      }
+      umma_commit(drain_bar);
+      mbar_drain(drain_bar, 0);
+    }
+  }
+  } else {
+    // ------------------------------------------------------------ softmax
+    set_max_regs_inc<kRegsSoftmax>();
+    const int w = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const int tok = row / p.s.g;
+    const int head = row - tok * p.s.g;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t sp = tmem + lane_off + static_cast<uint32_t>(w * 256);
+    const uint32_t od = sp + 128u;
+    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
+    int gc = 0;  // chunks processed (all items)
+    bool ok = true;
+    for (int64_t item = blockIdx.x; item < p.total_items; item += gridDim.x) {
+      const Item it = make_item(p, item);
+      int first, last;
+      active_span(p, it, w, &first, &last);
+      const int t = it.t0[w] + tok;
+      const bool valid = tok < p.tt && t < it.t1[w];
+      // rows past the tile's tokens follow its last one: their values are not used
+      const int pos = min(t, it.t1[w] - 1) + p.s.n - p.s.m;
+      const int gh = it.kvh * p.s.g + head;
+      const bool has_sink = p.sink != nullptr && tok < p.tt;
+      const float sink2 = has_sink ? __ldg(p.sink + gh) * kLog2e : -INFINITY;
+      float m = sink2, l = 0.f;
+      for (int c = first; c <= last; ++c) {
+        if (!tile_active(p, it, w, c)) continue;
+        const int nb = chunk_blocks(it, c);
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[w], gc & 1, abort_flag, p.err,
+                                               DSA_DEVERR_WIN_WAIT));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t v[kChunkBlks][32];
+#pragma unroll
+        for (int i = 0; i < kChunkBlks; ++i)
+          if (i < nb) tmem_ld_32x32b_x32_nowait(sp + static_cast<uint32_t>(i * kBlk), v[i]);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < kChunkBlks; ++i) {
+          if (i < nb) {
+            tmem_wait_ld_dep(v[i]);
+            const uint32_t seen = seen_bits(p.s, it.r, c * kChunkBlks + i, pos, it.kv_len);
+            if (!__all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu)) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (!((seen >> k) & 1u)) v[i][k] = 0xFF800000u;
+            }
+            float a = fmaxf(__uint_as_float(v[i][0]), __uint_as_float(v[i][1]));
+            float b = fmaxf(__uint_as_float(v[i][2]), __uint_as_float(v[i][3]));
+#pragma unroll
+            for (int k = 4; k < 32; k += 4) {
+              a = fmax3(a, __uint_as_float(v[i][k]), __uint_as_float(v[i][k + 1]));
+              b = fmax3(b, __uint_as_float(v[i][k + 2]), __uint_as_float(v[i][k + 3]));
+            }
+            mx = fmax3(mx, a, b);
+          }
+        }
+        const float mz = mx * p.scale_log2;
+        if (c == first) {
+          m = fmaxf(m, mz);  // nothing accumulated yet
+        } else {
+          float factor = 1.f;
+          if (mz > m + kRescaleLog2) {  // m = -inf: l and O are 0
+            factor = ex2_approx(m - mz);
+            m = mz;
+            l *= factor;
+          }
+          if (__any_sync(0xFFFFFFFFu, factor != 1.f)) {
+            // this chunk's S was issued after the previous PV product completed
+#pragma unroll 1
+            for (int q = 0; q < D / 32; ++q) {
+              uint32_t ov[32];
+              tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) ov[k] = __float_as_uint(__uint_as_float(ov[k]) * factor);
+              tmem_st_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
+            }
+          }
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        const uint64_t neg2 = f2_pack(-ref, -ref);
+        uint64_t sum2[2] = {0ull, 0ull};
+#pragma unroll
+        for (int i = 0; i < kChunkBlks; ++i) {
+          if (i < nb) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float d0, d1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(v[i][2 * k]), __uint_as_float(v[i][2 * k + 1])),
+                               scale2, neg2),
+                        d0, d1);
+              const float e0 = ex2_approx(d0), e1 = ex2_approx(d1);
+              sum2[k & 1] = f2_add(sum2[k & 1], f2_pack(e0, e1));
+              pk[k] = T::pack(e0, e1);
+            }
+            tmem_st_x16_nowait(sp + static_cast<uint32_t>(i * 16), pk);
+          }
+        }
+        float a0, a1, b0, b1;
+        f2_unpack(sum2[0], a0, a1);
+        f2_unpack(sum2[1], b0, b1);
+        l += (a0 + a1) + (b0 + b1);
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[w]);
+        ++gc;
+      }
+      if (!ok) break;
+      // ---- epilogue: O / (l + sink term)
+      const float ref = m == -INFINITY ? 0.f : m;
+      const float total = l + (has_sink ? ex2_approx(sink2 - ref) : 0.f);
+      const float inv = total > 0.f ? 1.0f / total : (total == 0.f ? 0.f : total);
+      const int64_t orow = (static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + gh;
+      if (last >= 0) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&o_done[w], (gc - 1) & 1, abort_flag, p.err,
+                                               DSA_DEVERR_WIN_WAIT));
+        if (!ok) break;
+        tc_fence_after();
+      }
+#pragma unroll 1
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t ov[32];
+        if (last >= 0) {
+          tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) ov[k] = 0u;
+        }
+        if (valid) {
+          uint4* dst = reinterpret_cast<uint4*>(p.out + orow * D + q * 32);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              x[u] = T::pack(__uint_as_float(ov[8 * j + 2 * u]) * inv,
+                             __uint_as_float(ov[8 * j + 2 * u + 1]) * inv);
+            dst[j] = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        }
+      }
+      if (last >= 0) {
+        tc_fence_before();
+        mbar_arrive(&o_empty[w]);
+      }
+      if (valid && p.lse != nullptr) p.lse[orow] = (ref + log2f(total)) * kLn2;
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kTmemCols);
+  }
+}
+
+template <typename T, int D>
+int launch_fwd(const Tensors& x, const Shape& s, int64_t batch, float scale, const float* sink,
+               void* out, float* lse, cudaStream_t stream) {
+  using C = FwdCfg<D>;
+  DeviceInfo di;
+  int st = current_device_info(&di);
+  if (st != DSA_OK) return st;
+  if (di.max_smem_optin < C::kSmemBytes) return DSA_ERR_UNSUPPORTED;
+  unsigned int* err = nullptr;
+  st = device_error_word(&err);
+  if (st != DSA_OK) return st;
+  FwdParams p;
+  p.s = s;
+  p.tt = kRows / s.g;
+  p.tiles = (s.m + p.tt - 1) / p.tt;
+  p.items_per_head = (p.tiles + 1) / 2;
+  p.total_items = batch * s.hk * p.items_per_head;
+  p.scale_log2 = scale * kLog2e;
+  p.sink = sink;
+  p.out = static_cast<uint16_t*>(out);
+  p.lse = lse;
+  p.shared = x.v == x.k && same_strides(x.vs, x.ks);
+  p.err = err;
+  CUtensorMap tm_q, tm_k, tm_v;
+  st = map_rows_by_head(&tm_q, T::kFmt, x.q, x.qs, batch, s.m, s.h, D, s.g, p.tt);
+  if (st == DSA_OK) st = map_head_by_rows(&tm_k, T::kFmt, x.k, x.ks, batch, s.n, s.hk, D, kBlk);
+  if (st == DSA_OK) st = map_head_by_rows(&tm_v, T::kFmt, x.v, x.vs, batch, s.n, s.hk, D, kBlk);
+  if (st != DSA_OK) return st;
+  auto kernel = window_fwd_kernel<T, D>;
+  st = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), C::kSmemBytes);
+  if (st != DSA_OK) return st;
+  const int64_t grid = p.total_items < di.num_sms ? p.total_items : di.num_sms;
+  kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmemBytes, stream>>>(tm_q, tm_k, tm_v, p);
+  return cuda_status(cudaGetLastError());
+}
+
+}  // namespace win
+}  // namespace dsa
+
+extern "C" int dsa_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k,
+                                   const int64_t* k_strides, const void* v,
+                                   const int64_t* v_strides, const float* sink, const int* kv_lens,
+                                   void* out, float* lse, int dtype, int64_t batch, int64_t m,
+                                   int64_t n, int n_heads, int n_kv_heads, int head_dim,
+                                   int64_t window, int64_t n_first, float softmax_scale,
+                                   void* stream) {
+  using namespace dsa;
+  using namespace dsa::win;
+  Tensors x;
+  Shape s;
+  const int st = check_window_args(q, q_strides, k, k_strides, v, v_strides, kv_lens, dtype, batch,
+                                   m, n, n_heads, n_kv_heads, head_dim, window, n_first,
+                                   softmax_scale, &x, &s);
+  if (st != DSA_OK) return st;
+  if (batch == 0 || m == 0) return DSA_OK;
+  if (out == nullptr) return DSA_ERR_INVALID_ARGUMENT;
+  if (!aligned16(out)) return DSA_ERR_MISALIGNED;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if (head_dim == 128)
+    return dtype == DSA_DTYPE_BF16
+               ? launch_fwd<Bf16, 128>(x, s, batch, softmax_scale, sink, out, lse, cs)
+               : launch_fwd<Fp16, 128>(x, s, batch, softmax_scale, sink, out, lse, cs);
+  return dtype == DSA_DTYPE_BF16
+             ? launch_fwd<Bf16, 64>(x, s, batch, softmax_scale, sink, out, lse, cs)
+             : launch_fwd<Fp16, 64>(x, s, batch, softmax_scale, sink, out, lse, cs);
+}

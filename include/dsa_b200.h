@@ -43,7 +43,13 @@ typedef enum dsa_status {
 #define DSA_DEVERR_SA_WAIT 0x0001u     /* sparse attention pipeline wait timed out */
 #define DSA_DEVERR_IX_WAIT 0x0002u     /* indexer pipeline wait timed out */
 #define DSA_DEVERR_GEMM_WAIT 0x0004u   /* projection GEMM pipeline wait timed out */
+#define DSA_DEVERR_WIN_WAIT 0x0020u    /* windowed attention pipeline wait timed out */
+#define DSA_DEVERR_CACHE 0x0040u       /* a page number or length outside the paged cache */
 #define DSA_DEVERR_TOPK_RANGE 0x0010u  /* top-k selection found fewer keys than expected */
+
+/* 16-bit element types of the operators that take both. */
+#define DSA_DTYPE_BF16 0
+#define DSA_DTYPE_FP16 1
 
 /* Human-readable name of a dsa_status_t value (static storage). */
 const char* dsa_status_string(int status);
@@ -314,6 +320,37 @@ int dsa_chain_fwd(const void* x, const void* qr, const void* wq_b, const void* w
                   const void* kv, int n_kv, int attn_heads, int attn_head_dim,
                   const float* sink, float softmax_scale, void* out, void* workspace,
                   size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Attention with a sliding window and a few first tokens that stay visible.
+ *   q   [batch, m, n_heads, head_dim], out like q (contiguous)
+ *   k,v [batch, n, n_kv_heads, head_dim]; v may be k (one tensor for both)
+ * Query t stands at position p = t + n - m and sees key j when j <= p,
+ * j < kv_lens[b] (NULL: n) and (j > p - window or j < n_first). With s_j =
+ * softmax_scale q.k_j over the keys it sees (n_heads / n_kv_heads query heads
+ * share a kv head):
+ *   lse = log(sum_j e^s_j + e^sink[h]),  out = sum_j e^(s_j - lse) v_j
+ * (sink: [n_heads] fp32 logits or NULL). A row that sees no key and has no sink
+ * gets out = 0, lse = -inf. k and v rows at or past kv_lens[b] may hold
+ * anything. Products of the 16-bit operands are summed in fp32; the softmax
+ * runs in fp32; its weights are rounded to the operands' type for the second
+ * product and out once at the end.
+ * dtype: DSA_DTYPE_*, of q, k, v and out. q_strides, k_strides, v_strides:
+ * strides in elements of (batch, token, head), host arrays, NULL for
+ * contiguous; head_dim is contiguous. lse [batch, m, n_heads] fp32 or NULL.
+ * kv_lens: [batch] int32 on the device or NULL (values are clamped to [0, n]).
+ * Supported: head_dim 64 or 128, n_heads / n_kv_heads <= 128, softmax_scale >
+ * 0, m and n up to 2^28 (m > n leaves the first rows empty), strides multiples
+ * of 8 elements, pointers 16-byte aligned. No workspace. No counterpart in the
+ * reference, whose ModelArgs declares window_size
+ * (reference/task2_v0_ref.py:21-61) and holds no attention that uses it.
+ */
+int dsa_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k,
+                        const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                        const float* sink, const int* kv_lens, void* out, float* lse, int dtype,
+                        int64_t batch, int64_t m, int64_t n, int n_heads, int n_kv_heads,
+                        int head_dim, int64_t window, int64_t n_first, float softmax_scale,
+                        void* stream);
 
 #ifdef __cplusplus
 }
