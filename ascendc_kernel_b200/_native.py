@@ -71,6 +71,13 @@ SIGNATURES = {
     "dsa_window_attn_fwd": (_i32, [_c_void_p, _i64p, _c_void_p, _i64p, _c_void_p, _i64p,
                                    _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64,
                                    _i64, _i32, _i32, _i32, _i64, _i64, _f32, _c_void_p]),
+    "dsa_window_attn_bwd_workspace_bytes": (_size_t, [_i64, _i64, _i64, _i32, _i32, _i32, _i64,
+                                                      _i64, _i32]),
+    "dsa_window_attn_bwd": (_i32, [_c_void_p, _i64p, _c_void_p, _i64p, _c_void_p, _i64p,
+                                   _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64p,
+                                   _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64,
+                                   _i64, _i32, _i32, _i32, _i64, _i64, _f32, _c_void_p, _size_t,
+                                   _c_void_p]),
 }
 
 _LIB = None

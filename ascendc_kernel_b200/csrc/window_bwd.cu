@@ -1,0 +1,1219 @@
+// Attention with a sliding window and a few first tokens, backward, for sm_100a.
+//
+// With P_j = e^(s_j - lse) over the keys a row sees (window_common.cuh), D =
+// rowsum(dout * out) and dS_j = P_j (dout.v_j - D):
+//   dq = scale sum_j dS_j k_j      dk_j = scale sum_rows dS_j q      dv_j = sum_rows P_j dout
+//   dsink_h = -sum_rows e^(sink_h - lse) D       (v the same tensor as k: dk + dv in one)
+//
+// Deterministic without atomics, in up to five launches:
+//   window_stat_kernel  per row -lse log2(e) and -D, HBM bound (out and dout read once)
+//   window_dkv_kernel   a key tile stays, the rows that see it stream by (4 products)
+//   window_join_kernel  sums the fp32 parts of key tiles whose rows were split
+//   window_dq_kernel    a row tile stays, its keys stream by (3 products); S and dout V^T
+//                       are computed again, which costs 2 products of 7 and keeps dq out of
+//                       atomics, whose order would change results from run to run
+//   window_dsink_*      the rows' sink terms summed in a fixed order
+// P and dS are rounded to the operands' 16-bit type for the products that sum
+// over them (relative 2^-9 for bf16, the size of the gradients' own rounding);
+// every sum is fp32. D comes from the rounded out; the sink's gradient, an fp32
+// output, uses the unrounded D = sum_j P_j (dout.v_j) that the dq kernel sees.
+#include "host_util.h"
+#include "window_common.cuh"
+#include "window_host.h"
+
+namespace dsa {
+namespace win {
+
+constexpr int kBwdThreads = 384;
+constexpr int kBwdRegsAux = 88;       // 128 x 88 + 256 x 208 = 384 x 168 at launch
+constexpr int kBwdRegsSoftmax = 208;
+constexpr uint32_t kBwdTmemCols = 512;
+constexpr int kCB = 2;                // key blocks of a chunk (dq), 64 keys
+constexpr int kStream = 64;           // rows of a streamed tile (dkv)
+constexpr int kHalfBox = kStream * 128;  // one [64 rows x 64 columns] SW128 box
+
+// ------------------------------------------------------------------ row statistics
+// stat[row] = (-lse log2 e, -D); D / 8 threads a row, 16-byte loads.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) window_stat_kernel(const uint16_t* out, const uint16_t* dout,
+                                                          Strides ds, const float* lse, float2* stat,
+                                                          int64_t rows, int m, int h) {
+  constexpr int kLanes = D / 8;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  const int x = threadIdx.x % kLanes;
+  float sum = 0.f;
+  if (row < rows) {
+    const int64_t bt = row / h;
+    const int head = static_cast<int>(row - bt * h);
+    const int64_t b = bt / m;
+    const int64_t t = bt - b * m;
+    const uint4 a = *reinterpret_cast<const uint4*>(out + row * D + x * 8);
+    const uint4 g = *reinterpret_cast<const uint4*>(dout + b * ds.b + t * ds.t + head * ds.h + x * 8);
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      sum = fmaf(T::lo(aw[i]), T::lo(gw[i]), sum);
+      sum = fmaf(T::hi(aw[i]), T::hi(gw[i]), sum);
+    }
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if (row < rows && x == 0) {
+    const float l = lse[row];
+    // a row that sees nothing has no weights: 2^(s - inf) = 0
+    stat[row] = make_float2(l == -INFINITY ? -INFINITY : -l * kLog2e, -sum);
+  }
+}
+
+// ------------------------------------------------------------------ dk, dv
+template <int D>
+struct DkvCfg {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTileBytes = kRows * D * 2;
+  static constexpr int kStageBytes = 2 * kStream * D * 2;  // q rows, dout rows
+  static constexpr int kStages = 4;
+  static constexpr int kOffK = 0;
+  static constexpr int kOffV = kTileBytes;
+  static constexpr int kOffS = 2 * kTileBytes;
+  static constexpr int kOffStat = kOffS + kStages * kStageBytes;  // [stage][2][64] f32
+  static constexpr int kOffBar = kOffStat + kStages * 2 * kStream * 4;
+  static constexpr int kNumBars = 2 + 2 * kStages + 2 + 2 + 2 + 1 + 1 + 1;
+  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
+};
+
+struct DkvParams {
+  Shape s;
+  int gb, hb, tt;        // heads and tokens of a streamed tile, head parts of a group
+  int key_tiles;         // per (batch, kv head)
+  int first_tiles;       // of them, those with first tokens (every later row sees them)
+  int split_first, split;  // units of a key tile
+  int units_per_head;
+  int64_t units;
+  float scale, scale_log2;
+  const float2* stat;    // [batch, m, h]
+  uint16_t* dk;          // [batch, n, hk, D]
+  uint16_t* dv;          // null: dk receives dk + dv
+  float* parts;          // [unit][dv ? 2 : 1][128][D] of the key tiles with several units
+  unsigned int* err;
+};
+
+// Tokens [ta, tb) that see a key of tile kt (an upper bound when kv_lens is short).
+__host__ __device__ __forceinline__ void dkv_tokens(const Shape& s, int kt, int* ta, int* tb) {
+  const int off = s.n - s.m;
+  const int k0 = kt * kRows;
+  const int64_t top = k0 < s.n_first ? s.n : static_cast<int64_t>(k0) + kRows - 1 + s.window;
+  const int pe = top < s.n ? static_cast<int>(top) : s.n;  // positions [k0, pe)
+  *ta = k0 - off > 0 ? k0 - off : 0;
+  *tb = pe - off > *ta ? pe - off : *ta;
+}
+
+struct Unit {
+  int b, kvh, kv_len;
+  int kt, part, parts;
+  int ta, tb;      // tokens of the key tile
+  int r0, r1;      // streamed tiles of the unit
+};
+
+__device__ __forceinline__ Unit make_unit(const DkvParams& p, int64_t unit) {
+  Unit u;
+  const int64_t bh = unit / p.units_per_head;
+  int x = static_cast<int>(unit - bh * p.units_per_head);
+  u.b = static_cast<int>(bh / p.s.hk);
+  u.kvh = static_cast<int>(bh - static_cast<int64_t>(u.b) * p.s.hk);
+  u.kv_len = kv_len_of(p.s, u.b);
+  const int heavy = p.first_tiles * p.split_first;
+  if (x < heavy) {
+    u.parts = p.split_first;
+    u.kt = x / p.split_first;
+    u.part = x - u.kt * p.split_first;
+  } else {
+    x -= heavy;
+    u.parts = p.split;
+    u.kt = x / p.split;
+    u.part = x - u.kt * p.split;
+    u.kt += p.first_tiles;
+  }
+  dkv_tokens(p.s, u.kt, &u.ta, &u.tb);
+  if (u.kt * kRows >= u.kv_len) u.tb = u.ta;
+  const int64_t tiles = static_cast<int64_t>((u.tb - u.ta + p.tt - 1) / p.tt) * p.hb;
+  u.r0 = static_cast<int>(tiles * u.part / u.parts);
+  u.r1 = static_cast<int>(tiles * (u.part + 1) / u.parts);
+  return u;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                      const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                      const DkvParams p) {
+  using C = DkvCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* kv_full = bars;
+  uint64_t* kv_empty = bars + 1;
+  uint64_t* st_full = bars + 2;                // [kStages] rows and statistics (1 + 32 arrivals)
+  uint64_t* st_empty = st_full + C::kStages;   // [kStages] products done and statistics read
+  uint64_t* s_full = st_empty + C::kStages;    // [2] S^T and dP^T of a tile in TMEM
+  uint64_t* p_full = s_full + 2;               // [2] P^T and dS^T written (128 arrivals)
+  uint64_t* o_done = p_full + 2;               // [2] products of a tile completed
+  uint64_t* acc_full = o_done + 2;             // all products of the unit completed
+  uint64_t* acc_empty = acc_full + 1;          // accumulators read (256 arrivals)
+  uint64_t* drain_bar = acc_empty + 1;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+  float* stat_s = reinterpret_cast<float*>(smem + C::kOffStat);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    mbar_init(kv_empty, 1);
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(&st_full[s], 33);
+      mbar_init(&st_empty[s], 1);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], 128);
+      mbar_init(&o_done[w], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 256);
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_do);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  // rows that no copy writes (a group size that does not fill the tile) take part
+  // in the products over rows with weight 0: they must be finite
+  for (int i = threadIdx.x; i < C::kStages * C::kStageBytes / 16; i += kBwdThreads)
+    st_shared_v4(smem_u32(smem + C::kOffS + i * 16), 0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, kBwdTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+  const int off = p.s.n - p.s.m;
+
+  // first token and first head (in the group) of streamed tile r; the second head
+  // part of a group of more than 64 ends at the group's last head, its first `dup`
+  // rows repeat heads of the first part and carry weight 0
+  auto tile_token = [&](const Unit& u, int r) { return u.ta + (r / p.hb) * p.tt; };
+  auto tile_head = [&](int r) { return (r % p.hb) == 0 ? 0 : p.s.g - p.gb; };
+
+  if (warp < 4) {
+    set_max_regs_dec<kBwdRegsAux>();
+    if (warp == 0) {
+      // ---------------------------------------------------------- producer
+      int gs = 0, uses = 0;
+      bool ok = true;
+      for (int64_t x = blockIdx.x; ok && x < p.units; x += gridDim.x) {
+        const Unit u = make_unit(p, x);
+        if (u.r1 <= u.r0) continue;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(kv_empty, (uses & 1) ^ 1, abort_flag, p.err,
+                                               DSA_DEVERR_WIN_WAIT));
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(kv_full, 2 * C::kTileBytes);
+#pragma unroll
+          for (int half = 0; half < C::kHalves; ++half) {
+            tma_load_4d(smem + C::kOffK + half * kBoxBytes, &tm_k, half * 64, u.kt * kRows, u.kvh,
+                        u.b, kv_full);
+            tma_load_4d(smem + C::kOffV + half * kBoxBytes, &tm_v, half * 64, u.kt * kRows, u.kvh,
+                        u.b, kv_full);
+          }
+        }
+        ++uses;
+        for (int r = u.r0; r < u.r1; ++r, ++gs) {
+          const int s = gs % C::kStages;
+          const int t0 = tile_token(u, r), h0 = u.kvh * p.s.g + tile_head(r);
+          // the rows' statistics, fetched while the stage is still in use
+          float2 st[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int row = lane + 32 * i;
+            const int tok = row / p.gb;
+            st[i] = make_float2(-INFINITY, 0.f);
+            if (tok < p.tt && t0 + tok < p.s.m)
+              st[i] = __ldg(p.stat + (static_cast<int64_t>(u.b) * p.s.m + t0 + tok) * p.s.h + h0 +
+                            (row - tok * p.gb));
+          }
+          ok = __all_sync(0xFFFFFFFFu, mbar_wait(&st_empty[s], ((gs / C::kStages) & 1) ^ 1, abort_flag,
+                                                 p.err, DSA_DEVERR_WIN_WAIT));
+          if (!ok) break;
+          if (lane == 0) {
+            uint8_t* dst = smem + C::kOffS + s * C::kStageBytes;
+            mbar_arrive_expect_tx(&st_full[s], static_cast<uint32_t>(2 * p.gb * p.tt * D * 2));
+#pragma unroll
+            for (int half = 0; half < C::kHalves; ++half) {
+              tma_load_4d(dst + half * kHalfBox, &tm_q, half * 64, h0, t0, u.b, &st_full[s]);
+              tma_load_4d(dst + C::kStageBytes / 2 + half * kHalfBox, &tm_do, half * 64, h0, t0, u.b,
+                          &st_full[s]);
+            }
+          }
+          float* ss = stat_s + s * 2 * kStream;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            ss[lane + 32 * i] = st[i].x;
+            ss[kStream + lane + 32 * i] = st[i].y;
+          }
+          mbar_arrive(&st_full[s]);
+        }
+      }
+      // copies in flight land before the CTA's shared memory goes away
+      if (uses > 0) mbar_drain(kv_full, (uses - 1) & 1);
+      for (int i = (gs > C::kStages ? gs - C::kStages : 0); i < gs; ++i)
+        mbar_drain(&st_full[i % C::kStages], (i / C::kStages) & 1);
+    } else if (warp == 1 && lane == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      constexpr uint32_t idesc_s = make_idesc<T>(128, kStream, 0);
+      constexpr uint32_t idesc_o = make_idesc<T>(128, D, 1);
+      const uint64_t dk0 = make_smem_desc(smem_u32(smem + C::kOffK), 16u, 1024u, kLayoutSW128);
+      const uint32_t hi = static_cast<uint32_t>(dk0 >> 32);
+      const uint32_t k_lo = static_cast<uint32_t>(dk0);
+      const uint32_t v_lo = k_lo + static_cast<uint32_t>((C::kOffV - C::kOffK) >> 4);
+      const uint32_t s_lo = k_lo + static_cast<uint32_t>((C::kOffS - C::kOffK) >> 4);
+      const uint32_t mn_lo = static_cast<uint32_t>(make_smem_desc(
+          smem_u32(smem + C::kOffS), static_cast<uint32_t>(kHalfBox), 1024u, kLayoutSW128));
+      int gs = 0, uses = 0;
+      int gp[2] = {0, 0};
+      bool ok = true;
+      auto issue_s = [&](int i) -> bool {  // i: global tile number; buffer i & 1
+        const int w = i & 1, s = i % C::kStages;
+        if (!mbar_wait(&st_full[s], (i / C::kStages) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
+          return false;
+        if (gp[w] >= 1 && !mbar_wait(&o_done[w], (gp[w] - 1) & 1, abort_flag, p.err,
+                                     DSA_DEVERR_WIN_WAIT))
+          return false;
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(w * 128);
+        const uint32_t qb = s_lo + static_cast<uint32_t>(s * (C::kStageBytes >> 4));
+        const uint32_t ob = qb + static_cast<uint32_t>(C::kStageBytes >> 5);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+          const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
+          umma_bf16(d, desc_from_words(k_lo + ao, hi), desc_from_words(qb + bo, hi), idesc_s,
+                    k > 0 ? 1u : 0u);
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+          const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
+          umma_bf16(d + 64u, desc_from_words(v_lo + ao, hi), desc_from_words(ob + bo, hi), idesc_s,
+                    k > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[w]);
+        return true;
+      };
+      auto issue_o = [&](int i, bool fresh) -> bool {
+        const int w = i & 1, s = i % C::kStages;
+        if (!mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) return false;
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(w * 128);
+        const uint32_t qb = mn_lo + static_cast<uint32_t>(s * (C::kStageBytes >> 4));
+        const uint32_t ob = qb + static_cast<uint32_t>(C::kStageBytes >> 5);
+#pragma unroll
+        for (int st = 0; st < kStream / 16; ++st) {
+          const uint32_t acc = (fresh && st == 0) ? 0u : 1u;
+          const uint32_t bo = static_cast<uint32_t>(st * 128);
+          umma_bf16_tmem_a(tmem + 384u, d + static_cast<uint32_t>(st * 8), desc_from_words(ob + bo, hi),
+                           idesc_o, acc);
+          umma_bf16_tmem_a(tmem + 256u, d + 64u + static_cast<uint32_t>(st * 8),
+                           desc_from_words(qb + bo, hi), idesc_o, acc);
+        }
+        umma_commit(&o_done[w]);
+        umma_commit(&st_empty[s]);
+        ++gp[w];
+        return true;
+      };
+      for (int64_t x = blockIdx.x; ok && x < p.units; x += gridDim.x) {
+        const Unit u = make_unit(p, x);
+        const int nt = u.r1 - u.r0;
+        if (nt <= 0) continue;
+        ok = mbar_wait(kv_full, uses & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+        ok = ok && issue_s(gs) && (nt < 2 || issue_s(gs + 1));
+        if (ok && nt <= 2) umma_commit(kv_empty);
+        ok = ok && (uses == 0 || mbar_wait(acc_empty, (uses - 1) & 1, abort_flag, p.err,
+                                           DSA_DEVERR_WIN_WAIT));
+        for (int i = 0; i < nt && ok; ++i) {
+          ok = issue_o(gs + i, i == 0);
+          if (ok && i + 2 < nt) {
+            ok = issue_s(gs + i + 2);
+            if (ok && i + 3 == nt) umma_commit(kv_empty);  // the key tile is no longer read
+          }
+        }
+        if (!ok) break;
+        umma_commit(acc_full);
+        gs += nt;
+        ++uses;
+      }
+      umma_commit(drain_bar);
+      mbar_drain(drain_bar, 0);
+    }
+  } else {
+    // ------------------------------------------------------------ P^T and dS^T
+    set_max_regs_inc<kBwdRegsSoftmax>();
+    const int w = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;  // key of the tile
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t sp = tmem + lane_off + static_cast<uint32_t>(w * 128);
+    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
+    int gs = 0, gw = 0, uses = 0;
+    bool ok = true;
+    for (int64_t x = blockIdx.x; x < p.units; x += gridDim.x) {
+      const Unit u = make_unit(p, x);
+      const int nt = max(u.r1 - u.r0, 0);
+      const int key = u.kt * kRows + row;
+      // positions [key, end) see this key
+      const int64_t far = static_cast<int64_t>(key) + p.s.window;
+      int end = p.s.n;
+      if (key >= p.s.n_first && far < end) end = static_cast<int>(far);
+      if (key >= u.kv_len) end = key;
+      for (int i = 0; i < nt; ++i) {
+        if (((gs + i) & 1) != w) continue;
+        const int s = (gs + i) % C::kStages;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[w], gw & 1, abort_flag, p.err,
+                                               DSA_DEVERR_WIN_WAIT));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sv[2][32], dv[2][32];
+        tmem_ld_32x32b_x32_nowait(sp, sv[0]);
+        tmem_ld_32x32b_x32_nowait(sp + 64u, dv[0]);
+        tmem_ld_32x32b_x32_nowait(sp + 32u, sv[1]);
+        tmem_ld_32x32b_x32_nowait(sp + 96u, dv[1]);
+        // the columns (rows of the streamed tile) that see this key: one range,
+        // since rows are token-major
+        const int r = u.r0 + i;
+        const int p0 = tile_token(u, r) + off;
+        const int tok_a = min(max(key - p0, 0), p.tt);
+        const int tok_b = min(max(end - p0, 0), p.tt);
+        const int dup = (r % p.hb) == 0 ? 0 : p.hb * p.gb - p.s.g;
+        const int ca = max(tok_a * p.gb, dup), cb = tok_b * p.gb;
+        const float4* stat4 = reinterpret_cast<const float4*>(stat_s + s * 2 * kStream);
+        // the statistics were written with ordinary stores: their barrier is waited
+        // for here too (it completed before this tile's products were issued)
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&st_full[s], ((gs + i) / C::kStages) & 1, abort_flag,
+                                               p.err, DSA_DEVERR_WIN_WAIT));
+        if (!ok) break;
+        tmem_wait_ld_dep(sv[0]);
+        tmem_wait_ld_dep(dv[0]);
+        tmem_wait_ld_dep(sv[1]);
+        tmem_wait_ld_dep(dv[1]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const uint32_t seen = bits_between(ca - 32 * q, cb - 32 * q);
+          const bool all = __all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu);
+          uint32_t pk[16], dk[16];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float4 nl = stat4[q * 8 + k], nd = stat4[16 + q * 8 + k];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int c = 4 * k + 2 * e;
+              const uint64_t l2 = e ? f2_pack(nl.z, nl.w) : f2_pack(nl.x, nl.y);
+              const uint64_t d2 = e ? f2_pack(nd.z, nd.w) : f2_pack(nd.x, nd.y);
+              float z0, z1, g0, g1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[q][c]), __uint_as_float(sv[q][c + 1])),
+                               scale2, l2),
+                        z0, z1);
+              const float e0 = ex2_approx(z0), e1 = ex2_approx(z1);
+              f2_unpack(f2_mul(f2_pack(e0, e1),
+                               f2_add(f2_pack(__uint_as_float(dv[q][c]),
+                                              __uint_as_float(dv[q][c + 1])),
+                                      d2)),
+                        g0, g1);
+              pk[c >> 1] = T::pack(e0, e1);
+              dk[c >> 1] = T::pack(g0, g1);
+            }
+          }
+          if (!all) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const uint32_t two = (seen >> (2 * k)) & 3u;
+              const uint32_t keep = (two & 1u ? 0x0000FFFFu : 0u) | (two & 2u ? 0xFFFF0000u : 0u);
+              pk[k] &= keep;
+              dk[k] &= keep;
+            }
+          }
+          tmem_st_x16_nowait(sp + static_cast<uint32_t>(q * 16), pk);
+          tmem_st_x16_nowait(sp + 64u + static_cast<uint32_t>(q * 16), dk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[w]);
+        ++gw;
+      }
+      if (!ok) break;
+      gs += nt;
+      // ---- epilogue: warpgroup 0 the first half of the columns, 1 the second
+      if (nt > 0) {
+        ok = __all_sync(0xFFFFFFFFu,
+                        mbar_wait(acc_full, uses & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+        if (!ok) break;
+        tc_fence_after();
+        ++uses;
+      }
+      const bool live = nt > 0 && key < u.kv_len;
+      const int c0 = w * (D / 2);
+#pragma unroll 1
+      for (int q = 0; q < D / 64; ++q) {
+        uint32_t a[32], b[32];
+        if (nt > 0) {
+          tmem_ld_32x32b_x32(tmem + lane_off + 256u + static_cast<uint32_t>(c0 + q * 32), a);
+          tmem_ld_32x32b_x32(tmem + lane_off + 384u + static_cast<uint32_t>(c0 + q * 32), b);
+        }
+        float fk[32], fv[32];
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          fk[k] = live ? __uint_as_float(a[k]) * p.scale : 0.f;
+          fv[k] = live ? __uint_as_float(b[k]) : 0.f;
+          if (p.dv == nullptr) fk[k] += fv[k];
+        }
+        if (u.parts > 1) {
+          const int kinds = p.dv == nullptr ? 1 : 2;
+          float* dst = p.parts + ((x * kinds) * kRows + row) * D + c0 + q * 32;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            reinterpret_cast<float4*>(dst)[k] =
+                make_float4(fk[4 * k], fk[4 * k + 1], fk[4 * k + 2], fk[4 * k + 3]);
+            if (kinds == 2)
+              reinterpret_cast<float4*>(dst + kRows * D)[k] =
+                  make_float4(fv[4 * k], fv[4 * k + 1], fv[4 * k + 2], fv[4 * k + 3]);
+          }
+        } else if (key < p.s.n) {
+          const int64_t at =
+              ((static_cast<int64_t>(u.b) * p.s.n + key) * p.s.hk + u.kvh) * D + c0 + q * 32;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            reinterpret_cast<uint4*>(p.dk + at)[k] =
+                make_uint4(T::pack(fk[8 * k], fk[8 * k + 1]), T::pack(fk[8 * k + 2], fk[8 * k + 3]),
+                           T::pack(fk[8 * k + 4], fk[8 * k + 5]), T::pack(fk[8 * k + 6], fk[8 * k + 7]));
+            if (p.dv != nullptr)
+              reinterpret_cast<uint4*>(p.dv + at)[k] = make_uint4(
+                  T::pack(fv[8 * k], fv[8 * k + 1]), T::pack(fv[8 * k + 2], fv[8 * k + 3]),
+                  T::pack(fv[8 * k + 4], fv[8 * k + 5]), T::pack(fv[8 * k + 6], fv[8 * k + 7]));
+          }
+        }
+      }
+      if (nt > 0) {
+        tc_fence_before();
+        mbar_arrive(acc_empty);
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kBwdTmemCols);
+  }
+}
+
+// Sums the parts of the key tiles with several units, in the order of the parts;
+// a thread four columns of a key.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) window_join_kernel(const DkvParams p, int64_t batch) {
+  const bool two = p.split > 1;  // all key tiles have parts, else only the first ones
+  const int tiles = two ? p.key_tiles : p.first_tiles;
+  const int kinds = p.dv == nullptr ? 1 : 2;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  const int col = static_cast<int>(i % (D / 4)) * 4;
+  int64_t x = i / (D / 4);
+  const int row = static_cast<int>(x % kRows);
+  x /= kRows;
+  const int kind = static_cast<int>(x % kinds);
+  x /= kinds;
+  const int kt = static_cast<int>(x % tiles);
+  const int64_t bh = x / tiles;
+  const int key = kt * kRows + row;
+  if (bh >= batch * p.s.hk || key >= p.s.n) return;
+  const bool first = kt < p.first_tiles;
+  const int parts = first ? p.split_first : p.split;
+  if (parts <= 1) return;
+  const int64_t unit = bh * p.units_per_head +
+                       (first ? static_cast<int64_t>(kt) * p.split_first
+                              : static_cast<int64_t>(p.first_tiles) * p.split_first +
+                                    static_cast<int64_t>(kt - p.first_tiles) * p.split);
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < parts; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(
+        p.parts + (((unit + s) * kinds + kind) * kRows + row) * D + col);
+    sum.x += v.x;
+    sum.y += v.y;
+    sum.z += v.z;
+    sum.w += v.w;
+  }
+  const int64_t b = bh / p.s.hk;
+  uint16_t* out = kind ? p.dv : p.dk;
+  *reinterpret_cast<uint2*>(out + ((b * p.s.n + key) * p.s.hk + (bh - b * p.s.hk)) * D + col) =
+      make_uint2(T::pack(sum.x, sum.y), T::pack(sum.z, sum.w));
+}
+
+// ------------------------------------------------------------------ dq
+template <int D>
+struct DqCfg {
+  static constexpr int kHalves = D / 64;
+  static constexpr int kTileBytes = kRows * D * 2;
+  static constexpr int kSlotBytes = kCB * kBlk * D * 2;
+  static constexpr int kSlots = D == 128 ? 6 : 8;
+  static constexpr int kOffQ = 0;                      // [2 tiles] q, dout
+  static constexpr int kOffKV = 4 * kTileBytes;
+  static constexpr int kOffBar = kOffKV + kSlots * kSlotBytes;
+  static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 2 + 2 + 2 + 2 + 1;
+  static constexpr int kOffMisc = kOffBar + kNumBars * 8;
+  static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
+};
+
+struct DqParams {
+  Shape s;
+  TileGrid grid;
+  float scale, scale_log2;
+  const float2* stat;   // [batch, m, h]
+  const float* sink;    // [h] or null
+  uint16_t* dq;         // [batch, m, h, D]
+  float* sink_rows;     // [batch, m, h]: e^(sink - lse) sum_j P_j dP_j, with sink
+  int shared;
+  unsigned int* err;
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+    window_dq_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
+                     const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                     const DqParams p) {
+  using C = DqCfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
+  uint64_t* q_full = bars;                  // [2] TMA -> MMA
+  uint64_t* q_empty = q_full + 2;           // [2] last products of the tile's rows done -> TMA
+  uint64_t* kv_full = q_empty + 2;          // [kSlots]
+  uint64_t* kv_empty = kv_full + C::kSlots; // [kSlots]
+  uint64_t* s_full = kv_empty + C::kSlots;  // [2] S and dP of a chunk in TMEM
+  uint64_t* p_full = s_full + 2;            // [2] dS written (128 arrivals)
+  uint64_t* o_done = p_full + 2;            // [2] dq product of a chunk completed
+  uint64_t* o_empty = o_done + 2;           // [2] dq read by the epilogue (128 arrivals)
+  uint64_t* drain_bar = o_empty + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int per = p.shared ? 1 : 2;
+
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&q_full[w], 1);
+      mbar_init(&q_empty[w], 1);
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_full[w], 128);
+      mbar_init(&o_done[w], 1);
+      mbar_init(&o_empty[w], 128);
+    }
+    for (int s = 0; s < C::kSlots; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_q);
+    tma_prefetch_desc(&tm_do);
+    tma_prefetch_desc(&tm_k);
+    tma_prefetch_desc(&tm_v);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_holder, kBwdTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;
+
+  if (warp < 4) {
+    set_max_regs_dec<kBwdRegsAux>();
+    if (warp == 0 && lane == 0) {
+      // ---------------------------------------------------------- producer
+      int seq = 0;
+      int uses[2] = {0, 0};
+      bool ok = true;
+      auto load_slot = [&](const Item& it, const CUtensorMap* tm, int c) -> bool {
+        const int s = seq % C::kSlots;
+        if (!mbar_wait(&kv_empty[s], ((seq / C::kSlots) & 1) ^ 1, abort_flag, p.err,
+                       DSA_DEVERR_WIN_WAIT))
+          return false;
+        const int nb = it.blocks<kCB>(c);
+        uint8_t* dst = smem + C::kOffKV + s * C::kSlotBytes;
+        mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(nb * kBlk * D * 2));
+        for (int i = 0; i < nb; ++i) {
+          const int key = it.r.key(c * kCB + i);
+#pragma unroll
+          for (int half = 0; half < C::kHalves; ++half)
+            tma_load_4d(dst + half * kHalfBox + i * kBlk * 128, tm, half * 64, key, it.kvh, it.b,
+                        &kv_full[s]);
+        }
+        ++seq;
+        return true;
+      };
+      for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
+        const Item it = make_item(p.s, p.grid, item);
+        for (int w = 0; w < 2 && ok; ++w) {
+          int f, l;
+          it.span<kCB>(p.s, w, &f, &l);
+          if (l < 0) continue;
+          if (!mbar_wait(&q_empty[w], (uses[w] & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) {
+            ok = false;
+            break;
+          }
+          uint8_t* qs = smem + C::kOffQ + 2 * w * C::kTileBytes;
+          mbar_arrive_expect_tx(&q_full[w], static_cast<uint32_t>(2 * p.grid.tt * p.s.g * D * 2));
+#pragma unroll
+          for (int half = 0; half < C::kHalves; ++half) {
+            tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0[w], it.b,
+                        &q_full[w]);
+            tma_load_4d(qs + C::kTileBytes + half * kBoxBytes, &tm_do, half * 64, it.kvh * p.s.g,
+                        it.t0[w], it.b, &q_full[w]);
+          }
+          ++uses[w];
+        }
+        const int chunks = it.chunks<kCB>();
+        for (int c = 0; c < chunks && ok; ++c) {
+          ok = load_slot(it, &tm_k, c);
+          if (ok && !p.shared) ok = load_slot(it, &tm_v, c);
+        }
+      }
+      for (int i = (seq > C::kSlots ? seq - C::kSlots : 0); i < seq; ++i)
+        mbar_drain(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
+      for (int w = 0; w < 2; ++w)
+        if (uses[w] > 0) mbar_drain(&q_full[w], (uses[w] - 1) & 1);
+    } else if (warp == 1 && lane == 0) {
+      // ---------------------------------------------------------- MMA issuer
+      constexpr uint32_t idesc_o = make_idesc<T>(128, D, 1);
+      const uint64_t dq0 = make_smem_desc(smem_u32(smem + C::kOffQ), 16u, 1024u, kLayoutSW128);
+      const uint32_t hi = static_cast<uint32_t>(dq0 >> 32);
+      const uint32_t q_lo = static_cast<uint32_t>(dq0);
+      const uint32_t k_lo = q_lo + static_cast<uint32_t>((C::kOffKV - C::kOffQ) >> 4);
+      const uint32_t mn_lo = static_cast<uint32_t>(make_smem_desc(
+          smem_u32(smem + C::kOffKV), static_cast<uint32_t>(kHalfBox), 1024u, kLayoutSW128));
+      int seq = 0;
+      int gp[2] = {0, 0};
+      int uses[2] = {0, 0};
+      int first[2] = {0, 0}, last[2] = {-1, -1};
+      bool ok = true;
+      auto issue_s = [&](int w, int c, int ks, int vs, int nb) -> bool {
+        if (gp[w] >= 1 && !mbar_wait(&o_done[w], (gp[w] - 1) & 1, abort_flag, p.err,
+                                     DSA_DEVERR_WIN_WAIT))
+          return false;
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(w * 256);
+        const uint32_t qa = q_lo + static_cast<uint32_t>(2 * w * (C::kTileBytes >> 4));
+        const uint32_t oa = qa + static_cast<uint32_t>(C::kTileBytes >> 4);
+        const uint32_t kb = k_lo + static_cast<uint32_t>(ks * (C::kSlotBytes >> 4));
+        const uint32_t vb = k_lo + static_cast<uint32_t>(vs * (C::kSlotBytes >> 4));
+        const uint32_t idesc_s =
+            make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(nb * kBlk / 8) << 17);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+          const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
+          umma_bf16(d, desc_from_words(qa + ao, hi), desc_from_words(kb + bo, hi), idesc_s,
+                    k > 0 ? 1u : 0u);
+        }
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+          const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
+          umma_bf16(d + 64u, desc_from_words(oa + ao, hi), desc_from_words(vb + bo, hi), idesc_s,
+                    k > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[w]);
+        if (c == last[w]) umma_commit(&q_empty[w]);
+        return true;
+      };
+      auto issue_o = [&](int w, int c, int slot, int nb) -> bool {
+        if (!mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) return false;
+        if (c == first[w] && uses[w] > 1 &&
+            !mbar_wait(&o_empty[w], (uses[w] - 2) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
+          return false;
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(w * 256);
+        const uint32_t kb = mn_lo + static_cast<uint32_t>(slot * (C::kSlotBytes >> 4));
+        for (int st = 0; st < nb * 2; ++st)
+          umma_bf16_tmem_a(d + 128u, d + static_cast<uint32_t>(st * 8),
+                           desc_from_words(kb + static_cast<uint32_t>(st * 128), hi), idesc_o,
+                           (c > first[w] || st > 0) ? 1u : 0u);
+        umma_commit(&o_done[w]);
+        ++gp[w];
+        return true;
+      };
+      auto wait_slot = [&](int i) -> bool {
+        return mbar_wait(&kv_full[i % C::kSlots], (i / C::kSlots) & 1, abort_flag, p.err,
+                         DSA_DEVERR_WIN_WAIT);
+      };
+      // K rows at or past kv_len may hold anything, and 0 x NaN is NaN: cleared before
+      // the product that sums over them
+      auto clear_tail = [&](const Item& it, int c, int slot, int nb) {
+        uint8_t* base = smem + C::kOffKV + slot * C::kSlotBytes;
+        bool wrote = false;
+        for (int i = 0; i < nb; ++i) {
+          const int key = it.r.key(c * kCB + i);
+          for (int r = max(it.kv_len - key, 0); r < kBlk; ++r) {
+            wrote = true;
+            for (int x = 0; x < C::kHalves * 8; ++x)
+              st_shared_v4(smem_u32(base + (x >> 3) * kHalfBox + (i * kBlk + r) * 128 + (x & 7) * 16),
+                           0u, 0u, 0u, 0u);
+          }
+        }
+        if (wrote) fence_proxy_async_smem();
+      };
+      for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
+        const Item it = make_item(p.s, p.grid, item);
+        for (int w = 0; w < 2 && ok; ++w) {
+          it.span<kCB>(p.s, w, &first[w], &last[w]);
+          if (last[w] < 0) continue;
+          ok = mbar_wait(&q_full[w], uses[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+          ++uses[w];
+        }
+        if (!ok) break;
+        const int chunks = it.chunks<kCB>();
+        auto k_slot = [&](int c) { return seq + c * per; };
+        auto v_slot = [&](int c) { return seq + c * per + per - 1; };
+        if (chunks > 0) {
+          ok = wait_slot(k_slot(0)) && wait_slot(v_slot(0));
+          for (int w = 0; w < 2 && ok; ++w)
+            if (it.active<kCB>(p.s, w, 0))
+              ok = issue_s(w, 0, k_slot(0) % C::kSlots, v_slot(0) % C::kSlots, it.blocks<kCB>(0));
+          if (ok && !p.shared) umma_commit(&kv_empty[v_slot(0) % C::kSlots]);
+        }
+        for (int c = 0; c < chunks && ok; ++c) {
+          const int nb = it.blocks<kCB>(c);
+          const bool more = c + 1 < chunks;
+          const int sk = k_slot(c) % C::kSlots;
+          if (p.s.kv_lens != nullptr) clear_tail(it, c, sk, nb);
+          if (more) ok = wait_slot(k_slot(c + 1)) && wait_slot(v_slot(c + 1));
+          for (int w = 0; w < 2 && ok; ++w) {
+            if (it.active<kCB>(p.s, w, c)) ok = issue_o(w, c, sk, nb);
+            if (ok && more && it.active<kCB>(p.s, w, c + 1))
+              ok = issue_s(w, c + 1, k_slot(c + 1) % C::kSlots, v_slot(c + 1) % C::kSlots,
+                           it.blocks<kCB>(c + 1));
+          }
+          if (!ok) break;
+          umma_commit(&kv_empty[sk]);
+          if (more && !p.shared) umma_commit(&kv_empty[v_slot(c + 1) % C::kSlots]);
+        }
+        seq += chunks * per;
+      }
+      umma_commit(drain_bar);
+      mbar_drain(drain_bar, 0);
+    }
+  } else {
+    // ------------------------------------------------------------ dS
+    set_max_regs_inc<kBwdRegsSoftmax>();
+    const int w = (warp - 4) >> 2;
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const int tok = row / p.s.g;
+    const int head = row - tok * p.s.g;
+    const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
+    const uint32_t sp = tmem + lane_off + static_cast<uint32_t>(w * 256);
+    const uint32_t od = sp + 128u;
+    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
+    int gc = 0;
+    bool ok = true;
+    for (int64_t item = blockIdx.x; item < p.grid.items; item += gridDim.x) {
+      const Item it = make_item(p.s, p.grid, item);
+      int first, last;
+      it.span<kCB>(p.s, w, &first, &last);
+      const int t = it.t0[w] + tok;
+      const bool valid = tok < p.grid.tt && t < it.t1[w];
+      const int pos = min(t, it.t1[w] - 1) + p.s.n - p.s.m;
+      const int64_t orow = (static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + it.kvh * p.s.g + head;
+      const float2 st = valid ? __ldg(p.stat + orow) : make_float2(-INFINITY, 0.f);
+      const uint64_t l2 = f2_pack(st.x, st.x), d2 = f2_pack(st.y, st.y);
+      uint64_t psum[2] = {0ull, 0ull};  // sum_j P_j dP_j
+      for (int c = first; c <= last; ++c) {
+        if (!it.active<kCB>(p.s, w, c)) continue;
+        const int nb = it.blocks<kCB>(c);
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[w], gc & 1, abort_flag, p.err,
+                                               DSA_DEVERR_WIN_WAIT));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sv[kCB][32], dv[kCB][32];
+#pragma unroll
+        for (int i = 0; i < kCB; ++i) {
+          if (i < nb) {
+            tmem_ld_32x32b_x32_nowait(sp + static_cast<uint32_t>(i * kBlk), sv[i]);
+            tmem_ld_32x32b_x32_nowait(sp + 64u + static_cast<uint32_t>(i * kBlk), dv[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kCB; ++i) {
+          if (i < nb) {
+            tmem_wait_ld_dep(sv[i]);
+            tmem_wait_ld_dep(dv[i]);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < kCB; ++i) {
+          if (i < nb) {
+            const uint32_t seen = seen_bits(p.s, it.r, c * kCB + i, pos, it.kv_len);
+            if (!__all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu)) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (!((seen >> k) & 1u)) {
+                  sv[i][k] = 0xFF800000u;  // P = 0
+                  dv[i][k] = 0u;
+                }
+            }
+            uint32_t pk[16];
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float z0, z1, g0, g1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[i][2 * k]), __uint_as_float(sv[i][2 * k + 1])),
+                               scale2, l2),
+                        z0, z1);
+              const uint64_t e2 = f2_pack(ex2_approx(z0), ex2_approx(z1));
+              const uint64_t g2 =
+                  f2_pack(__uint_as_float(dv[i][2 * k]), __uint_as_float(dv[i][2 * k + 1]));
+              psum[k & 1] = f2_fma(e2, g2, psum[k & 1]);
+              f2_unpack(f2_mul(e2, f2_add(g2, d2)), g0, g1);
+              pk[k] = T::pack(g0, g1);
+            }
+            tmem_st_x16_nowait(sp + static_cast<uint32_t>(i * 16), pk);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[w]);
+        ++gc;
+      }
+      if (!ok) break;
+      if (last >= 0) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&o_done[w], (gc - 1) & 1, abort_flag, p.err,
+                                               DSA_DEVERR_WIN_WAIT));
+        if (!ok) break;
+        tc_fence_after();
+      }
+#pragma unroll 1
+      for (int q = 0; q < D / 32; ++q) {
+        uint32_t ov[32];
+        if (last >= 0) {
+          tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) ov[k] = 0u;
+        }
+        if (valid) {
+          uint4* dst = reinterpret_cast<uint4*>(p.dq + orow * D + q * 32);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t x[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              x[u] = T::pack(__uint_as_float(ov[8 * j + 2 * u]) * p.scale,
+                             __uint_as_float(ov[8 * j + 2 * u + 1]) * p.scale);
+            dst[j] = make_uint4(x[0], x[1], x[2], x[3]);
+          }
+        }
+      }
+      if (last >= 0) {
+        tc_fence_before();
+        mbar_arrive(&o_empty[w]);
+      }
+      if (valid && p.sink != nullptr) {
+        float a0, a1, b0, b1;
+        f2_unpack(psum[0], a0, a1);
+        f2_unpack(psum[1], b0, b1);
+        // the sink's own weight e^(sink - lse): 0 where the sink is -inf
+        const float weight = ex2_approx(fmaf(__ldg(p.sink + it.kvh * p.s.g + head), kLog2e, st.x));
+        const float sum = (a0 + a1) + (b0 + b1);
+        p.sink_rows[orow] = st.x == -INFINITY ? 0.f : weight * sum;
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kBwdTmemCols);
+  }
+}
+
+// ------------------------------------------------------------------ dsink
+// Column sums of sink_rows [rows, h] in two fixed-order steps: blocks of
+// kSinkRows rows, then the blocks. A block holds 32 heads x 8 row lanes.
+constexpr int kSinkRows = 512;
+
+__global__ void __launch_bounds__(256) window_dsink_kernel(const float* in, float* out, int64_t rows,
+                                                           int h, float sign) {
+  __shared__ float part[8][33];
+  const int head = blockIdx.y * 32 + (threadIdx.x & 31);
+  const int y = threadIdx.x >> 5;
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kSinkRows;
+  const int64_t r1 = r0 + kSinkRows < rows ? r0 + kSinkRows : rows;
+  float sum = 0.f;
+  if (head < h)
+    for (int64_t r = r0 + y; r < r1; r += 8) sum += in[r * h + head];
+  part[y][threadIdx.x & 31] = sum;
+  __syncthreads();
+  if (y == 0 && head < h) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) sum += part[i][threadIdx.x];
+    out[static_cast<int64_t>(blockIdx.x) * h + head] = sum * sign;
+  }
+}
+
+// ------------------------------------------------------------------ host
+struct BwdPlan {
+  int gb, hb, tt;
+  int key_tiles, first_tiles, split_first, split, units_per_head;
+  int64_t units;
+  size_t off_stat, off_rows, off_sum, off_parts, bytes;
+};
+
+inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Key tiles are split over their rows so that no unit is much longer than an equal
+// share of a third of an SM (kUnits = 3 x 148), and none is shorter than 16
+// streamed tiles, below which the fp32 parts cost more than the balance gives.
+inline BwdPlan plan_bwd(const Shape& s, int64_t batch, int d, bool shared) {
+  constexpr int64_t kUnits = 3 * 148;
+  BwdPlan b;
+  b.hb = s.g <= kStream ? 1 : 2;
+  b.gb = b.hb == 1 ? s.g : (s.g + 1) / 2;
+  b.tt = b.hb == 1 ? kStream / s.g : 1;
+  b.key_tiles = static_cast<int>(div_up(s.n, kRows));
+  b.first_tiles = static_cast<int>(div_up(s.n_first, kRows));
+  int64_t total = 0, most_first = 0, most = 0;
+  for (int kt = 0; kt < b.key_tiles; ++kt) {
+    int ta, tb;
+    dkv_tokens(s, kt, &ta, &tb);
+    const int64_t tiles = div_up(tb - ta, b.tt) * b.hb;
+    total += tiles;
+    int64_t& top = kt < b.first_tiles ? most_first : most;
+    if (tiles > top) top = tiles;
+  }
+  int64_t share = div_up(total * batch * s.hk, kUnits);
+  if (share < 16) share = 16;
+  b.split_first = static_cast<int>(most_first > 0 ? div_up(most_first, share) : 1);
+  b.split = static_cast<int>(most > 0 ? div_up(most, share) : 1);
+  b.units_per_head = b.first_tiles * b.split_first + (b.key_tiles - b.first_tiles) * b.split;
+  b.units = batch * s.hk * b.units_per_head;
+  const auto pad = [](size_t x) { return (x + 255) & ~static_cast<size_t>(255); };
+  const size_t rows = static_cast<size_t>(batch) * s.m * s.h;
+  b.off_stat = 0;
+  b.off_rows = pad(rows * sizeof(float2));
+  b.off_sum = b.off_rows + pad(rows * sizeof(float));
+  b.off_parts = b.off_sum + pad(static_cast<size_t>(div_up(batch * s.m, kSinkRows)) * s.h * sizeof(float));
+  const bool parts = b.split > 1 || (b.first_tiles > 0 && b.split_first > 1);
+  b.bytes = b.off_parts +
+            (parts ? static_cast<size_t>(b.units) * (shared ? 1 : 2) * kRows * d * sizeof(float) : 0);
+  return b;
+}
+
+template <typename T, int D>
+int launch_bwd(const Tensors& x, const Shape& s, int64_t batch, float scale, const float* sink,
+               const void* out, const void* dout, const Strides& dos, const float* lse, void* dq,
+               void* dk, void* dv, float* dsink, uint8_t* ws, const BwdPlan& b, cudaStream_t stream) {
+  DeviceInfo di;
+  int st = current_device_info(&di);
+  if (st != DSA_OK) return st;
+  if (di.max_smem_optin < DkvCfg<D>::kSmemBytes || di.max_smem_optin < DqCfg<D>::kSmemBytes)
+    return DSA_ERR_UNSUPPORTED;
+  unsigned int* err = nullptr;
+  st = device_error_word(&err);
+  if (st != DSA_OK) return st;
+  const int64_t rows = batch * s.m * s.h;
+  float2* stat = reinterpret_cast<float2*>(ws + b.off_stat);
+  float* sink_rows = reinterpret_cast<float*>(ws + b.off_rows);
+  float* sink_sum = reinterpret_cast<float*>(ws + b.off_sum);
+  if (rows > 0) {
+    window_stat_kernel<T, D>
+        <<<static_cast<unsigned>(div_up(rows, 256 / (D / 8))), 256, 0, stream>>>(
+            static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(dout), dos, lse, stat,
+            rows, s.m, s.h);
+    st = cuda_status(cudaGetLastError());
+    if (st != DSA_OK) return st;
+  }
+  CUtensorMap tm_q, tm_do, tm_k, tm_v;
+  if (s.n > 0) {
+    st = map_rows_by_head(&tm_q, T::kFmt, x.q, x.qs, batch, s.m, s.h, D, b.gb, b.tt);
+    if (st == DSA_OK)
+      st = map_rows_by_head(&tm_do, T::kFmt, dout, dos, batch, s.m, s.h, D, b.gb, b.tt);
+    if (st == DSA_OK) st = map_head_by_rows(&tm_k, T::kFmt, x.k, x.ks, batch, s.n, s.hk, D, kRows);
+    if (st == DSA_OK) st = map_head_by_rows(&tm_v, T::kFmt, x.v, x.vs, batch, s.n, s.hk, D, kRows);
+    if (st != DSA_OK) return st;
+    DkvParams p;
+    p.s = s;
+    p.gb = b.gb;
+    p.hb = b.hb;
+    p.tt = b.tt;
+    p.key_tiles = b.key_tiles;
+    p.first_tiles = b.first_tiles;
+    p.split_first = b.split_first;
+    p.split = b.split;
+    p.units_per_head = b.units_per_head;
+    p.units = b.units;
+    p.scale = scale;
+    p.scale_log2 = scale * kLog2e;
+    p.stat = stat;
+    p.dk = static_cast<uint16_t*>(dk);
+    p.dv = static_cast<uint16_t*>(dv);
+    p.parts = reinterpret_cast<float*>(ws + b.off_parts);
+    p.err = err;
+    auto kernel = window_dkv_kernel<T, D>;
+    st = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), DkvCfg<D>::kSmemBytes);
+    if (st != DSA_OK) return st;
+    const int64_t grid = p.units < di.num_sms ? p.units : di.num_sms;
+    kernel<<<static_cast<unsigned>(grid), kBwdThreads, DkvCfg<D>::kSmemBytes, stream>>>(
+        tm_q, tm_do, tm_k, tm_v, p);
+    st = cuda_status(cudaGetLastError());
+    if (st != DSA_OK) return st;
+    const int tiles = b.split > 1 ? b.key_tiles : (b.split_first > 1 ? b.first_tiles : 0);
+    if (tiles > 0) {
+      const int64_t work = batch * s.hk * tiles * (dv ? 2 : 1) * kRows * (D / 4);
+      window_join_kernel<T, D><<<static_cast<unsigned>(div_up(work, 256)), 256, 0, stream>>>(p, batch);
+      st = cuda_status(cudaGetLastError());
+      if (st != DSA_OK) return st;
+    }
+  }
+  if (rows == 0) {
+    if (dsink != nullptr) return cuda_status(cudaMemsetAsync(dsink, 0, s.h * sizeof(float), stream));
+    return DSA_OK;
+  }
+  DqParams p;
+  p.s = s;
+  p.grid = tile_grid(s, batch);
+  p.scale = scale;
+  p.scale_log2 = scale * kLog2e;
+  p.stat = stat;
+  p.sink = dsink != nullptr ? sink : nullptr;
+  p.dq = static_cast<uint16_t*>(dq);
+  p.sink_rows = sink_rows;
+  p.shared = x.v == x.k && same_strides(x.vs, x.ks);
+  p.err = err;
+  st = map_rows_by_head(&tm_q, T::kFmt, x.q, x.qs, batch, s.m, s.h, D, s.g, p.grid.tt);
+  if (st == DSA_OK)
+    st = map_rows_by_head(&tm_do, T::kFmt, dout, dos, batch, s.m, s.h, D, s.g, p.grid.tt);
+  if (st == DSA_OK) st = map_head_by_rows(&tm_k, T::kFmt, x.k, x.ks, batch, s.n, s.hk, D, kBlk);
+  if (st == DSA_OK) st = map_head_by_rows(&tm_v, T::kFmt, x.v, x.vs, batch, s.n, s.hk, D, kBlk);
+  if (st != DSA_OK) return st;
+  auto kernel = window_dq_kernel<T, D>;
+  st = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), DqCfg<D>::kSmemBytes);
+  if (st != DSA_OK) return st;
+  const int64_t grid = p.grid.items < di.num_sms ? p.grid.items : di.num_sms;
+  kernel<<<static_cast<unsigned>(grid), kBwdThreads, DqCfg<D>::kSmemBytes, stream>>>(tm_q, tm_do, tm_k,
+                                                                                    tm_v, p);
+  st = cuda_status(cudaGetLastError());
+  if (st != DSA_OK || dsink == nullptr) return st;
+  // rows of all heads -> blocks of rows -> one row; more steps while one block is not enough
+  const float* in = sink_rows;
+  int64_t left = batch * s.m;
+  float* sums = sink_sum;
+  const unsigned hx = static_cast<unsigned>(div_up(s.h, 32));
+  while (true) {
+    const int64_t blocks = div_up(left, kSinkRows);
+    const bool end = blocks == 1;
+    window_dsink_kernel<<<dim3(static_cast<unsigned>(blocks), hx), 256, 0, stream>>>(
+        in, end ? dsink : sums, left, s.h, end ? -1.f : 1.f);
+    st = cuda_status(cudaGetLastError());
+    if (st != DSA_OK || end) return st;
+    // the next step reads this one's sums and writes over the rows, which are done with
+    in = sums;
+    left = blocks;
+    sums = sums == sink_sum ? sink_rows : sink_sum;
+  }
+}
+
+}  // namespace win
+}  // namespace dsa
+
+extern "C" size_t dsa_window_attn_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t n,
+                                                      int n_heads, int n_kv_heads, int head_dim,
+                                                      int64_t window, int64_t n_first, int shared_kv) {
+  using namespace dsa::win;
+  static const char dummy = 0;
+  const void* at = reinterpret_cast<const void*>(reinterpret_cast<uintptr_t>(&dummy) & ~uintptr_t{15});
+  Tensors x;
+  Shape s;
+  if (check_window_args(at, nullptr, at, nullptr, at, nullptr, nullptr, DSA_DTYPE_BF16, batch, m, n,
+                        n_heads, n_kv_heads, head_dim, window, n_first, 1.f, &x, &s) != DSA_OK)
+    return 0;
+  return plan_bwd(s, batch, head_dim, shared_kv != 0).bytes;
+}
+
+extern "C" int dsa_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k,
+                                   const int64_t* k_strides, const void* v,
+                                   const int64_t* v_strides, const float* sink, const int* kv_lens,
+                                   const void* out, const float* lse, const void* dout,
+                                   const int64_t* dout_strides, void* dq, void* dk, void* dv,
+                                   float* dsink, int dtype, int64_t batch, int64_t m, int64_t n,
+                                   int n_heads, int n_kv_heads, int head_dim, int64_t window,
+                                   int64_t n_first, float softmax_scale, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
+  using namespace dsa;
+  using namespace dsa::win;
+  Tensors x;
+  Shape s;
+  int st = check_window_args(q, q_strides, k, k_strides, v, v_strides, kv_lens, dtype, batch, m, n,
+                             n_heads, n_kv_heads, head_dim, window, n_first, softmax_scale, &x, &s);
+  if (st != DSA_OK) return st;
+  Strides dos;
+  st = read_strides(dout_strides, batch, m, n_heads, head_dim, &dos);
+  if (st != DSA_OK) return st;
+  const bool shared = dv == nullptr;
+  if (shared && !(x.v == x.k && same_strides(x.vs, x.ks))) return DSA_ERR_INVALID_ARGUMENT;
+  if (dsink != nullptr && sink == nullptr) return DSA_ERR_INVALID_ARGUMENT;
+  cudaStream_t cs = static_cast<cudaStream_t>(stream);
+  if (batch == 0)
+    return dsink ? cuda_status(cudaMemsetAsync(dsink, 0, n_heads * sizeof(float), cs)) : DSA_OK;
+  if (m > 0 && (out == nullptr || lse == nullptr || dout == nullptr || dq == nullptr))
+    return DSA_ERR_INVALID_ARGUMENT;
+  if (n > 0 && dk == nullptr) return DSA_ERR_INVALID_ARGUMENT;
+  if (!aligned16(out) || !aligned16(dout) || !aligned16(dq) || !aligned16(dk) || !aligned16(dv))
+    return DSA_ERR_MISALIGNED;
+  if (m == 0) {  // no row sees any key
+    const size_t bytes = static_cast<size_t>(batch) * n * n_kv_heads * head_dim * 2;
+    if (n > 0) st = cuda_status(cudaMemsetAsync(dk, 0, bytes, cs));
+    if (st == DSA_OK && n > 0 && dv) st = cuda_status(cudaMemsetAsync(dv, 0, bytes, cs));
+    if (st == DSA_OK && dsink)
+      st = cuda_status(cudaMemsetAsync(dsink, 0, n_heads * sizeof(float), cs));
+    return st;
+  }
+  const BwdPlan b = plan_bwd(s, batch, head_dim, shared);
+  if (workspace == nullptr || workspace_bytes < b.bytes) return DSA_ERR_WORKSPACE;
+  if ((reinterpret_cast<uintptr_t>(workspace) & 255u) != 0) return DSA_ERR_MISALIGNED;
+  if (b.units > (int64_t{1} << 40) || batch * m * n_heads > (int64_t{1} << 34))
+    return DSA_ERR_UNSUPPORTED;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (head_dim == 128)
+    return dtype == DSA_DTYPE_BF16
+               ? launch_bwd<Bf16, 128>(x, s, batch, softmax_scale, sink, out, dout, dos, lse, dq, dk,
+                                       dv, dsink, ws, b, cs)
+               : launch_bwd<Fp16, 128>(x, s, batch, softmax_scale, sink, out, dout, dos, lse, dq, dk,
+                                       dv, dsink, ws, b, cs);
+  return dtype == DSA_DTYPE_BF16
+             ? launch_bwd<Bf16, 64>(x, s, batch, softmax_scale, sink, out, dout, dos, lse, dq, dk, dv,
+                                    dsink, ws, b, cs)
+             : launch_bwd<Fp16, 64>(x, s, batch, softmax_scale, sink, out, dout, dos, lse, dq, dk, dv,
+                                    dsink, ws, b, cs);
+}

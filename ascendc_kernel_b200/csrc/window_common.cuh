@@ -130,5 +130,87 @@ __device__ __forceinline__ uint32_t seen_bits(const Shape& s, const Range& r, in
   return near | bits_between(0, min(top, s.n_first - key));
 }
 
+__device__ __forceinline__ void tmem_st_x16_nowait(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
+      "%14,%15,%16};\n"
+      :
+      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+        "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+        "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// Work items of the kernels that walk the keys of fixed rows: two tiles of
+// consecutive tokens of one (batch, kv head).
+struct TileGrid {
+  int tt;               // tokens of a tile
+  int items_per_head;   // pairs of tiles
+  int64_t items;
+};
+
+inline TileGrid tile_grid(const Shape& s, int64_t batch) {
+  TileGrid g;
+  g.tt = kRows / s.g;
+  g.items_per_head = ((s.m + g.tt - 1) / g.tt + 1) / 2;
+  g.items = batch * s.hk * g.items_per_head;
+  return g;
+}
+
+// The item's keys are read in chunks of CB blocks (the last one may be shorter).
+struct Item {
+  int b, kvh, kv_len;
+  int t0[2], t1[2];  // tokens of each tile, empty when t1 <= t0
+  Range r;
+
+  template <int CB>
+  __device__ __forceinline__ int chunks() const {
+    return (r.nblk + CB - 1) / CB;
+  }
+  template <int CB>
+  __device__ __forceinline__ int blocks(int c) const {
+    return min(CB, r.nblk - c * CB);
+  }
+  // Whether any row of tile w sees a key of chunk c.
+  template <int CB>
+  __device__ __forceinline__ bool active(const Shape& s, int w, int c) const {
+    if (t1[w] <= t0[w]) return false;
+    const int off = s.n - s.m;
+    const int hi = min(t1[w] + off, kv_len);
+    const int lo = t0[w] + off - s.window + 1;
+    const int nb = blocks<CB>(c);
+    bool any = false;
+    for (int i = 0; i < nb; ++i) {
+      const int k = r.key(c * CB + i);
+      any = any || (k < hi && (c * CB + i < r.nfb || k + kBlk > lo || k < s.n_first));
+    }
+    return any;
+  }
+  // First and last active chunk of tile w (last = -1 when none).
+  template <int CB>
+  __device__ __forceinline__ void span(const Shape& s, int w, int* first, int* last) const {
+    int f = 0, l = chunks<CB>() - 1;
+    while (l >= 0 && !active<CB>(s, w, l)) --l;
+    while (f <= l && !active<CB>(s, w, f)) ++f;
+    *first = f;
+    *last = l;
+  }
+};
+
+__device__ __forceinline__ Item make_item(const Shape& s, const TileGrid& g, int64_t item) {
+  Item it;
+  const int64_t bh = item / g.items_per_head;
+  const int pair = static_cast<int>(item - bh * g.items_per_head);
+  it.b = static_cast<int>(bh / s.hk);
+  it.kvh = static_cast<int>(bh - static_cast<int64_t>(it.b) * s.hk);
+  it.kv_len = kv_len_of(s, it.b);
+  for (int w = 0; w < 2; ++w) {
+    it.t0[w] = min((2 * pair + w) * g.tt, s.m);
+    it.t1[w] = min((2 * pair + w + 1) * g.tt, s.m);
+  }
+  it.r = key_range(s, it.t0[0], max(it.t1[0], it.t1[1]), it.kv_len);
+  return it;
+}
+
 }  // namespace win
 }  // namespace dsa

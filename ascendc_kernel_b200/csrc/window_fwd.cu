@@ -54,10 +54,7 @@ struct FwdCfg {
 
 struct FwdParams {
   Shape s;
-  int tt;               // tokens of a tile
-  int tiles;            // token tiles per (batch, kv head)
-  int items_per_head;   // pairs of them
-  int64_t total_items;
+  TileGrid grid;
   float scale_log2;
   const float* sink;    // [h] or null
   uint16_t* out;        // [batch, m, h, D]
@@ -65,70 +62,6 @@ struct FwdParams {
   int shared;           // K and V are one tensor
   unsigned int* err;
 };
-
-struct Item {
-  int b, kvh, kv_len;
-  int t0[2], t1[2];  // tokens of each tile, empty when t1 <= t0
-  Range r;
-  int chunks;
-};
-
-__device__ __forceinline__ Item make_item(const FwdParams& p, int64_t item) {
-  Item it;
-  const int64_t bh = item / p.items_per_head;
-  const int pair = static_cast<int>(item - bh * p.items_per_head);
-  it.b = static_cast<int>(bh / p.s.hk);
-  it.kvh = static_cast<int>(bh - static_cast<int64_t>(it.b) * p.s.hk);
-  it.kv_len = kv_len_of(p.s, it.b);
-  for (int w = 0; w < 2; ++w) {
-    it.t0[w] = min((2 * pair + w) * p.tt, p.s.m);
-    it.t1[w] = min((2 * pair + w + 1) * p.tt, p.s.m);
-  }
-  it.r = key_range(p.s, it.t0[0], max(it.t1[0], it.t1[1]), it.kv_len);
-  it.chunks = (it.r.nblk + kChunkBlks - 1) / kChunkBlks;
-  return it;
-}
-
-__device__ __forceinline__ int chunk_blocks(const Item& it, int c) {
-  return min(kChunkBlks, it.r.nblk - c * kChunkBlks);
-}
-
-// Whether any row of tile w sees a key of chunk c.
-__device__ __forceinline__ bool tile_active(const FwdParams& p, const Item& it, int w, int c) {
-  if (it.t1[w] <= it.t0[w]) return false;
-  const int off = p.s.n - p.s.m;
-  const int hi = min(it.t1[w] + off, it.kv_len);
-  const int lo = it.t0[w] + off - p.s.window + 1;
-  const int nb = chunk_blocks(it, c);
-  bool any = false;
-  for (int i = 0; i < nb; ++i) {
-    const int k = it.r.key(c * kChunkBlks + i);
-    const bool first = c * kChunkBlks + i < it.r.nfb;
-    any = any || (k < hi && (first || k + kBlk > lo || k < p.s.n_first));
-  }
-  return any;
-}
-
-// First and last active chunk of tile w (last = -1 when none).
-__device__ __forceinline__ void active_span(const FwdParams& p, const Item& it, int w, int* first,
-                                            int* last) {
-  int f = 0, l = it.chunks - 1;
-  while (l >= 0 && !tile_active(p, it, w, l)) --l;
-  while (f <= l && !tile_active(p, it, w, f)) ++f;
-  *first = f;
-  *last = l;
-}
-
-__device__ __forceinline__ void tmem_st_x16_nowait(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,"
-      "%14,%15,%16};\n"
-      :
-      : "r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
-        "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
-        "r"(r[14]), "r"(r[15])
-      : "memory");
-}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -197,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!mbar_wait(&kv_empty[s], ((seq / C::kSlots) & 1) ^ 1, abort_flag, p.err,
                        DSA_DEVERR_WIN_WAIT))
           return false;
-        const int nb = chunk_blocks(it, c);
+        const int nb = it.blocks<kChunkBlks>(c);
         uint8_t* dst = smem + C::kOffKV + s * C::kTileBytes;
         mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(nb * kBlk * D * 2));
         for (int i = 0; i < nb; ++i) {
@@ -210,11 +143,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++seq;
         return true;
       };
-      for (int64_t item = blockIdx.x; ok && item < p.total_items; item += gridDim.x) {
-        const Item it = make_item(p, item);
+      for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
+        const Item it = make_item(p.s, p.grid, item);
         for (int w = 0; w < 2 && ok; ++w) {
           int f, l;
-          active_span(p, it, w, &f, &l);
+          it.span<kChunkBlks>(p.s, w, &f, &l);
           if (l < 0) continue;
           if (!mbar_wait(&q_empty[w], (uses[w] & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) {
             ok = false;
@@ -222,14 +155,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           uint8_t* qs = smem + C::kOffQ + w * C::kTileBytes;
           mbar_arrive_expect_tx(&q_full[w],
-                                static_cast<uint32_t>(p.tt * p.s.g * D * 2));
+                                static_cast<uint32_t>(p.grid.tt * p.s.g * D * 2));
 #pragma unroll
           for (int half = 0; half < C::kHalves; ++half)
             tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0[w], it.b,
                         &q_full[w]);
           ++uses[w];
         }
-        for (int c = 0; c < it.chunks && ok; ++c) {
+        for (int c = 0; c < it.chunks<kChunkBlks>() && ok; ++c) {
           ok = load_slot(it, &tm_k, c);
           if (ok && !p.shared) ok = load_slot(it, &tm_v, c);
         }
@@ -314,10 +247,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (wrote) fence_proxy_async_smem();
       };
-      for (int64_t item = blockIdx.x; ok && item < p.total_items; item += gridDim.x) {
-        const Item it = make_item(p, item);
+      for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
+        const Item it = make_item(p.s, p.grid, item);
         for (int w = 0; w < 2 && ok; ++w) {
-          active_span(p, it, w, &first[w], &last[w]);
+          it.span<kChunkBlks>(p.s, w, &first[w], &last[w]);
           if (last[w] < 0) continue;
           ok = mbar_wait(&q_full[w], uses[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
           ++uses[w];
@@ -325,31 +258,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         auto k_slot = [&](int c) { return seq + c * per; };
         auto v_slot = [&](int c) { return seq + c * per + per - 1; };
-        if (it.chunks > 0) {
-          const int nb = chunk_blocks(it, 0);
+        if (it.chunks<kChunkBlks>() > 0) {
+          const int nb = it.blocks<kChunkBlks>(0);
           ok = wait_slot(k_slot(0));
           for (int w = 0; w < 2 && ok; ++w)
-            if (tile_active(p, it, w, 0)) ok = issue_s(w, 0, k_slot(0) % C::kSlots, nb);
+            if (it.active<kChunkBlks>(p.s, w, 0)) ok = issue_s(w, 0, k_slot(0) % C::kSlots, nb);
           if (ok && !p.shared) umma_commit(&kv_empty[k_slot(0) % C::kSlots]);
         }
-        for (int c = 0; c < it.chunks && ok; ++c) {
-          const int nb = chunk_blocks(it, c);
-          const bool more = c + 1 < it.chunks;
-          const int nbn = more ? chunk_blocks(it, c + 1) : 0;
+        for (int c = 0; c < it.chunks<kChunkBlks>() && ok; ++c) {
+          const int nb = it.blocks<kChunkBlks>(c);
+          const bool more = c + 1 < it.chunks<kChunkBlks>();
+          const int nbn = more ? it.blocks<kChunkBlks>(c + 1) : 0;
           const int sv = v_slot(c) % C::kSlots;
           ok = wait_slot(v_slot(c));
           if (ok && p.s.kv_lens != nullptr) clear_tail(it, c, sv, nb);
           if (ok && more) ok = wait_slot(k_slot(c + 1));
           for (int w = 0; w < 2 && ok; ++w) {
-            if (tile_active(p, it, w, c)) ok = issue_pv(w, c, sv, nb);
-            if (ok && more && tile_active(p, it, w, c + 1))
+            if (it.active<kChunkBlks>(p.s, w, c)) ok = issue_pv(w, c, sv, nb);
+            if (ok && more && it.active<kChunkBlks>(p.s, w, c + 1))
               ok = issue_s(w, c + 1, k_slot(c + 1) % C::kSlots, nbn);
           }
           if (!ok) break;
           umma_commit(&kv_empty[sv]);
           if (more && !p.shared) umma_commit(&kv_empty[k_slot(c + 1) % C::kSlots]);
         }
-        seq += it.chunks * per;
+        seq += it.chunks<kChunkBlks>() * per;
       }
       umma_commit(drain_bar);
       mbar_drain(drain_bar, 0);
@@ -369,21 +302,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int gc = 0;  // chunks processed (all items)
     bool ok = true;
-    for (int64_t item = blockIdx.x; item < p.total_items; item += gridDim.x) {
-      const Item it = make_item(p, item);
+    for (int64_t item = blockIdx.x; item < p.grid.items; item += gridDim.x) {
+      const Item it = make_item(p.s, p.grid, item);
       int first, last;
-      active_span(p, it, w, &first, &last);
+      it.span<kChunkBlks>(p.s, w, &first, &last);
       const int t = it.t0[w] + tok;
-      const bool valid = tok < p.tt && t < it.t1[w];
+      const bool valid = tok < p.grid.tt && t < it.t1[w];
       // rows past the tile's tokens follow its last one: their values are not used
       const int pos = min(t, it.t1[w] - 1) + p.s.n - p.s.m;
       const int gh = it.kvh * p.s.g + head;
-      const bool has_sink = p.sink != nullptr && tok < p.tt;
+      const bool has_sink = p.sink != nullptr && tok < p.grid.tt;
       const float sink2 = has_sink ? __ldg(p.sink + gh) * kLog2e : -INFINITY;
       float m = sink2, l = 0.f;
       for (int c = first; c <= last; ++c) {
-        if (!tile_active(p, it, w, c)) continue;
-        const int nb = chunk_blocks(it, c);
+        if (!it.active<kChunkBlks>(p.s, w, c)) continue;
+        const int nb = it.blocks<kChunkBlks>(c);
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[w], gc & 1, abort_flag, p.err,
                                                DSA_DEVERR_WIN_WAIT));
         if (!ok) break;
@@ -528,10 +461,7 @@ int launch_fwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   if (st != DSA_OK) return st;
   FwdParams p;
   p.s = s;
-  p.tt = kRows / s.g;
-  p.tiles = (s.m + p.tt - 1) / p.tt;
-  p.items_per_head = (p.tiles + 1) / 2;
-  p.total_items = batch * s.hk * p.items_per_head;
+  p.grid = tile_grid(s, batch);
   p.scale_log2 = scale * kLog2e;
   p.sink = sink;
   p.out = static_cast<uint16_t*>(out);
@@ -539,14 +469,14 @@ int launch_fwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   p.shared = x.v == x.k && same_strides(x.vs, x.ks);
   p.err = err;
   CUtensorMap tm_q, tm_k, tm_v;
-  st = map_rows_by_head(&tm_q, T::kFmt, x.q, x.qs, batch, s.m, s.h, D, s.g, p.tt);
+  st = map_rows_by_head(&tm_q, T::kFmt, x.q, x.qs, batch, s.m, s.h, D, s.g, p.grid.tt);
   if (st == DSA_OK) st = map_head_by_rows(&tm_k, T::kFmt, x.k, x.ks, batch, s.n, s.hk, D, kBlk);
   if (st == DSA_OK) st = map_head_by_rows(&tm_v, T::kFmt, x.v, x.vs, batch, s.n, s.hk, D, kBlk);
   if (st != DSA_OK) return st;
   auto kernel = window_fwd_kernel<T, D>;
   st = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), C::kSmemBytes);
   if (st != DSA_OK) return st;
-  const int64_t grid = p.total_items < di.num_sms ? p.total_items : di.num_sms;
+  const int64_t grid = p.grid.items < di.num_sms ? p.grid.items : di.num_sms;
   kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmemBytes, stream>>>(tm_q, tm_k, tm_v, p);
   return cuda_status(cudaGetLastError());
 }

@@ -17,7 +17,7 @@ import ctypes
 import torch
 import torch.nn as nn
 
-from ._native import call
+from ._native import call, lib
 
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # DSA_DTYPE_*
 
@@ -87,6 +87,70 @@ def _forward(q, k, v, sink, window, n_first, kv_lens, scale, out, want_lse):
     return out, lse
 
 
+def window_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                    v: torch.Tensor | None, sink: torch.Tensor | None, out: torch.Tensor,
+                    lse: torch.Tensor, *, window: int, n_first: int = 0,
+                    kv_lens: torch.Tensor | None = None, softmax_scale: float | None = None):
+    """Gradients of :func:`window_attn` from its inputs, its ``out`` and ``lse`` and the
+    upstream gradient ``dout``: (dq, dk, dv, dsink), contiguous and of the inputs' types (dv
+    None when v is None: dk is then the gradient of the shared tensor; dsink fp32, None
+    without a sink). Runs in a fixed order: the same inputs give the same bits."""
+    scale = float(q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale)
+    _check(q, k, v, sink, window, n_first, kv_lens, scale)
+    window, n_first = min(int(window), 1 << 28), min(int(n_first), 1 << 28)
+    b, m, h, d = q.shape
+    n, hk = k.shape[1], k.shape[2]
+    for x in (dout, out):
+        assert x.shape == q.shape and x.dtype == q.dtype and x.device == q.device, \
+            "dout and out must be like q"
+    assert out.is_contiguous(), "out must be contiguous"
+    assert lse.shape == (b, m, h) and lse.dtype == torch.float32 and lse.is_contiguous() \
+        and lse.device == q.device, "lse must be fp32 [b, m, h], contiguous"
+    q, k, dout = _strided(q), _strided(k), _strided(dout)
+    values = k if v is None else _strided(v)
+    sink = _sink_on(sink, q.device)
+    kv_lens = None if kv_lens is None else kv_lens.contiguous()
+    dev = q.device
+    dq = torch.empty(b, m, h, d, dtype=q.dtype, device=dev)
+    dk = torch.empty(b, n, hk, d, dtype=q.dtype, device=dev)
+    dv = None if v is None else torch.empty_like(dk)
+    dsink = None if sink is None else torch.empty(h, dtype=torch.float32, device=dev)
+    nbytes = lib().dsa_window_attn_bwd_workspace_bytes(b, m, n, h, hk, d, window, n_first,
+                                                       1 if v is None else 0)
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    with torch.cuda.device(dev):
+        call("dsa_window_attn_bwd", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
+             values.data_ptr(), _strides(values), _ptr(sink), _ptr(kv_lens), out.data_ptr(),
+             lse.data_ptr(), dout.data_ptr(), _strides(dout), dq.data_ptr(), dk.data_ptr(),
+             _ptr(dv), _ptr(dsink), DTYPES[q.dtype], b, m, n, h, hk, d, window, n_first, scale,
+             ws.data_ptr(), ws.numel(), stream)
+    return dq, dk, dv, dsink
+
+
+class _WindowAttn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, sink, window, n_first, kv_lens, scale):
+        out, lse = _forward(q, k, v, _sink_on(sink, q.device), window, n_first, kv_lens, scale,
+                            None, True)
+        ctx.save_for_backward(q, k, v, sink, kv_lens, out, lse)
+        ctx.args = (window, n_first, scale)
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _):
+        q, k, v, sink, kv_lens, out, lse = ctx.saved_tensors
+        window, n_first, scale = ctx.args
+        dq, dk, dv, dsink = window_attn_bwd(dout, q, k, v, sink, out, lse, window=window,
+                                            n_first=n_first, kv_lens=kv_lens,
+                                            softmax_scale=scale)
+        if dsink is not None:
+            dsink = dsink.to(device=sink.device, dtype=sink.dtype).reshape(sink.shape)
+        return dq, dk, dv, dsink, None, None, None, None
+
+
 def window_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None,
                 sink: torch.Tensor | None = None, *, window: int, n_first: int = 0,
                 kv_lens: torch.Tensor | None = None, softmax_scale: float | None = None,
@@ -108,6 +172,31 @@ def window_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None,
     if out is not None:
         assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device \
             and out.is_contiguous(), "out must be contiguous and like q"
+    if torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, sink)):
+        assert out is None, "a differentiable call allocates its own out"
+        out, lse = _WindowAttn.apply(q, k, v, sink, window, n_first, kv_lens, scale)
+        return (out, lse) if return_lse else out
     out, lse = _forward(q, k, v, _sink_on(sink, q.device), window, n_first, kv_lens, scale, out,
                         return_lse)
     return (out, lse) if return_lse else out
+
+
+class WindowAttention(nn.Module):
+    """:func:`window_attn` with its window and a learned sink logit per head, as
+    :class:`ascendc_kernel_b200.sparse_attn.ModelNew` holds them. ``window`` defaults to the
+    reference's ``ModelArgs.window_size``."""
+
+    def __init__(self, n_heads: int, head_dim: int, window: int = 128, n_first: int = 0):
+        super().__init__()
+        self.n_heads = n_heads
+        self.head_dim = head_dim
+        self.window = window
+        self.n_first = n_first
+        self.softmax_scale = head_dim ** -0.5
+        self.attn_sink = nn.Parameter(torch.zeros(n_heads, dtype=torch.float32))
+
+    def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None,
+                kv_lens: torch.Tensor | None = None) -> torch.Tensor:
+        assert q.shape[2] == self.n_heads and q.shape[3] == self.head_dim
+        return window_attn(q, k, v, self.attn_sink, window=self.window, n_first=self.n_first,
+                           kv_lens=kv_lens, softmax_scale=self.softmax_scale)

@@ -352,6 +352,29 @@ int dsa_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k,
                         int head_dim, int64_t window, int64_t n_first, float softmax_scale,
                         void* stream);
 
+/* Its gradients. Inputs as dsa_window_attn_fwd, with that call's out and lse and
+ * the upstream gradient dout [batch, m, n_heads, head_dim] (strides like q's):
+ *   P_j = e^(s_j - lse), D = rowsum(dout * out), dS_j = P_j (dout.v_j - D)
+ *   dq = scale sum_j dS_j k_j, dk_j = scale sum dS_j q, dv_j = sum P_j dout (over
+ *   the query heads of the group and all rows that see j), dsink[h] =
+ *   -sum over batch and rows of e^(sink[h] - lse) sum_j P_j (dout.v_j)
+ * dq like q, dk and dv like k and v (contiguous, the type of q; rows at or past
+ * kv_lens[b] get 0); dv NULL when v is k: dk receives the sum of both. dsink
+ * [n_heads] fp32 or NULL. Deterministic: no atomics, sums in a fixed order in
+ * fp32; P and dS are rounded to the operands' type for the products that sum over
+ * them. workspace: dsa_window_attn_bwd_workspace_bytes(...) bytes (shared_kv:
+ * dv is NULL; 0 for arguments the call refuses), 256-byte aligned. */
+size_t dsa_window_attn_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t n, int n_heads,
+                                           int n_kv_heads, int head_dim, int64_t window,
+                                           int64_t n_first, int shared_kv);
+int dsa_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k,
+                        const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                        const float* sink, const int* kv_lens, const void* out, const float* lse,
+                        const void* dout, const int64_t* dout_strides, void* dq, void* dk, void* dv,
+                        float* dsink, int dtype, int64_t batch, int64_t m, int64_t n, int n_heads,
+                        int n_kv_heads, int head_dim, int64_t window, int64_t n_first,
+                        float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
