@@ -78,6 +78,11 @@ SIGNATURES = {
                                    _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64, _i64,
                                    _i64, _i32, _i32, _i32, _i64, _i64, _f32, _c_void_p, _size_t,
                                    _c_void_p]),
+    "dsa_paged_attn_workspace_bytes": (_size_t, [_i64, _i32, _i32, _i32, _i64, _i64, _i32]),
+    "dsa_paged_attn_fwd": (_i32, [_c_void_p, _i64p, _c_void_p, _i64p, _c_void_p, _i64p, _c_void_p,
+                                  _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64,
+                                  _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _c_void_p,
+                                  _size_t, _c_void_p]),
 }
 
 _LIB = None

@@ -1,0 +1,105 @@
+"""A paged key-value cache and the operators that write it, read it and shrink it.
+
+The pool is ``k_pages`` and ``v_pages`` [num_pages, page_size, hk, d] (``v_pages`` None:
+the keys serve as values, as in :mod:`ascendc_kernel_b200.sparse_attn`) and, where
+eviction is wanted, ``weights`` [num_pages, page_size] fp32: the attention that each row
+has gathered. ``block_table`` [b, max_pages] int32 names each sequence's pages.
+
+* :func:`paged_attn`   -- one new token per sequence over the cache
+
+Shape preconditions are checked with ``assert``; CUDA-level failures raise DsaError.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from ._native import call, lib
+from .window_attn import DTYPES, _ptr, _sink_on
+
+
+def _check_pool(k_pages, v_pages, weights, block_table):
+    assert k_pages.is_cuda and k_pages.dtype in DTYPES and k_pages.dim() == 4, \
+        "k_pages must be a CUDA tensor [num_pages, page_size, hk, d], bf16 or fp16"
+    n, page, hk, d = k_pages.shape
+    for x in (k_pages, v_pages):
+        if x is not None:
+            assert x.shape == k_pages.shape and x.dtype == k_pages.dtype \
+                and x.device == k_pages.device, "v_pages must be like k_pages"
+            assert x.stride(3) == 1 and all(s % 8 == 0 and s > 0 for s in x.stride()[:3]) \
+                and x.data_ptr() % 16 == 0, \
+                "pages need a contiguous head_dim and strides in multiples of 8 elements"
+    assert n >= 1 and page >= 1 and page % 8 == 0, "page_size must be a multiple of 8"
+    assert d in (64, 128), "kernel specialised to head_dim in (64, 128)"
+    if weights is not None:
+        assert weights.shape == (n, page) and weights.dtype == torch.float32 \
+            and weights.is_contiguous() and weights.device == k_pages.device, \
+            "weights must be fp32 [num_pages, page_size], contiguous"
+    assert block_table.dtype == torch.int32 and block_table.dim() == 2 \
+        and block_table.device == k_pages.device and block_table.shape[1] >= 1, \
+        "block_table must be int32 [b, max_pages]"
+
+
+def _check_lens(lens, b, device, name="lens"):
+    assert lens.dtype == torch.int32 and lens.shape == (b,) and lens.device == device, \
+        f"{name} must be int32 [b] on the pool's device"
+
+
+def _page_strides(x):
+    return (ctypes.c_int64 * 3)(*x.stride()[:3])
+
+
+def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor | None,
+               block_table: torch.Tensor, lens: torch.Tensor, sink: torch.Tensor | None = None, *,
+               window: int = 0, n_first: int = 0, softmax_scale: float | None = None,
+               weights: torch.Tensor | None = None, out: torch.Tensor | None = None,
+               return_lse: bool = False):
+    """Attention of one new token per sequence over the cache, whose rows include it.
+
+    q [b, h, d]; lens [b] int32 counts each sequence's rows. The token sees rows
+    j < lens[b], with ``window`` > 0 only the last ``window`` and the first ``n_first`` of
+    them; sink [h] fp32 logits or None; softmax_scale defaults to d ** -0.5. Returns out
+    like q (0 where nothing is visible and there is no sink) and with ``return_lse`` the
+    fp32 log of the softmax divisor [b, h]. With ``weights`` the slot of each visible row
+    gains its attention weight summed over the heads, in place.
+    """
+    assert q.is_cuda and q.dim() == 3, "q must be a CUDA tensor [b, h, d]"
+    _check_pool(k_pages, v_pages, weights, block_table)
+    b, h, d = q.shape
+    n, page, hk, _ = k_pages.shape
+    assert q.dtype == k_pages.dtype and q.device == k_pages.device and d == k_pages.shape[3], \
+        "q must have the pool's type, device and head_dim"
+    assert h % hk == 0 and 1 <= h // hk <= 128, \
+        "n_heads must be a multiple of n_kv_heads, at most 128 to a group"
+    assert block_table.shape[0] == b
+    _check_lens(lens, b, q.device)
+    scale = float(d ** -0.5 if softmax_scale is None else softmax_scale)
+    assert window >= 0 and n_first >= 0 and scale > 0
+    if sink is not None:
+        assert sink.numel() == h, "sink must have n_heads entries"
+    if q.stride(2) != 1 or q.data_ptr() % 16 or any(
+            m > 1 and (s <= 0 or s % 8) for m, s in zip(q.shape, q.stride()[:2])):
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty(b, h, d, dtype=q.dtype, device=q.device)
+    else:
+        assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device \
+            and out.is_contiguous(), "out must be contiguous and like q"
+    lse = torch.empty(b, h, dtype=torch.float32, device=q.device) if return_lse else None
+    sink = _sink_on(sink, q.device)
+    table, lens = block_table.contiguous(), lens.contiguous()
+    values = k_pages if v_pages is None else v_pages
+    nbytes = lib().dsa_paged_attn_workspace_bytes(b, h, hk, d, table.shape[1], page,
+                                                  0 if weights is None else 1)
+    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=q.device)
+    stream = torch.cuda.current_stream(q.device).cuda_stream
+    with torch.cuda.device(q.device):
+        call("dsa_paged_attn_fwd", q.data_ptr(), (ctypes.c_int64 * 2)(*q.stride()[:2]),
+             k_pages.data_ptr(), _page_strides(k_pages), values.data_ptr(), _page_strides(values),
+             table.data_ptr(), lens.data_ptr(), _ptr(sink), out.data_ptr(), _ptr(lse),
+             _ptr(weights), DTYPES[q.dtype], b, h, hk, d, n, page, table.shape[1],
+             min(int(window), 1 << 28), min(int(n_first), 1 << 28), scale, ws.data_ptr(),
+             ws.numel(), stream)
+    return (out, lse) if return_lse else out

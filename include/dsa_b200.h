@@ -375,6 +375,40 @@ int dsa_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k,
                         int n_kv_heads, int head_dim, int64_t window, int64_t n_first,
                         float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------
+ * Paged key-value cache. The cache is a pool of pages of page_size slots,
+ *   k_pages, v_pages [num_pages, page_size, n_kv_heads, head_dim]  (v may be k)
+ *   weights          [num_pages, page_size] fp32, one per slot (optional)
+ * and a table of pages per sequence, block_table [batch, max_pages] int32: row j of
+ * a sequence lies in slot j % page_size of page block_table[b, j / page_size].
+ * Tables, lengths and the pool are device memory. A table entry outside [0,
+ * num_pages) is not read: its rows count as hidden, and DSA_DEVERR_CACHE is set in
+ * the device error word; lengths are clamped to [0, max_pages * page_size] with the
+ * same bit. Slots at or past a sequence's length may hold anything.
+ *
+ * Attention of one new token per sequence (its row is in the cache already):
+ *   q [batch, n_heads, head_dim], out alike (contiguous); lens [batch] int32: rows of
+ *   each sequence, the new token's included.
+ * The token sees rows j < lens[b], with window > 0 only j >= lens[b] - window or
+ * j < n_first. out, lse [batch, n_heads] (fp32 or NULL), sink and the numerics as
+ * dsa_window_attn_fwd. With weights, each visible row's slot gains sum_h e^(s_j -
+ * lse_h) (one add per row and sequence; the other slots are untouched).
+ * dtype: DSA_DTYPE_*. Strides in elements, host arrays or NULL for contiguous:
+ * q_strides (batch, head), k_strides and v_strides (page, slot, head). Supported:
+ * head_dim 64 or 128, n_heads / n_kv_heads <= 128, page_size a multiple of 8,
+ * max_pages * page_size <= 2^28, batch <= 65535. workspace:
+ * dsa_paged_attn_workspace_bytes(...) bytes (want_weights: weights is given),
+ * 256-byte aligned. No counterpart in the reference. */
+size_t dsa_paged_attn_workspace_bytes(int64_t batch, int n_heads, int n_kv_heads, int head_dim,
+                                      int64_t max_pages, int64_t page_size, int want_weights);
+int dsa_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* k_pages,
+                       const int64_t* k_strides, const void* v_pages, const int64_t* v_strides,
+                       const int* block_table, const int* lens, const float* sink, void* out,
+                       float* lse, float* weights, int dtype, int64_t batch, int n_heads,
+                       int n_kv_heads, int head_dim, int64_t num_pages, int64_t page_size,
+                       int64_t max_pages, int64_t window, int64_t n_first, float softmax_scale,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
