@@ -83,6 +83,12 @@ SIGNATURES = {
                                   _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i32, _i64,
                                   _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _f32, _c_void_p,
                                   _size_t, _c_void_p]),
+    "dsa_cache_append": (_i32, [_c_void_p, _i64p, _c_void_p, _i64p, _c_void_p, _i64p, _c_void_p,
+                                _i64p, _c_void_p, _c_void_p, _c_void_p, _i64, _i64, _i32, _i32,
+                                _i64, _i64, _i64, _c_void_p]),
+    "dsa_cache_evict": (_i32, [_c_void_p, _i64p, _c_void_p, _i64p, _c_void_p, _c_void_p, _c_void_p,
+                               _c_void_p, _c_void_p, _c_void_p, _i64, _i32, _i32, _i64, _i64, _i64,
+                               _i64, _i64, _i64, _i64, _c_void_p]),
 }
 
 _LIB = None

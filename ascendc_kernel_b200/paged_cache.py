@@ -5,7 +5,10 @@ the keys serve as values, as in :mod:`ascendc_kernel_b200.sparse_attn`) and, whe
 eviction is wanted, ``weights`` [num_pages, page_size] fp32: the attention that each row
 has gathered. ``block_table`` [b, max_pages] int32 names each sequence's pages.
 
+* :func:`cache_append` -- new rows into the pages
 * :func:`paged_attn`   -- one new token per sequence over the cache
+* :func:`cache_evict`  -- the rows that gathered most attention move to fresh pages
+* :class:`PagedKVCache` -- a pool with its tables and free pages, on which the three run
 
 Shape preconditions are checked with ``assert``; CUDA-level failures raise DsaError.
 """
@@ -17,7 +20,7 @@ import ctypes
 import torch
 
 from ._native import call, lib
-from .window_attn import DTYPES, _ptr, _sink_on
+from .window_attn import DTYPES, _ptr, _sink_on, _strided, _strides
 
 
 def _check_pool(k_pages, v_pages, weights, block_table):
@@ -103,3 +106,61 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor | N
              min(int(window), 1 << 28), min(int(n_first), 1 << 28), scale, ws.data_ptr(),
              ws.numel(), stream)
     return (out, lse) if return_lse else out
+
+
+def cache_append(k: torch.Tensor, v: torch.Tensor | None, k_pages: torch.Tensor,
+                 v_pages: torch.Tensor | None, block_table: torch.Tensor, start: torch.Tensor,
+                 weights: torch.Tensor | None = None) -> None:
+    """Writes k, v [b, t, hk, d] to rows start[b] .. start[b] + t - 1 of each sequence and
+    sets their slots' ``weights`` to 0. ``start`` int32 [b]. Rows past the table's room or
+    of pages that do not exist are not written (see ``_native.device_error``)."""
+    _check_pool(k_pages, v_pages, weights, block_table)
+    assert (v is None) == (v_pages is None), "v and v_pages are both given or both None"
+    b, t, hk, d = k.shape
+    n, page = k_pages.shape[:2]
+    assert (hk, d) == tuple(k_pages.shape[2:]) and k.dtype == k_pages.dtype \
+        and k.device == k_pages.device, "k must be [b, t, hk, d] of the pool's type and device"
+    if v is not None:
+        assert v.shape == k.shape and v.dtype == k.dtype and v.device == k.device
+    assert block_table.shape[0] == b
+    _check_lens(start, b, k.device, "start")
+    k = _strided(k)
+    v = None if v is None else _strided(v)
+    table, start = block_table.contiguous(), start.contiguous()
+    stream = torch.cuda.current_stream(k.device).cuda_stream
+    with torch.cuda.device(k.device):
+        call("dsa_cache_append", k.data_ptr(), _strides(k), _ptr(v),
+             None if v is None else _strides(v), k_pages.data_ptr(), _page_strides(k_pages),
+             _ptr(v_pages), None if v_pages is None else _page_strides(v_pages), _ptr(weights),
+             table.data_ptr(), start.data_ptr(), b, t, hk, d, n, page, table.shape[1], stream)
+
+
+def cache_evict(k_pages: torch.Tensor, v_pages: torch.Tensor | None, weights: torch.Tensor,
+                block_table: torch.Tensor, lens: torch.Tensor, dst_table: torch.Tensor, *,
+                budget: int, n_first: int = 0, n_recent: int = 0):
+    """Keeps at most ``budget`` rows of each sequence: the first ``n_first``, the last
+    ``n_recent`` and, of those between, the ones with the largest weights (equal weights:
+    the lower row). The kept rows and their weights are copied in ascending order to rows
+    0, 1, ... of the pages of ``dst_table`` [b, dst_pages] int32 (distinct pages that no
+    sequence of the call uses); the old pages stay as they are. Returns the kept rows
+    [b, budget] int32, filled up with -1, and the new lengths [b] int32."""
+    _check_pool(k_pages, v_pages, weights, block_table)
+    n, page, hk, d = k_pages.shape
+    b = block_table.shape[0]
+    assert weights is not None, "eviction goes by the weights"
+    _check_lens(lens, b, k_pages.device)
+    assert dst_table.dtype == torch.int32 and dst_table.dim() == 2 and dst_table.shape[0] == b \
+        and dst_table.device == k_pages.device, "dst_table must be int32 [b, dst_pages]"
+    assert budget >= 1 and n_first >= 0 and n_recent >= 0 and n_first + n_recent <= budget, \
+        "n_first + n_recent <= budget"
+    assert budget <= dst_table.shape[1] * page, "dst_table has no room for budget rows"
+    table, lens, dst = block_table.contiguous(), lens.contiguous(), dst_table.contiguous()
+    kept = torch.empty(b, budget, dtype=torch.int32, device=k_pages.device)
+    left = torch.empty(b, dtype=torch.int32, device=k_pages.device)
+    stream = torch.cuda.current_stream(k_pages.device).cuda_stream
+    with torch.cuda.device(k_pages.device):
+        call("dsa_cache_evict", k_pages.data_ptr(), _page_strides(k_pages), _ptr(v_pages),
+             None if v_pages is None else _page_strides(v_pages), weights.data_ptr(),
+             table.data_ptr(), lens.data_ptr(), dst.data_ptr(), kept.data_ptr(), left.data_ptr(),
+             b, hk, d, n, page, table.shape[1], dst.shape[1], budget, n_first, n_recent, stream)
+    return kept, left

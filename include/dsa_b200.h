@@ -409,6 +409,41 @@ int dsa_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* k_pa
                        int64_t max_pages, int64_t window, int64_t n_first, float softmax_scale,
                        void* workspace, size_t workspace_bytes, void* stream);
 
+/* Writes k, v [batch, t, n_kv_heads, head_dim] (2-byte elements, 16-byte aligned) to
+ * rows start[b] .. start[b] + t - 1 of each sequence and sets those slots' weights (if
+ * given) to 0. v and v_pages are both NULL when the keys serve as values. Strides in
+ * elements, NULL for contiguous: k_strides, v_strides (batch, token, head), kp_strides,
+ * vp_strides (page, slot, head). A row outside the table's room, or of a page that
+ * does not exist, is not written (DSA_DEVERR_CACHE). Two rows of one call must not
+ * name one slot. Supported: head_dim a multiple of 8 and <= 1024, strides multiples
+ * of 8. No counterpart in the reference. */
+int dsa_cache_append(const void* k, const int64_t* k_strides, const void* v,
+                     const int64_t* v_strides, void* k_pages, const int64_t* kp_strides,
+                     void* v_pages, const int64_t* vp_strides, float* weights,
+                     const int* block_table, const int* start, int64_t batch, int64_t t,
+                     int n_kv_heads, int head_dim, int64_t num_pages, int64_t page_size,
+                     int64_t max_pages, void* stream);
+
+/* Eviction by accumulated attention weight. Of each sequence's lens[b] rows at most
+ * `budget` stay: all when lens[b] <= budget; else the first n_first, the last n_recent
+ * and of the rows between those with the largest weights (equal weights: the lower
+ * row; NaN counts as the largest). kept [batch, budget] int32 receives the kept rows in
+ * ascending order, then -1, and new_lens [batch] their number. The kept rows' K, V and
+ * weights are copied, in that order, to rows 0, 1, ... of the pages that dst_table
+ * [batch, dst_pages] names; the weights of these pages' other slots are set to 0. The
+ * old pages are left as they are. The pages of dst_table must be distinct and belong to
+ * no sequence of the call. A dst_table entry that names no page: its rows are not
+ * copied (DSA_DEVERR_CACHE); the same for rows of block_table entries that name none
+ * (their weights rank below all others). Requires n_first + n_recent <= budget <=
+ * dst_pages * page_size, max_pages * page_size <= 2^28, batch <= 65535. Exact and
+ * deterministic. No counterpart in the reference. */
+int dsa_cache_evict(void* k_pages, const int64_t* kp_strides, void* v_pages,
+                    const int64_t* vp_strides, float* weights, const int* block_table,
+                    const int* lens, const int* dst_table, int* kept, int* new_lens, int64_t batch,
+                    int n_kv_heads, int head_dim, int64_t num_pages, int64_t page_size,
+                    int64_t max_pages, int64_t dst_pages, int64_t budget, int64_t n_first,
+                    int64_t n_recent, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
