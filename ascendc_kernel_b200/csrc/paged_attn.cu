@@ -27,7 +27,7 @@
 // moves (O and the sums are rescaled) only when a score exceeds it by more than
 // 2^8, so the common chunk needs one vote and no reduction over keys; the sums
 // stay per thread until the piece ends. P is rounded to the operands' type
-// (relative 2^-9 for bf16, the size of the output's own rounding); sums are fp32.
+// (relative 2^-8 at most for bf16, the size of the output's own rounding); sums are fp32.
 // TMEM: S^T of warpgroup w [w NM, +NM), O^T [2 NM + w NM, +NM).
 #include "host_util.h"
 #include "window_common.cuh"

@@ -14,7 +14,7 @@
 //                       atomics, whose order would change results from run to run
 //   window_dsink_*      the rows' sink terms summed in a fixed order
 // P and dS are rounded to the operands' 16-bit type for the products that sum
-// over them (relative 2^-9 for bf16, the size of the gradients' own rounding);
+// over them (relative 2^-8 at most for bf16, the size of the gradients' own rounding);
 // every sum is fp32. D comes from the rounded out; the sink's gradient, an fp32
 // output, uses the unrounded D = sum_j P_j (dout.v_j) that the dq kernel sees.
 #include "host_util.h"

@@ -18,7 +18,7 @@
 //   warps 4..11 softmax: a warpgroup per tile, a thread per row: no exchange
 //               between threads for the row's maximum and sum.
 // P is rounded to the operands' 16-bit type for the second product (its sum is
-// taken before the rounding, in fp32): a relative 2^-9 (2^-12 for fp16) a term,
+// taken before the rounding, in fp32): a relative 2^-8 (2^-11 for fp16) a term at most,
 // the size of the output's own rounding. The reference moves, and O is rescaled,
 // only when a row's maximum exceeds it by more than 2^8, so P stays within fp16.
 // TMEM per tile w: S/P columns [256w, 256w+128), O columns [256w+128, 256w+128+D).
@@ -311,9 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // rows past the tile's tokens follow its last one: their values are not used
       const int pos = min(t, it.t1[w] - 1) + p.s.n - p.s.m;
       const int gh = it.kvh * p.s.g + head;
-      const bool has_sink = p.sink != nullptr && tok < p.grid.tt;
-      const float sink2 = has_sink ? __ldg(p.sink + gh) * kLog2e : -INFINITY;
-      float m = sink2, l = 0.f;
+      float m = -INFINITY, l = 0.f;
       for (int c = first; c <= last; ++c) {
         if (!it.active<kChunkBlks>(p.s, w, c)) continue;
         const int nb = it.blocks<kChunkBlks>(c);
@@ -398,10 +396,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++gc;
       }
       if (!ok) break;
-      // ---- epilogue: O / (l + sink term)
-      const float ref = m == -INFINITY ? 0.f : m;
-      const float total = l + (has_sink ? ex2_approx(sink2 - ref) : 0.f);
-      const float inv = total > 0.f ? 1.0f / total : (total == 0.f ? 0.f : total);
+      // ---- epilogue: O / (l + sink term), both relative to the larger of the reference
+      // and the sink
+      const float sink2 =
+          p.sink != nullptr && tok < p.grid.tt ? __ldg(p.sink + gh) * kLog2e : -INFINITY;
+      const float top = fmaxf(m, sink2);
+      const float ref = top == -INFINITY ? 0.f : top;
+      const float mine = ex2_approx(m - ref);  // 0 when no key was seen
+      const float total = fmaf(l, mine, ex2_approx(sink2 - ref));
+      const float inv = total == 0.f ? 0.f : mine / total;
       const int64_t orow = (static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + gh;
       if (last >= 0) {
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&o_done[w], (gc - 1) & 1, abort_flag, p.err,

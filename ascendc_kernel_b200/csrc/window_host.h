@@ -33,7 +33,7 @@ inline int read_strides(const int64_t* given, int64_t batch, int64_t tokens, int
   s.h = d;
   s.t = static_cast<int64_t>(heads) * d;
   s.b = tokens * s.t;
-  if (given != nullptr) {
+  if (given != nullptr && batch > 0 && tokens > 0) {
     if (batch > 1) s.b = given[0];
     if (tokens > 1) s.t = given[1];
     if (heads > 1) s.h = given[2];

@@ -164,3 +164,92 @@ def cache_evict(k_pages: torch.Tensor, v_pages: torch.Tensor | None, weights: to
              table.data_ptr(), lens.data_ptr(), dst.data_ptr(), kept.data_ptr(), left.data_ptr(),
              b, hk, d, n, page, table.shape[1], dst.shape[1], budget, n_first, n_recent, stream)
     return kept, left
+
+
+class PagedKVCache:
+    """A pool of pages with the tables, lengths and free pages of a batch of sequences.
+
+    Page numbers and lengths are kept on the host as well, so no call waits for the GPU;
+    the pool is used on the caller's current stream, in call order. ``shared`` holds one
+    tensor that serves as keys and values; ``track_weights`` holds the attention each row
+    gathers (needed for :meth:`evict`).
+    """
+
+    def __init__(self, batch: int, num_pages: int, page_size: int, max_len: int, n_kv_heads: int,
+                 head_dim: int, *, shared: bool = False, track_weights: bool = False,
+                 dtype: torch.dtype = torch.bfloat16, device="cuda"):
+        assert page_size >= 8 and page_size % 8 == 0, "page_size must be a multiple of 8"
+        assert batch >= 1 and num_pages >= 1 and max_len >= 1
+        self.batch, self.page_size, self.max_len = batch, page_size, max_len
+        shape = (num_pages, page_size, n_kv_heads, head_dim)
+        self.k_pages = torch.zeros(shape, dtype=dtype, device=device)
+        self.v_pages = None if shared else torch.zeros(shape, dtype=dtype, device=device)
+        self.weights = (torch.zeros(num_pages, page_size, dtype=torch.float32, device=device)
+                        if track_weights else None)
+        self.max_pages = -(-max_len // page_size)
+        self.block_table = torch.full((batch, self.max_pages), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.host_lens = [0] * batch
+        self.pages = [[] for _ in range(batch)]
+        self.free = list(range(num_pages - 1, -1, -1))
+
+    def _take(self, count: int) -> list[int]:
+        if count > len(self.free):
+            raise RuntimeError(f"the page pool is exhausted: {count} pages wanted, "
+                               f"{len(self.free)} free")
+        taken = self.free[len(self.free) - count:][::-1]
+        del self.free[len(self.free) - count:]
+        return taken
+
+    def _upload(self, rows: list[list[int]], width: int) -> torch.Tensor:
+        flat = torch.tensor([r + [-1] * (width - len(r)) for r in rows], dtype=torch.int32)
+        return flat.to(self.block_table.device)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor | None = None) -> None:
+        """Adds the next rows k, v [batch, t, hk, d] of every sequence."""
+        t = k.shape[1]
+        assert k.shape[0] == self.batch
+        need = []
+        for i in range(self.batch):
+            assert self.host_lens[i] + t <= self.max_len, "sequence longer than max_len"
+            need.append(-(-(self.host_lens[i] + t) // self.page_size) - len(self.pages[i]))
+        taken = self._take(sum(max(n, 0) for n in need))
+        if taken:
+            for i, n in enumerate(need):
+                if n > 0:
+                    self.pages[i] += taken[:n]
+                    del taken[:n]
+            self.block_table.copy_(self._upload(self.pages, self.max_pages))
+        cache_append(k, v, self.k_pages, self.v_pages, self.block_table, self.lens, self.weights)
+        self.lens += t
+        self.host_lens = [n + t for n in self.host_lens]
+
+    def attend(self, q: torch.Tensor, sink: torch.Tensor | None = None, *, window: int = 0,
+               n_first: int = 0, softmax_scale: float | None = None) -> torch.Tensor:
+        """:func:`paged_attn` of q [batch, h, d] over the cache; the weights, where they are
+        tracked, gain this step's attention."""
+        return paged_attn(q, self.k_pages, self.v_pages, self.block_table, self.lens, sink,
+                          window=window, n_first=n_first, softmax_scale=softmax_scale,
+                          weights=self.weights)
+
+    def evict(self, budget: int, n_first: int = 0, n_recent: int = 0) -> torch.Tensor:
+        """:func:`cache_evict` of every sequence to at most ``budget`` rows. The old pages
+        are free again; returns the kept rows [batch, budget] int32, filled up with -1."""
+        assert self.weights is not None, "eviction needs track_weights"
+        width = -(-budget // self.page_size)
+        after = [min(n, budget) for n in self.host_lens]
+        need = [-(-n // self.page_size) for n in after]
+        flat, fresh = self._take(sum(need)), []
+        for n in need:
+            fresh.append(flat[:n])
+            del flat[:n]
+        kept, left = cache_evict(self.k_pages, self.v_pages, self.weights, self.block_table,
+                                 self.lens, self._upload(fresh, width), budget=budget,
+                                 n_first=n_first, n_recent=n_recent)
+        self.host_lens = after
+        for old in self.pages:
+            self.free += old
+        self.pages = fresh
+        self.block_table.copy_(self._upload(self.pages, self.max_pages))
+        self.lens.copy_(left)
+        return kept

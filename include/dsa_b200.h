@@ -432,9 +432,9 @@ int dsa_cache_append(const void* k, const int64_t* k_strides, const void* v,
  * weights are copied, in that order, to rows 0, 1, ... of the pages that dst_table
  * [batch, dst_pages] names; the weights of these pages' other slots are set to 0. The
  * old pages are left as they are. The pages of dst_table must be distinct and belong to
- * no sequence of the call. A dst_table entry that names no page: its rows are not
- * copied (DSA_DEVERR_CACHE); the same for rows of block_table entries that name none
- * (their weights rank below all others). Requires n_first + n_recent <= budget <=
+ * no sequence of the call; entries past the kept rows may name none (-1). A kept row
+ * whose dst_table entry names no page is not copied (DSA_DEVERR_CACHE); the same for
+ * rows of block_table entries that name none (their weights rank below all others). Requires n_first + n_recent <= budget <=
  * dst_pages * page_size, max_pages * page_size <= 2^28, batch <= 65535. Exact and
  * deterministic. No counterpart in the reference. */
 int dsa_cache_evict(void* k_pages, const int64_t* kp_strides, void* v_pages,
