@@ -7,9 +7,12 @@
 // rows move in ascending order to rows 0, 1, ... of fresh pages: the old pages stay as
 // they are (other sequences may share them), and nothing is read after it was
 // overwritten.
-//   evict_select_kernel  a block per sequence: radix select of the threshold over the
+//   evict_select_kernel  a cluster per sequence: radix select of the threshold over the
 //                        32 bits of the orderable weight, then one ordered pass
 //   evict_copy_kernel    rows and weights to their new slots, HBM bound
+#include <cooperative_groups.h>
+
+#include "common.cuh"
 #include "host_util.h"
 
 namespace dsa {
@@ -31,49 +34,125 @@ __device__ __forceinline__ int lookup(const Pool& p, const int* table, int64_t m
   return page >= 0 && page < p.num_pages ? page : -1;
 }
 
+// ------------------------------------------------------------------ row copies
+constexpr int kCopyThreads = 256;
+constexpr int kAhead = 8;       // 16-byte loads in flight per thread
+constexpr int kCopyRows = 16;   // rows of a block, at most
+
+// Byte offsets of one row's source and target in K and V; -1: the row is not copied.
+struct RowPlan {
+  int64_t src[2][kCopyRows], dst[2][kCopyRows];
+};
+
+struct RowCopy {
+  const uint8_t* src[2];  // K, V
+  uint8_t* dst[2];
+  int64_t src_head[2], dst_head[2];  // bytes from head to head
+  int kinds, rows;        // tensors; rows of the block
+  int units, row16;       // 16-byte units of a row (all heads) and of a head
+  uint32_t magic_units, magic_row16;  // floor(2^32 / x) + 1
+};
+
+// i / x for i * x < 2^32, from magic = floor(2^32 / x) + 1 (x > 1; x = 1: magic 0)
+__host__ __device__ __forceinline__ uint32_t div_magic(uint32_t x) {
+  return x == 1 ? 0u : 0xFFFFFFFFu / x + 1u;
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t i, uint32_t magic) {
+  return magic == 0u ? i : __umulhi(i, magic);
+}
+
+// The block's rows, a thread 16 bytes at a time with kAhead loads in flight, units of a
+// row on neighbouring threads. Flat: a row's heads follow one another without a gap on
+// both sides, so a unit's offset is its number.
+template <bool Flat>
+__device__ __forceinline__ void copy_rows(const RowCopy& c, const RowPlan& plan) {
+  const int total = c.rows * c.units;
+  for (int kind = 0; kind < c.kinds; ++kind) {
+    const uint8_t* src = c.src[kind];
+    uint8_t* dst = c.dst[kind];
+    for (int i0 = threadIdx.x; i0 < total; i0 += kCopyThreads * kAhead) {
+      uint4 x[kAhead];
+      int64_t to[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        const int i = i0 + k * kCopyThreads;
+        to[k] = -1;
+        if (i < total) {
+          const int row = static_cast<int>(div_by(i, c.magic_units));
+          const int u = i - row * c.units;
+          const int64_t from = plan.src[kind][row];
+          if (from >= 0) {
+            int64_t a = u * 16, b = u * 16;
+            if (!Flat) {
+              const int head = static_cast<int>(div_by(u, c.magic_row16));
+              a = head * c.src_head[kind] + (u - head * c.row16) * 16;
+              b = head * c.dst_head[kind] + (u - head * c.row16) * 16;
+            }
+            x[k] = __ldcs(reinterpret_cast<const uint4*>(src + from + a));
+            to[k] = plan.dst[kind][row] + b;
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        if (to[k] >= 0) *reinterpret_cast<uint4*>(dst + to[k]) = x[k];
+    }
+  }
+}
+
+// Rows of a block: few enough that the call fills the GPU's thread slots about twice,
+// one at least.
+inline int rows_per_block(int64_t rows) {
+  const int64_t r = rows / (2 * 148 * 8);
+  return static_cast<int>(r < 1 ? 1 : (r > kCopyRows ? kCopyRows : r));
+}
+
 // ------------------------------------------------------------------ append
 struct AppendParams {
   Pool pool;
-  const uint8_t* k;
-  const uint8_t* v;
-  int64_t ks[3], vs[3];  // (batch, token, head) strides in bytes
+  RowCopy copy;
+  int64_t ks[2], vs[2];  // (batch, token) strides of the new rows in bytes
   const int* table;
   const int* start;
   int64_t max_pages;
   int64_t batch, t;
 };
 
-// A thread per 16-byte unit of a row; blockIdx.y: K or V.
-__global__ void __launch_bounds__(256) cache_append_kernel(const AppendParams p) {
-  const int units = p.pool.hk * p.pool.row16;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t r = i / units;
-  if (r >= p.batch * p.t) return;
-  const int u = static_cast<int>(i - r * units);
-  const int64_t b = r / p.t, t = r - b * p.t;
-  const int64_t row = static_cast<int64_t>(__ldg(p.start + b)) + t;
-  const bool room = row >= 0 && row < p.max_pages * p.pool.page;
-  const int page = room ? lookup(p.pool, p.table, p.max_pages, b, row) : -1;
-  if (page < 0) {
-    if (u == 0) atomicOr(p.pool.err, DSA_DEVERR_CACHE);
-    return;
+template <bool Flat>
+__global__ void __launch_bounds__(kCopyThreads) cache_append_kernel(const AppendParams p) {
+  __shared__ RowPlan plan;
+  if (threadIdx.x < p.copy.rows) {
+    const int64_t r = static_cast<int64_t>(blockIdx.x) * p.copy.rows + threadIdx.x;
+    int64_t s[2] = {-1, -1}, d[2] = {-1, -1};
+    if (r < p.batch * p.t) {
+      const int64_t b = r / p.t, t = r - b * p.t;
+      const int64_t row = static_cast<int64_t>(__ldg(p.start + b)) + t;
+      const bool room = row >= 0 && row < p.max_pages * p.pool.page;
+      const int64_t page = room ? lookup(p.pool, p.table, p.max_pages, b, row) : -1;
+      if (page < 0) {
+        atomicOr(p.pool.err, DSA_DEVERR_CACHE);
+      } else {
+        const int64_t slot = row % p.pool.page;
+        s[0] = b * p.ks[0] + t * p.ks[1];
+        s[1] = b * p.vs[0] + t * p.vs[1];
+        d[0] = page * p.pool.ks[0] + slot * p.pool.ks[1];
+        d[1] = page * p.pool.vs[0] + slot * p.pool.vs[1];
+        if (p.pool.weights != nullptr) p.pool.weights[page * p.pool.page + slot] = 0.f;
+      }
+    }
+    for (int k = 0; k < 2; ++k) {
+      plan.src[k][threadIdx.x] = s[k];
+      plan.dst[k][threadIdx.x] = d[k];
+    }
   }
-  const int slot = static_cast<int>(row % p.pool.page);
-  const int head = u / p.pool.row16, x = u - head * p.pool.row16;
-  const bool second = blockIdx.y == 1;
-  const int64_t* ss = second ? p.vs : p.ks;
-  const int64_t* ds = second ? p.pool.vs : p.pool.ks;
-  const uint8_t* src = (second ? p.v : p.k) + b * ss[0] + t * ss[1] + head * ss[2] + x * 16;
-  uint8_t* dst =
-      (second ? p.pool.v : p.pool.k) + page * ds[0] + slot * ds[1] + head * ds[2] + x * 16;
-  *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
-  if (u == 0 && !second && p.pool.weights != nullptr)
-    p.pool.weights[static_cast<int64_t>(page) * p.pool.page + slot] = 0.f;
+  __syncthreads();
+  copy_rows<Flat>(p.copy, plan);
 }
 
 // ------------------------------------------------------------------ evict
 struct EvictParams {
   Pool pool;
+  RowCopy copy;
   const int* table;      // [batch, max_pages]
   const int* lens;       // [batch]
   const int* dst_table;  // [batch, dst_pages]
@@ -81,10 +160,13 @@ struct EvictParams {
   int budget, n_first, n_recent;
   int* kept;             // [batch, budget]: kept rows ascending, then -1
   int* new_lens;         // [batch]
+  int staged;            // rows of the select kernel's shared memory
 };
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 512;
 constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kSelMaxCluster = 8;
+constexpr int kSelStaged = 48 * 1024;  // rows of a block whose weights fit in shared memory
 
 // Orderable bits of a weight: larger weights have larger bits, NaN the largest.
 __device__ __forceinline__ uint32_t order_bits(float w) {
@@ -93,58 +175,102 @@ __device__ __forceinline__ uint32_t order_bits(float w) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
+// A cluster of 1, 2, 4 or 8 blocks per sequence (select_cluster), each with a contiguous
+// stretch of its rows. Latency bound: the weights are read once through the table and
+// staged; each pass is a few shared-memory atomics per thread, one cluster barrier and
+// the sum of the blocks' 256 counts over distributed shared memory.
 __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictParams p) {
-  __shared__ int hist[256];
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  __shared__ int hist[2][256];  // passes alternate, so one barrier a pass is enough
+  __shared__ int total[256];
   __shared__ int warp_gt[kSelWarps], warp_eq[kSelWarps];
+  __shared__ int block_gt, block_eq;
   __shared__ uint32_t sh_prefix;
   __shared__ int sh_need;
-  const int b = blockIdx.x;
+  extern __shared__ uint32_t staged[];
+  const int blocks = static_cast<int>(cluster.num_blocks());
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int b = blockIdx.x / blocks;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int ctid = rank * kSelThreads + tid, cthreads = blocks * kSelThreads;
   const int64_t room = p.max_pages * p.pool.page;
   int len = __ldg(p.lens + b);
-  if (tid == 0 && (len < 0 || len > room)) atomicOr(p.pool.err, DSA_DEVERR_CACHE);
+  if (ctid == 0 && (len < 0 || len > room)) atomicOr(p.pool.err, DSA_DEVERR_CACHE);
   len = max(len, 0);
   if (len > room) len = static_cast<int>(room);
   int* kept = p.kept + static_cast<int64_t>(b) * p.budget;
   const int left = min(len, p.budget);
-  if (tid == 0) p.new_lens[b] = left;
-  for (int i = left + tid; i < p.budget; i += kSelThreads) kept[i] = -1;
+  if (ctid == 0) p.new_lens[b] = left;
+  for (int i = left + ctid; i < p.budget; i += cthreads) kept[i] = -1;
   if (len <= p.budget) {
-    for (int i = tid; i < len; i += kSelThreads) kept[i] = i;
+    for (int i = ctid; i < len; i += cthreads) kept[i] = i;
     return;
   }
-  const int a = p.n_first, e = len - p.n_recent;  // the rows between, e - a > need >= 0
-  for (int i = tid; i < a; i += kSelThreads) kept[i] = i;
-  for (int i = tid; i < p.n_recent; i += kSelThreads) kept[p.budget - p.n_recent + i] = e + i;
+  const int e = len - p.n_recent;  // rows [n_first, e) compete; more than need >= 0
+  for (int i = ctid; i < p.n_first; i += cthreads) kept[i] = i;
+  for (int i = ctid; i < p.n_recent; i += cthreads) kept[p.budget - p.n_recent + i] = e + i;
   int need = p.budget - p.n_first - p.n_recent;
   if (need == 0) return;
+  // this block's rows: [a, a + n)
+  const int64_t all = e - p.n_first;
+  const int a = p.n_first + static_cast<int>(all * rank / blocks);
+  const int n = p.n_first + static_cast<int>(all * (rank + 1) / blocks) - a;
   // an entry of the table that names no page: its rows rank below every weight
-  auto bits_of = [&](int row) -> uint32_t {
+  auto read = [&](int i) -> uint32_t {
+    const int row = a + i;
     const int page = lookup(p.pool, p.table, p.max_pages, b, row);
     return page < 0 ? 0u
                     : order_bits(p.pool.weights[static_cast<int64_t>(page) * p.pool.page +
                                                 row % p.pool.page]);
   };
+  // the weights are read once through the table, and the passes below run on the copy; a
+  // stretch that does not fit is read again in each pass
+  const bool whole = n <= p.staged;
+  if (whole) {
+    for (int i0 = tid; i0 < n; i0 += 8 * kSelThreads) {
+      uint32_t u[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) u[k] = i0 + k * kSelThreads < n ? read(i0 + k * kSelThreads) : 0u;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (i0 + k * kSelThreads < n) staged[i0 + k * kSelThreads] = u[k];
+    }
+  }
+  auto bits_of = [&](int i) -> uint32_t { return whole ? staged[i] : read(i); };
+  for (int i = tid; i < 512; i += kSelThreads) (&hist[0][0])[i] = 0;
+  __syncthreads();
   // ---- the need-th largest value, a byte a pass from the top
   uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i0 = a; i0 < e; i0 += kSelThreads) {
-      const int row = i0 + tid;
-      bool in = row < e;
+  for (int shift = 24, pass = 0; shift >= 0; shift -= 8, ++pass) {
+    int* mine = hist[pass & 1];
+    for (int i0 = 0; i0 < n; i0 += kSelThreads) {
+      const int i = i0 + tid;
+      bool in = i < n;
       uint32_t u = 0;
       if (in) {
-        u = bits_of(row);
+        u = bits_of(i);
         in = shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8));
       }
       const uint32_t live = __ballot_sync(0xFFFFFFFFu, in);
       if (in) {
-        // one add per distinct byte of the warp: many weights are alike
+        // many weights are alike: a warp whose rows share the byte adds once
         const uint32_t digit = (u >> shift) & 255u;
-        const uint32_t same = __match_any_sync(live, digit);
-        if (lane == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+        int same;
+        __match_all_sync(live, digit, &same);
+        if (!same)
+          atomicAdd(&mine[digit], 1);
+        else if (lane == __ffs(live) - 1)
+          atomicAdd(&mine[digit], __popc(live));
       }
+    }
+    cluster.sync();
+    for (int i = tid; i < 256; i += kSelThreads) {
+      int sum = 0;
+      for (int r = 0; r < blocks; ++r) sum += cluster.map_shared_rank(mine, r)[i];
+      total[i] = sum;
+      // the other buffer was read before this barrier; the next pass counts into it
+      hist[(pass & 1) ^ 1][i] = 0;
     }
     __syncthreads();
     if (warp == 0) {
@@ -152,7 +278,7 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
       int c[8], sum = 0;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        c[k] = hist[255 - 8 * lane - k];
+        c[k] = total[255 - 8 * lane - k];
         sum += c[k];
       }
       int incl = sum;
@@ -181,13 +307,12 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
   }
   // ---- rows above the threshold and the first `need` equal to it, in order: a warp a
   // contiguous stretch
-  const int n = e - a;
   const int stretch = (n + kSelWarps - 1) / kSelWarps;
   const int w0 = min(warp * stretch, n), w1 = min(w0 + stretch, n);
   int gt = 0, eq = 0;
   for (int i0 = w0; i0 < w1; i0 += 32) {
     const bool in = i0 + lane < w1;
-    const uint32_t u = in ? bits_of(a + i0 + lane) : 0u;
+    const uint32_t u = in ? bits_of(i0 + lane) : 0u;
     gt += __popc(__ballot_sync(0xFFFFFFFFu, in && u > prefix));
     eq += __popc(__ballot_sync(0xFFFFFFFFu, in && u == prefix));
   }
@@ -196,7 +321,20 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
     warp_eq[warp] = eq;
   }
   __syncthreads();
+  if (warp == 0) {
+    const int g = __reduce_add_sync(0xFFFFFFFFu, lane < kSelWarps ? warp_gt[lane] : 0);
+    const int q = __reduce_add_sync(0xFFFFFFFFu, lane < kSelWarps ? warp_eq[lane] : 0);
+    if (lane == 0) {
+      block_gt = g;
+      block_eq = q;
+    }
+  }
+  cluster.sync();
   gt = eq = 0;
+  for (int r = 0; r < rank; ++r) {
+    gt += *cluster.map_shared_rank(&block_gt, r);
+    eq += *cluster.map_shared_rank(&block_eq, r);
+  }
   for (int i = 0; i < warp; ++i) {
     gt += warp_gt[i];
     eq += warp_eq[i];
@@ -204,38 +342,44 @@ __global__ void __launch_bounds__(kSelThreads) evict_select_kernel(const EvictPa
   const uint32_t below = (1u << lane) - 1u;
   for (int i0 = w0; i0 < w1; i0 += 32) {
     const bool in = i0 + lane < w1;
-    const uint32_t u = in ? bits_of(a + i0 + lane) : 0u;
+    const uint32_t u = in ? bits_of(i0 + lane) : 0u;
     const uint32_t mg = __ballot_sync(0xFFFFFFFFu, in && u > prefix);
     const uint32_t me = __ballot_sync(0xFFFFFFFFu, in && u == prefix);
     const int g = gt + __popc(mg & below), q = eq + __popc(me & below);
-    if (in && (u > prefix || (u == prefix && q < need))) kept[a + g + min(q, need)] = a + i0 + lane;
+    if (in && (u > prefix || (u == prefix && q < need)))
+      kept[p.n_first + g + min(q, need)] = a + i0 + lane;
     gt += __popc(mg);
     eq += __popc(me);
   }
+  cluster.sync();  // no block leaves while another reads its counts
 }
 
-constexpr int kCopyThreads = 256;
+// Blocks of a sequence's cluster: a block per 1024 rows of the table's room, as long as
+// all clusters fit the GPU (2 blocks an SM) at once.
+inline int select_cluster(int64_t batch, int64_t room) {
+  int c = 1;
+  while (c < kSelMaxCluster && room > 1024 * c && batch * 2 * c <= 2 * 148) c *= 2;
+  return c;
+}
 
-// A block copies kCopyRows rows of a sequence's fresh pages, K and V, and their weights.
-constexpr int kCopyRows = 16;
-
+// A block copies copy.rows rows of a sequence's fresh pages, K and V, and their weights.
+template <bool Flat>
 __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictParams p) {
-  __shared__ int64_t src_at[2][kCopyRows], dst_at[2][kCopyRows];  // byte offsets, -1: no copy
+  __shared__ RowPlan plan;
   const int b = blockIdx.y;
-  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kCopyRows;
-  const int left = p.new_lens[b];
-  if (threadIdx.x < kCopyRows) {
+  const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.copy.rows;
+  if (threadIdx.x < p.copy.rows) {
+    const int left = p.new_lens[b];
     const int64_t row = r0 + threadIdx.x;
     int64_t s[2] = {-1, -1}, d[2] = {-1, -1};
     if (row < p.dst_pages * p.pool.page) {
-      const int dp = lookup(p.pool, p.dst_table, p.dst_pages, b, row);
-      const int ds = static_cast<int>(row % p.pool.page);
+      const int64_t dp = lookup(p.pool, p.dst_table, p.dst_pages, b, row);
+      const int64_t ds = row % p.pool.page;
       float weight = 0.f;
-      int sp = -1;
       if (row < left) {
         const int from = p.kept[static_cast<int64_t>(b) * p.budget + row];
-        sp = lookup(p.pool, p.table, p.max_pages, b, from);
-        const int ss = from % p.pool.page;
+        const int64_t sp = lookup(p.pool, p.table, p.max_pages, b, from);
+        const int64_t ss = from % p.pool.page;
         if (sp < 0 || dp < 0) {
           atomicOr(p.pool.err, DSA_DEVERR_CACHE);
         } else {
@@ -243,45 +387,18 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictPar
           s[1] = sp * p.pool.vs[0] + ss * p.pool.vs[1];
           d[0] = dp * p.pool.ks[0] + ds * p.pool.ks[1];
           d[1] = dp * p.pool.vs[0] + ds * p.pool.vs[1];
-          weight = p.pool.weights[static_cast<int64_t>(sp) * p.pool.page + ss];
+          weight = p.pool.weights[sp * p.pool.page + ss];
         }
       }
-      if (dp >= 0) p.pool.weights[static_cast<int64_t>(dp) * p.pool.page + ds] = weight;
+      if (dp >= 0) p.pool.weights[dp * p.pool.page + ds] = weight;
     }
     for (int k = 0; k < 2; ++k) {
-      src_at[k][threadIdx.x] = s[k];
-      dst_at[k][threadIdx.x] = d[k];
+      plan.src[k][threadIdx.x] = s[k];
+      plan.dst[k][threadIdx.x] = d[k];
     }
   }
   __syncthreads();
-  const int units = p.pool.hk * p.pool.row16;
-  const int kinds = p.pool.v == nullptr ? 1 : 2;
-  constexpr int kAhead = 8;  // loads in flight per thread
-  const int total = kinds * kCopyRows * units;
-  for (int i0 = threadIdx.x; i0 < total; i0 += kCopyThreads * kAhead) {
-    uint4 x[kAhead];
-    uint8_t* to[kAhead];
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const int i = i0 + k * kCopyThreads;
-      to[k] = nullptr;
-      if (i < total) {
-        const int kind = i / (kCopyRows * units);
-        const int y = i - kind * kCopyRows * units;
-        const int row = y / units, u = y - row * units;
-        const int head = u / p.pool.row16;
-        const int64_t at = (kind ? p.pool.vs[2] : p.pool.ks[2]) * head + (u - head * p.pool.row16) * 16;
-        uint8_t* base = kind ? p.pool.v : p.pool.k;
-        if (src_at[kind][row] >= 0) {
-          x[k] = *reinterpret_cast<const uint4*>(base + src_at[kind][row] + at);
-          to[k] = base + dst_at[kind][row] + at;
-        }
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k)
-      if (to[k] != nullptr) *reinterpret_cast<uint4*>(to[k]) = x[k];
-  }
+  copy_rows<Flat>(p.copy, plan);
 }
 
 // ------------------------------------------------------------------ host
@@ -304,7 +421,8 @@ inline int byte_strides(const int64_t* given, int64_t a, int64_t b, int heads, i
 inline int make_pool(void* k, const int64_t* k_strides, void* v, const int64_t* v_strides,
                      float* weights, int64_t num_pages, int64_t page, int heads, int d, Pool* p) {
   if (num_pages < 1 || page < 1 || heads < 1) return DSA_ERR_INVALID_ARGUMENT;
-  if (d < 8 || d % 8 != 0 || d > 1024 || heads > 4096 || page > (1 << 20) || num_pages > 0x7FFFFFFF)
+  // rows of at most 16383 units keep the divisions of copy_rows exact
+  if (d < 8 || d % 8 != 0 || d > 1024 || static_cast<int64_t>(heads) * (d / 8) > 16383 || page > (1 << 20) || num_pages > 0x7FFFFFFF)
     return DSA_ERR_UNSUPPORTED;
   if (!aligned16(k) || !aligned16(v)) return DSA_ERR_MISALIGNED;
   p->k = static_cast<uint8_t*>(k);
@@ -318,6 +436,29 @@ inline int make_pool(void* k, const int64_t* k_strides, void* v, const int64_t* 
   p->hk = heads;
   p->row16 = d / 8;
   return DSA_OK;
+}
+
+// The pool's side of a copy of `rows` rows; the source is the caller's to fill in.
+inline RowCopy row_copy(const Pool& p, int64_t rows) {
+  RowCopy c;
+  c.dst[0] = p.k;
+  c.dst[1] = p.v;
+  c.dst_head[0] = p.ks[2];
+  c.dst_head[1] = p.vs[2];
+  c.kinds = p.v != nullptr ? 2 : 1;
+  c.rows = rows_per_block(rows);
+  c.row16 = p.row16;
+  c.units = p.hk * p.row16;
+  c.magic_units = div_magic(c.units);
+  c.magic_row16 = div_magic(c.row16);
+  return c;
+}
+
+inline bool flat_rows(const RowCopy& c) {
+  for (int k = 0; k < c.kinds; ++k)
+    if (c.units != c.row16 && (c.src_head[k] != c.row16 * 16 || c.dst_head[k] != c.row16 * 16))
+      return false;
+  return true;
 }
 
 }  // namespace cache
@@ -341,17 +482,24 @@ extern "C" int dsa_cache_append(const void* k, const int64_t* k_strides, const v
   if (k == nullptr || k_pages == nullptr || block_table == nullptr || start == nullptr)
     return DSA_ERR_INVALID_ARGUMENT;
   if (!aligned16(k) || !aligned16(v)) return DSA_ERR_MISALIGNED;
-  st = byte_strides(k_strides, batch, t, n_kv_heads, head_dim, p.ks);
+  int64_t ks[3], vs[3];
+  st = byte_strides(k_strides, batch, t, n_kv_heads, head_dim, ks);
   if (st == DSA_OK)
-    st = byte_strides(v != nullptr ? v_strides : k_strides, batch, t, n_kv_heads, head_dim, p.vs);
+    st = byte_strides(v != nullptr ? v_strides : k_strides, batch, t, n_kv_heads, head_dim, vs);
   if (st != DSA_OK) return st;
   if (batch > (1 << 28) || t > (1 << 28) || max_pages > (int64_t{1} << 28))
     return DSA_ERR_UNSUPPORTED;
-  const int64_t work = batch * t * n_kv_heads * (head_dim / 8);
-  const int64_t blocks = (work + 255) / 256;
+  for (int i = 0; i < 2; ++i) {
+    p.ks[i] = ks[i];
+    p.vs[i] = vs[i];
+  }
+  p.copy = row_copy(p.pool, batch * t);
+  p.copy.src[0] = static_cast<const uint8_t*>(k);
+  p.copy.src[1] = static_cast<const uint8_t*>(v);
+  p.copy.src_head[0] = ks[2];
+  p.copy.src_head[1] = vs[2];
+  const int64_t blocks = (batch * t + p.copy.rows - 1) / p.copy.rows;
   if (blocks > 0x7FFFFFFF) return DSA_ERR_UNSUPPORTED;
-  p.k = static_cast<const uint8_t*>(k);
-  p.v = static_cast<const uint8_t*>(v);
   p.table = block_table;
   p.start = start;
   p.max_pages = max_pages;
@@ -359,8 +507,8 @@ extern "C" int dsa_cache_append(const void* k, const int64_t* k_strides, const v
   p.t = t;
   st = device_error_word(&p.pool.err);
   if (st != DSA_OK) return st;
-  cache_append_kernel<<<dim3(static_cast<unsigned>(blocks), v != nullptr ? 2 : 1), 256, 0,
-                        static_cast<cudaStream_t>(stream)>>>(p);
+  auto kernel = flat_rows(p.copy) ? cache_append_kernel<true> : cache_append_kernel<false>;
+  kernel<<<static_cast<unsigned>(blocks), kCopyThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
   return cuda_status(cudaGetLastError());
 }
 
@@ -401,11 +549,34 @@ extern "C" int dsa_cache_evict(void* k_pages, const int64_t* kp_strides, void* v
   st = device_error_word(&p.pool.err);
   if (st != DSA_OK) return st;
   cudaStream_t cs = static_cast<cudaStream_t>(stream);
-  evict_select_kernel<<<static_cast<unsigned>(batch), kSelThreads, 0, cs>>>(p);
-  st = cuda_status(cudaGetLastError());
+  const int64_t room = max_pages * page_size;
+  const int cluster = select_cluster(batch, room);
+  const int64_t stretch = (room + cluster - 1) / cluster;
+  p.staged = static_cast<int>(stretch < kSelStaged ? stretch : kSelStaged);
+  st = set_max_dynamic_smem(reinterpret_cast<const void*>(evict_select_kernel), kSelStaged * 4);
   if (st != DSA_OK) return st;
-  const int64_t blocks = (dst_pages * page_size + kCopyRows - 1) / kCopyRows;
-  evict_copy_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(batch)), kCopyThreads,
-                      0, cs>>>(p);
+  {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(batch * cluster));
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(p.staged) * 4;
+    cfg.stream = cs;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(cluster);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    st = cuda_status(cudaLaunchKernelEx(&cfg, evict_select_kernel, p));
+  }
+  if (st != DSA_OK) return st;
+  p.copy = row_copy(p.pool, batch * dst_pages * page_size);
+  p.copy.src[0] = p.pool.k;
+  p.copy.src[1] = p.pool.v;
+  p.copy.src_head[0] = p.pool.ks[2];
+  p.copy.src_head[1] = p.pool.vs[2];
+  const int64_t blocks = (dst_pages * page_size + p.copy.rows - 1) / p.copy.rows;
+  auto kernel = flat_rows(p.copy) ? evict_copy_kernel<true> : evict_copy_kernel<false>;
+  kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(batch)), kCopyThreads, 0, cs>>>(p);
   return cuda_status(cudaGetLastError());
 }

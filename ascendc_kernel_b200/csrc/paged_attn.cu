@@ -22,13 +22,13 @@
 //               page; rows of q
 //   warp 1      tcgen05 issuer
 //   warps 4..11 softmax: warpgroup w takes the chunks of parity w, with its own
-//               accumulator, reference and sums
+//               accumulator, reference and sums; S^T products run up to three chunks ahead
 // The reference of a head is set by a warpgroup's first chunk of a piece and
 // moves (O and the sums are rescaled) only when a score exceeds it by more than
 // 2^8, so the common chunk needs one vote and no reduction over keys; the sums
 // stay per thread until the piece ends. P is rounded to the operands' type
 // (relative 2^-8 at most for bf16, the size of the output's own rounding); sums are fp32.
-// TMEM: S^T of warpgroup w [w NM, +NM), O^T [2 NM + w NM, +NM).
+// TMEM: kSBufs S^T buffers of NM columns, then O^T of the two warpgroups.
 #include "host_util.h"
 #include "window_common.cuh"
 #include "window_host.h"
@@ -47,29 +47,44 @@ constexpr int kRegsSoftmax = 208;
 constexpr int kKeys = 128;          // keys of a chunk
 constexpr int kBox = kKeys * 128;   // one [128 keys x 64 columns] SW128 box
 constexpr float kRescaleLog2 = 8.0f;
+constexpr int kMaxSmem = 232448;
 constexpr float kNone = -1.0e30f;   // reference of a piece without a visible key
 
 template <int D, int NM>
 struct Cfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kSlotBytes = kKeys * D * 2;
-  static constexpr int kSlots = (NM == 128 ? 3 : 4) * (128 / D);
-  static constexpr int kQBufs = NM == 128 ? 1 : 2;
+  static constexpr int kSlots = (NM == 128 ? 3 : 5) * (128 / D);
+  static constexpr int kSBufs = NM == 128 ? 2 : 4;  // S^T products that may run ahead
+  static constexpr int kLag = kSBufs - 1;           // O^T of chunk i - kLag after S^T of i
   static constexpr int kQBytes = NM * D * 2;
-  static constexpr int kPBytes = kKeys * NM * 2;
+  static constexpr int kPBytes = kKeys * (NM < 64 ? 64 : NM) * 2;  // [128 keys x 64 heads] boxes
   static constexpr int kOffQ = 0;
-  static constexpr int kOffKV = kOffQ + kQBufs * kQBytes;
+  static constexpr int kOffKV = kOffQ + kQBytes;
   // the second 64-column half of V^T that a 64-wide head lacks is read from the
   // next slot, past the last one from P: rows 64.. of O^T are not used
   static constexpr int kOffP = kOffKV + kSlots * kSlotBytes;
   static constexpr int kOffMax = kOffP + 2 * kPBytes;         // [2][4 warps][NM] f32
-  static constexpr int kOffRef = kOffMax + 2 * 4 * NM * 4;    // [2][2: reference, factor][NM]
-  static constexpr int kOffMeta = kOffRef + 2 * 2 * NM * 4;   // [slot][16] granule states
-  static constexpr int kOffBar = kOffMeta + kSlots * 16 * 4;
-  static constexpr int kNumBars = 2 * kQBufs + 2 * kSlots + 2 + 2 + 2 + 2 + 1;
+  static constexpr int kOffRef = kOffMax + 2 * 4 * NM * 4;    // [2][2: reference, step][NM]
+  static constexpr int kOffMeta = kOffRef + 2 * 2 * NM * 4;   // [16 chunks][16] granule states
+  static constexpr int kOffBar = kOffMeta + 16 * 16 * 4;
+  static constexpr int kNumBars = 2 + 2 * kSlots + kSBufs + 2 + 2 + 2 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 48 + 1024;
-  static constexpr uint32_t kTmemCols = 4 * NM;
+  static constexpr int kColsO = kSBufs * NM;                  // TMEM: S^T buffers, then O^T
+  static constexpr uint32_t kTmemCols = kColsO + 2 * NM <= 256 ? 256 : 512;
+
+  // Number in the CTA's sequence of slot loads of chunk i's K and V, of n chunks in all:
+  // V follows kLag chunks behind K, in the order in which the products use them, so a
+  // slot is given back soon after its data arrived.
+  static __device__ __forceinline__ int64_t seq_k(bool shared, int64_t i) {
+    return shared || i < kLag ? i : 2 * i - kLag;
+  }
+  static __device__ __forceinline__ int64_t seq_v(bool shared, int64_t i, int64_t n) {
+    if (shared) return i;
+    const int64_t x = 2 * i + kLag + 1;
+    return x < n + i ? x : n + i;
+  }
 };
 
 struct Params {
@@ -185,8 +200,9 @@ __device__ __forceinline__ float warp_max(float v) {
   return r;
 }
 
-static_assert(Cfg<128, 64>::kSmemBytes <= 232448 && Cfg<128, 128>::kSmemBytes <= 232448 &&
-                  Cfg<64, 64>::kSmemBytes <= 232448 && Cfg<64, 128>::kSmemBytes <= 232448,
+static_assert(Cfg<128, 32>::kSmemBytes <= kMaxSmem && Cfg<128, 64>::kSmemBytes <= kMaxSmem &&
+                  Cfg<128, 128>::kSmemBytes <= kMaxSmem && Cfg<64, 32>::kSmemBytes <= kMaxSmem &&
+                  Cfg<64, 64>::kSmemBytes <= kMaxSmem && Cfg<64, 128>::kSmemBytes <= kMaxSmem,
               "227 KB of shared memory a CTA");
 
 template <typename T, int D, int NM>
@@ -198,15 +214,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t* q_full = bars;                    // [kQBufs]
-  uint64_t* q_empty = q_full + C::kQBufs;     // [kQBufs]
-  uint64_t* kv_full = q_empty + C::kQBufs;    // [kSlots]
+  uint64_t* q_full = bars;                    // rows of q -> MMA
+  uint64_t* q_empty = q_full + 1;             // last S^T of the piece done -> TMA
+  uint64_t* kv_full = q_empty + 1;            // [kSlots]
   uint64_t* kv_empty = kv_full + C::kSlots;   // [kSlots]
-  uint64_t* s_full = kv_empty + C::kSlots;    // [2] S^T of a chunk in TMEM
-  uint64_t* p_full = s_full + 2;              // [2] P written (128 arrivals)
+  uint64_t* s_full = kv_empty + C::kSlots;    // [kSBufs] S^T of a chunk in TMEM
+  uint64_t* p_full = s_full + C::kSBufs;      // [2] P written (128 arrivals)
   uint64_t* o_done = p_full + 2;              // [2] O^T product of a chunk completed
   uint64_t* o_empty = o_done + 2;             // [2] O^T read at a piece's end (128 arrivals)
-  uint64_t* drain_bar = o_empty + 2;
+  uint64_t* v_ready = o_empty + 2;            // [2] V of the warpgroup's chunk has arrived
+  uint64_t* drain_bar = v_ready + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
   int* walk_s = reinterpret_cast<int*>(smem + C::kOffMisc + 8);  // b, kvh, chunk, left (2 words)
@@ -214,24 +231,22 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int per = p.shared ? 1 : 2;
   const int npad = (p.g + 31) & ~31;
   const int gpc = kKeys / p.gran;  // granules of a chunk
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < C::kQBufs; ++i) {
-      mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
-    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
     for (int s = 0; s < C::kSlots; ++s) {
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
     }
+    for (int i = 0; i < C::kSBufs; ++i) mbar_init(&s_full[i], 1);
     for (int w = 0; w < 2; ++w) {
-      mbar_init(&s_full[w], 1);
       mbar_init(&p_full[w], 128);
       mbar_init(&o_done[w], 1);
       mbar_init(&o_empty[w], 128);
+      mbar_init(&v_ready[w], 1);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -241,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_v);
   }
   // rows of q past the group stay 0: their scores are 0, their columns are not used
-  for (int i = threadIdx.x; i < C::kQBufs * C::kQBytes / 16; i += kThreads)
+  for (int i = threadIdx.x; i < C::kQBytes / 16; i += kThreads)
     st_shared_v4(smem_u32(smem + C::kOffQ + i * 16), 0u, 0u, 0u, 0u);
   fence_proxy_async_smem();
   if (warp == 1) {
@@ -304,60 +319,109 @@ __global__ void __launch_bounds__(kThreads, 1)
   wk.kvh = walk_s[1];
   wk.c0 = walk_s[2];
   wk.left = *reinterpret_cast<const int64_t*>(walk_s + 4);
+  const int64_t chunks = wk.left;  // of the whole stretch
 
   if (warp < 4) {
     win::set_max_regs_dec<kRegsAux>();
     if (warp == 0) {
       // ---------------------------------------------------------- producer
-      int seq = 0, pieces = 0;
+      int64_t gc = 0, seq = 0;
+      int pieces = 0;
       bool ok = true;
-      for (; ok && walk_take(p, wk); walk_next(wk), ++pieces) {
-        const int qb = pieces % C::kQBufs;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&q_empty[qb], ((pieces / C::kQBufs) & 1) ^ 1,
-                                               abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&q_full[qb], static_cast<uint32_t>(p.g * D * 2));
+      // a lane's granule of a chunk: its page (-1: none), first slot of it, kv head
+      struct Gran {
+        int page, slot, kvh;
+      };
+      Gran late[C::kLag];  // of the chunks whose V is not yet requested
+      auto load = [&](const CUtensorMap* tm, const Gran& g, bool mine, int gi, int bytes) -> bool {
+        const int s = static_cast<int>(seq % C::kSlots);
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&kv_empty[s], static_cast<uint32_t>((seq / C::kSlots) & 1) ^ 1,
+                                               abort_flag, p.err, DSA_DEVERR_WIN_WAIT)))
+          return false;
+        if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(bytes));
+        __syncwarp();
+        if (mine && g.page >= 0) {
+          uint8_t* dst = smem + C::kOffKV + s * C::kSlotBytes + gi * p.gran * 128;
 #pragma unroll
           for (int half = 0; half < C::kHalves; ++half)
-            tma_load_3d(smem + C::kOffQ + qb * C::kQBytes + half * NM * 128, &tm_q, half * 64,
-                        wk.kvh * p.g, wk.b, &q_full[qb]);
+            tma_load_4d(dst + half * kBox, tm, half * 64, g.slot, g.kvh, g.page, &kv_full[s]);
         }
-        for (int c = wk.c0; ok && c < wk.c1; ++c) {
-          // a lane per granule: its page, looked up while the slots are still in use
-          const int i = c * gpc + lane;
-          const int row = gran_row(p, wk.s, i);
-          int page = -1;
-          if (lane < gpc && row < wk.s.len) {
-            page = page_of(p, wk.b, row);
-            if (page < 0) atomicOr(p.err, DSA_DEVERR_CACHE);
-          }
-          const uint32_t live = __ballot_sync(0xFFFFFFFFu, page >= 0);
-          const uint32_t bytes = static_cast<uint32_t>(__popc(live) * p.gran * D * 2);
-          for (int kind = 0; kind < per; ++kind, ++seq) {
-            const int s = seq % C::kSlots;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&kv_empty[s], ((seq / C::kSlots) & 1) ^ 1,
-                                                   abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
-            if (!ok) break;
-            if (lane < 16) meta[s * 16 + lane] = page >= 0 ? 1 : 0;
-            __syncwarp();
-            if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], bytes);
-            __syncwarp();
-            if (page >= 0) {
-              const CUtensorMap* tm = kind == 0 ? &tm_k : &tm_v;
-              uint8_t* dst = smem + C::kOffKV + s * C::kSlotBytes + lane * p.gran * 128;
+        ++seq;
+        return true;
+      };
+      // a lane per granule of the next `ahead` chunks: their pages are looked up while the
+      // copies of the chunks before them are waited for
+      const int ahead = 32 / gpc;
+      const int sub = lane / gpc, gi = lane - sub * gpc;
+      const int gran_bytes = p.gran * D * 2;
+      // V of chunk gc - kLag: lanes keep their entry of every chunk (page -1 for a chunk
+      // of another lane group), so each copy is issued by the lane that looked it up
+      auto shift = [&](const Gran& g) {
 #pragma unroll
-              for (int half = 0; half < C::kHalves; ++half)
-                tma_load_4d(dst + half * kBox, tm, half * 64, row % p.page, wk.kvh, page, &kv_full[s]);
+        for (int i = C::kLag - 1; i > 0; --i) late[i] = late[i - 1];
+        late[0] = g;
+      };
+      for (; ok && walk_take(p, wk); walk_next(wk), ++pieces) {
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(q_empty, (pieces & 1) ^ 1, abort_flag, p.err,
+                                               DSA_DEVERR_WIN_WAIT));
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.g * D * 2));
+#pragma unroll
+          for (int half = 0; half < C::kHalves; ++half)
+            tma_load_3d(smem + C::kOffQ + half * NM * 128, &tm_q, half * 64, wk.kvh * p.g, wk.b,
+                        q_full);
+        }
+        int page = -1, row = 0, next_page = -1, next_row = 0;
+        auto look = [&](int c) {
+          next_row = gran_row(p, wk.s, (c + sub) * gpc + gi);
+          next_page = c + sub < wk.c1 && next_row < wk.s.len
+                          ? __ldg(p.table + static_cast<int64_t>(wk.b) * p.max_pages + next_row / p.page)
+                          : -2;  // nothing to read
+        };
+        look(wk.c0);
+        for (int c = wk.c0; ok && c < wk.c1; ++c, ++gc) {
+          const int turn = (c - wk.c0) % ahead;
+          if (turn == 0) {
+            page = next_page;
+            row = next_row;
+            if (page != -2 && (page < 0 || page >= p.num_pages)) {
+              atomicOr(p.err, DSA_DEVERR_CACHE);
+              page = -1;
             }
+            look(c + ahead);
+          }
+          const bool mine = sub == turn;
+          const Gran g = {mine ? max(page, -1) : -1, row % p.page, wk.kvh};
+          const uint32_t live = __ballot_sync(0xFFFFFFFFu, g.page >= 0);
+          if (mine) meta[(gc & 15) * 16 + gi] = g.page >= 0 ? 1 : 0;
+          __syncwarp();
+          ok = load(&tm_k, g, mine, gi, __popc(live) * gran_bytes);
+          if (ok && !p.shared) {
+            if (gc >= C::kLag) {
+              const Gran& v = late[C::kLag - 1];
+              const uint32_t l = __ballot_sync(0xFFFFFFFFu, v.page >= 0);
+              ok = load(&tm_v, v, true, gi, __popc(l) * gran_bytes);
+            }
+            shift(g);
+          }
+        }
+      }
+      if (ok && !p.shared) {
+        // the last chunks' V
+        const int rest = gc < C::kLag ? static_cast<int>(gc) : C::kLag;
+#pragma unroll
+        for (int i = C::kLag - 1; i >= 0; --i) {
+          if (i < rest && ok) {
+            const uint32_t l = __ballot_sync(0xFFFFFFFFu, late[i].page >= 0);
+            ok = load(&tm_v, late[i], true, gi, __popc(l) * gran_bytes);
           }
         }
       }
       // copies in flight land before the CTA's shared memory goes away
-      for (int i = (seq > C::kSlots ? seq - C::kSlots : 0); i < seq; ++i)
-        mbar_drain(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
-      for (int i = (pieces > C::kQBufs ? pieces - C::kQBufs : 0); i < pieces; ++i)
-        mbar_drain(&q_full[i % C::kQBufs], (i / C::kQBufs) & 1);
+      for (int64_t i = (seq > C::kSlots ? seq - C::kSlots : 0); i < seq; ++i)
+        mbar_drain(&kv_full[i % C::kSlots], static_cast<uint32_t>((i / C::kSlots) & 1));
+      if (pieces > 0) mbar_drain(q_full, (pieces - 1) & 1);
     } else if (warp == 1 && lane == 0) {
       // ---------------------------------------------------------- MMA issuer
       const uint32_t idesc_s = win::make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(npad / 8) << 17);
@@ -371,19 +435,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           smem_u32(smem + C::kOffKV), static_cast<uint32_t>(kBox), 1024u, kLayoutSW128));
       const uint32_t p_lo = static_cast<uint32_t>(make_smem_desc(
           smem_u32(smem + C::kOffP), static_cast<uint32_t>(kBox), 1024u, kLayoutSW128));
-      int gc = 0, pieces = 0;
+      int64_t gc = 0;
+      int pieces = 0;
       int gp[2] = {0, 0};       // O^T products issued per warpgroup
       int drained[2] = {0, 0};  // pieces of the warpgroup whose O^T was to be read
-      int prev = -1;            // chunk whose O^T product is not yet issued
-      bool prev_fresh = false;
+      uint32_t fresh_bits = 0;  // bit k: chunk gc - 1 - k is its warpgroup's first of a piece
       bool ok = true;
-      auto issue_o = [&](int i, bool fresh) -> bool {
-        const int w = i & 1;
-        const int s = (i * per + per - 1) % C::kSlots;
-        if (!mbar_wait(&kv_full[s], ((i * per + per - 1) / C::kSlots) & 1, abort_flag, p.err,
-                       DSA_DEVERR_WIN_WAIT) ||
-            !mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
-          return false;
+      auto wait_slot = [&](int64_t i) -> bool {
+        return mbar_wait(&kv_full[i % C::kSlots], static_cast<uint32_t>((i / C::kSlots) & 1), abort_flag,
+                         p.err, DSA_DEVERR_WIN_WAIT);
+      };
+      auto issue_o = [&](int64_t i, bool fresh) -> bool {
+        const int w = static_cast<int>(i & 1);
+        const int64_t sv = C::seq_v(p.shared, i, chunks);
+        const int s = static_cast<int>(sv % C::kSlots);
+        if (!wait_slot(sv)) return false;
+        mbar_arrive(&v_ready[w]);  // the softmax may clear its hidden rows
+        if (!mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) return false;
         if (fresh) {
           if (drained[w] > 0 && !mbar_wait(&o_empty[w], (drained[w] - 1) & 1, abort_flag, p.err,
                                            DSA_DEVERR_WIN_WAIT))
@@ -393,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t va = v_lo + static_cast<uint32_t>(s * (C::kSlotBytes >> 4));
         const uint32_t pb = p_lo + static_cast<uint32_t>(w * (C::kPBytes >> 4));
-        const uint32_t d = tmem + static_cast<uint32_t>((2 + w) * NM);
+        const uint32_t d = tmem + static_cast<uint32_t>(C::kColsO + w * NM);
 #pragma unroll
         for (int st = 0; st < kKeys / 16; ++st)
           umma_bf16(d, desc_from_words(va + static_cast<uint32_t>(st * 128), hi),
@@ -405,149 +473,163 @@ __global__ void __launch_bounds__(kThreads, 1)
         return true;
       };
       for (; ok && walk_take(p, wk); walk_next(wk), ++pieces) {
-        const int qb = pieces % C::kQBufs;
-        ok = mbar_wait(&q_full[qb], (pieces / C::kQBufs) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+        ok = mbar_wait(q_full, pieces & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         const int n = wk.c1 - wk.c0;
         for (int j = 0; ok && j < n; ++j, ++gc) {
-          // S^T(i) while the softmax of chunk i - 1 runs. Its columns held S^T(i - 2),
-          // whose readers arrived before O^T(i - 2) was issued
-          const int w = gc & 1;
-          const int s = (gc * per) % C::kSlots;
-          ok = mbar_wait(&kv_full[s], ((gc * per) / C::kSlots) & 1, abort_flag, p.err,
-                         DSA_DEVERR_WIN_WAIT);
+          // S^T runs ahead of the softmax: the buffer held S^T(gc - kSBufs), whose readers
+          // arrived before O^T(gc - kSBufs) was issued
+          const int64_t sk = C::seq_k(p.shared, gc);
+          const int s = static_cast<int>(sk % C::kSlots);
+          ok = wait_slot(sk);
           if (!ok) break;
           tc_fence_after();
           const uint32_t ka = k_lo + static_cast<uint32_t>(s * (C::kSlotBytes >> 4));
-          const uint32_t qa = q_lo + static_cast<uint32_t>(qb * (C::kQBytes >> 4));
+          const uint32_t buf = static_cast<uint32_t>(gc % C::kSBufs);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBox + (k & 3) * 32) >> 4);
             const uint32_t bo = static_cast<uint32_t>(((k >> 2) * NM * 128 + (k & 3) * 32) >> 4);
-            umma_bf16(tmem + static_cast<uint32_t>(w * NM), desc_from_words(ka + ao, hi),
-                      desc_from_words(qa + bo, hi), idesc_s, k > 0 ? 1u : 0u);
+            umma_bf16(tmem + buf * NM, desc_from_words(ka + ao, hi), desc_from_words(q_lo + bo, hi),
+                      idesc_s, k > 0 ? 1u : 0u);
           }
-          umma_commit(&s_full[w]);
+          umma_commit(&s_full[buf]);
           if (!p.shared) umma_commit(&kv_empty[s]);
-          if (j == n - 1) umma_commit(&q_empty[qb]);
-          if (prev >= 0) ok = issue_o(prev, prev_fresh);
-          prev = gc;
-          prev_fresh = j < 2;
+          if (j == n - 1) umma_commit(q_empty);
+          if (gc >= C::kLag) ok = issue_o(gc - C::kLag, (fresh_bits >> (C::kLag - 1)) & 1u);
+          fresh_bits = (fresh_bits << 1) | (j < 2 ? 1u : 0u);
         }
       }
-      if (ok && prev >= 0) issue_o(prev, prev_fresh);
+      for (int64_t i = gc < C::kLag ? 0 : gc - C::kLag; ok && i < gc; ++i)
+        ok = issue_o(i, (fresh_bits >> (gc - 1 - i)) & 1u);
       umma_commit(drain_bar);
       mbar_drain(drain_bar, 0);
     }
   } else {
     // ------------------------------------------------------------ softmax
+    // After a wait that ran out the abort flag makes every later wait return at once: the
+    // loops run to their end, so that no thread misses a named barrier, on values that
+    // the error word declares void.
     win::set_max_regs_inc<kRegsSoftmax>();
     const int w = (warp - 4) >> 2;
     const int quarter = warp & 3;
     const int key = quarter * 32 + lane;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t sp = tmem + lane_off + static_cast<uint32_t>(w * NM);
-    const uint32_t od = tmem + lane_off + static_cast<uint32_t>((2 + w) * NM);
+    const uint32_t od = tmem + lane_off + static_cast<uint32_t>(C::kColsO + w * NM);
     const uint32_t bar = 1 + static_cast<uint32_t>(w);
     float* wmax = reinterpret_cast<float*>(smem + C::kOffMax) + w * 4 * NM;
-    float* ref = reinterpret_cast<float*>(smem + C::kOffRef) + w * 2 * NM;
-    float* fac = ref + NM;
+    float* nref = reinterpret_cast<float*>(smem + C::kOffRef) + w * 2 * NM;  // -reference
+    float* move = nref + NM;                                                 // its last step
     const uint32_t prow = smem_u32(smem + C::kOffP) + static_cast<uint32_t>(w * C::kPBytes + key * 128);
-    int gc = 0, gw = 0;
-    bool ok = true;
-    // a warpgroup leaves together: it meets at named barriers
-    auto wait_all = [&](uint64_t* b, uint32_t parity) -> bool {
-      return named_bar_and(bar, 128, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+    const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
+    int64_t gc = 0;
+    int gw = 0;
+    uint32_t sp = 0;  // the chunk's S^T
+    auto wait = [&](uint64_t* b, uint32_t parity) {  // whole warps
+      mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+      __syncwarp();
     };
-    for (; ok && walk_take(p, wk); walk_next(wk)) {
-      float l[NM];
+    // 32 scores of the key relative to their heads' references, log2-scaled
+    auto load_scores = [&](int q, uint64_t (&d)[16]) {
+      uint32_t v[32];
+      tmem_ld_32x32b_x32(sp + static_cast<uint32_t>(q * 32), v);
 #pragma unroll
-      for (int k = 0; k < NM; ++k) l[k] = 0.f;
+      for (int k = 0; k < 8; ++k) {
+        const float4 r = reinterpret_cast<const float4*>(nref)[q * 8 + k];
+        d[2 * k] = f2_fma(f2_pack(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1])), scale2,
+                          f2_pack(r.x, r.y));
+        d[2 * k + 1] = f2_fma(f2_pack(__uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3])),
+                              scale2, f2_pack(r.z, r.w));
+      }
+    };
+    for (; walk_take(p, wk); walk_next(wk)) {
+      uint64_t l2[NM / 2];  // sums of the key's weights, two heads a register pair
+#pragma unroll
+      for (int k = 0; k < NM / 2; ++k) l2[k] = 0ull;
       const int n = wk.c1 - wk.c0;
       bool fresh = true;
+      if (key < npad) nref[key] = 0.f;
+      named_bar_sync(bar, 128);
       for (int j = 0; j < n; ++j, ++gc) {
         if ((gc & 1) != w) continue;
-        ok = wait_all(&s_full[w], gw & 1);
-        if (!ok) break;
         const int c = wk.c0 + j;
-        const int sv = (gc * per + per - 1) % C::kSlots;
         const int gi = key / p.gran;
         const int row = gran_row(p, wk.s, c * gpc + gi) + (key - gi * p.gran);
-        // the granules' states are read from the V slot, which stays until this chunk's
-        // weights are used (the K slot is given back as soon as S^T is done)
-        ok = wait_all(&kv_full[sv], ((gc * per + per - 1) / C::kSlots) & 1);
-        if (!ok) break;
-        const bool valid = row_seen(wk.s, c * gpc + gi, row) && meta[sv * 16 + gi] != 0;
+        sp = tmem + lane_off + static_cast<uint32_t>(gc % C::kSBufs) * NM;
+        wait(&s_full[gc % C::kSBufs], static_cast<uint32_t>((gc / C::kSBufs) & 1));
         tc_fence_after();
-        // ---- does any score exceed its head's reference by more than 2^8?
-        bool over = fresh;
-        if (!fresh) {
-          float excess = -INFINITY;
+        const bool valid = row_seen(wk.s, c * gpc + gi, row) && meta[(gc & 15) * 16 + gi] != 0;
+        // up to 64 heads the scores stay in registers; beyond, they are loaded again
+        constexpr bool kHold = NM <= 64;
+        uint64_t d[kHold ? NM / 32 : 1][16];
+        float excess = -INFINITY;
+#pragma unroll
+        for (int q = 0; q < NM / 32; ++q) {
+          if (q * 32 < npad) {
+            uint64_t(&x)[16] = d[kHold ? q : 0];
+            load_scores(q, x);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float a, b;
+              f2_unpack(x[k], a, b);
+              excess = fmax3(excess, a, b);
+            }
+          }
+        }
+        // does any score exceed its head's reference by more than 2^8?
+        if (named_bar_or(bar, 128, fresh || (valid && excess > kRescaleLog2))) {
+          // the heads' maxima over the chunk's keys: warps, then the warpgroup
 #pragma unroll
           for (int q = 0; q < NM / 32; ++q) {
             if (q * 32 < npad) {
-              uint32_t v[32];
-              tmem_ld_32x32b_x32(sp + static_cast<uint32_t>(q * 32), v);
+              uint64_t(&x)[16] = d[kHold ? q : 0];
+              if (!kHold) load_scores(q, x);
+              float mine = 0.f;
 #pragma unroll
-              for (int k = 0; k < 8; ++k) {
-                const float4 r = reinterpret_cast<const float4*>(ref)[q * 8 + k];
-                excess = fmax3(excess, fmaf(__uint_as_float(v[4 * k]), p.scale_log2, -r.x),
-                               fmaf(__uint_as_float(v[4 * k + 1]), p.scale_log2, -r.y));
-                excess = fmax3(excess, fmaf(__uint_as_float(v[4 * k + 2]), p.scale_log2, -r.z),
-                               fmaf(__uint_as_float(v[4 * k + 3]), p.scale_log2, -r.w));
+              for (int k = 0; k < 16; ++k) {
+                float a, b;
+                f2_unpack(x[k], a, b);
+                const float ma = warp_max(valid ? a : kNone), mb = warp_max(valid ? b : kNone);
+                if (lane == 2 * k) mine = ma;
+                if (lane == 2 * k + 1) mine = mb;
               }
+              wmax[quarter * NM + q * 32 + lane] = mine;
             }
-          }
-          over = valid && excess > kRescaleLog2;
-        }
-        if (named_bar_or(bar, 128, over)) {
-          // the heads' maxima over the chunk's keys: warps, then the warpgroup
-#pragma unroll 1
-          for (int q = 0; q * 32 < npad; ++q) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(sp + static_cast<uint32_t>(q * 32), v);
-            float mine = 0.f;
-#pragma unroll
-            for (int k = 0; k < 32; ++k) {
-              const float m = warp_max(valid ? __uint_as_float(v[k]) * p.scale_log2 : kNone);
-              if (lane == k) mine = m;
-            }
-            wmax[quarter * NM + q * 32 + lane] = mine;
           }
           named_bar_sync(bar, 128);
           if (key < npad) {
             const float m = fmaxf(fmaxf(wmax[key], wmax[NM + key]),
                                   fmaxf(wmax[2 * NM + key], wmax[3 * NM + key]));
-            const float old = fresh ? m : ref[key];
-            const float now = m > old + kRescaleLog2 ? m : old;
-            ref[key] = now;
-            fac[key] = ex2_approx(old - now);
+            const float step = fresh || m > kRescaleLog2 ? m : 0.f;
+            nref[key] -= step;
+            move[key] = step;
           }
           named_bar_sync(bar, 128);
           if (!fresh) {
-            ok = wait_all(&o_done[w], (gw - 1) & 1);
-            if (!ok) break;
+            wait(&o_done[w], (gw - 1) & 1);
             tc_fence_after();
+          }
 #pragma unroll
-            for (int q = 0; q < NM / 32; ++q) {
-              if (q * 32 < npad) {
-                uint32_t v[32];
-                tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
+          for (int q = 0; q < NM / 32; ++q) {
+            if (q * 32 < npad) {
+              uint32_t v[32];
+              if (!fresh) tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                  const float f = fac[q * 32 + k];
-                  l[q * 32 + k] *= f;
-                  v[k] = __float_as_uint(__uint_as_float(v[k]) * f);
+              for (int k = 0; k < 16; ++k) {
+                const float s0 = move[q * 32 + 2 * k], s1 = move[q * 32 + 2 * k + 1];
+                if (kHold) d[q][k] = f2_sub(d[q][k], f2_pack(s0, s1));
+                if (!fresh) {
+                  const float f0 = ex2_approx(-s0), f1 = ex2_approx(-s1);
+                  l2[q * 16 + k] = f2_mul(l2[q * 16 + k], f2_pack(f0, f1));
+                  v[2 * k] = __float_as_uint(__uint_as_float(v[2 * k]) * f0);
+                  v[2 * k + 1] = __float_as_uint(__uint_as_float(v[2 * k + 1]) * f1);
                 }
-                tmem_st_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
               }
+              if (!fresh) tmem_st_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
             }
           }
         }
         // ---- P = 2^(z - reference), the key's weights of all heads
-        if (gw > 0) {  // the warpgroup's previous product has read P
-          ok = wait_all(&o_done[w], (gw - 1) & 1);
-          if (!ok) break;
-        }
+        if (gw > 0) wait(&o_done[w], (gw - 1) & 1);  // the previous product has read P
         float* zrow = nullptr;
         if (p.scores != nullptr) {
           // chunks of this sequence lie [kv head][chunk] at max_chunks of the table
@@ -555,31 +637,34 @@ __global__ void __launch_bounds__(kThreads, 1)
           zrow = p.scores +
                  (((static_cast<int64_t>(wk.b) * p.hk + wk.kvh) * cap + c) * kKeys + key) * p.g;
         }
+        const bool some = !__all_sync(0xFFFFFFFFu, valid);
 #pragma unroll
         for (int q = 0; q < NM / 32; ++q) {
           if (q * 32 < npad) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(sp + static_cast<uint32_t>(q * 32), v);
+            uint64_t(&x)[16] = d[kHold ? q : 0];
+            if (!kHold) load_scores(q, x);
+            if (some && !valid) {
+#pragma unroll
+              for (int k = 0; k < 16; ++k) x[k] = f2_pack(-INFINITY, -INFINITY);
+            }
             if (zrow != nullptr) {
 #pragma unroll
-              for (int k = 0; k < 32; ++k)
-                if (q * 32 + k < p.g)
-                  zrow[q * 32 + k] = valid ? __uint_as_float(v[k]) * p.scale_log2 : -INFINITY;
+              for (int k = 0; k < 16; ++k) {
+                float a, b;
+                f2_unpack(x[k], a, b);
+                if (q * 32 + 2 * k < p.g) zrow[q * 32 + 2 * k] = a - nref[q * 32 + 2 * k];
+                if (q * 32 + 2 * k + 1 < p.g) zrow[q * 32 + 2 * k + 1] = b - nref[q * 32 + 2 * k + 1];
+              }
             }
             uint32_t pk[16];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const float4 r = reinterpret_cast<const float4*>(ref)[q * 8 + k];
-              const float e0 = valid ? ex2_approx(fmaf(__uint_as_float(v[4 * k]), p.scale_log2, -r.x)) : 0.f;
-              const float e1 = valid ? ex2_approx(fmaf(__uint_as_float(v[4 * k + 1]), p.scale_log2, -r.y)) : 0.f;
-              const float e2 = valid ? ex2_approx(fmaf(__uint_as_float(v[4 * k + 2]), p.scale_log2, -r.z)) : 0.f;
-              const float e3 = valid ? ex2_approx(fmaf(__uint_as_float(v[4 * k + 3]), p.scale_log2, -r.w)) : 0.f;
-              l[q * 32 + 4 * k] += e0;
-              l[q * 32 + 4 * k + 1] += e1;
-              l[q * 32 + 4 * k + 2] += e2;
-              l[q * 32 + 4 * k + 3] += e3;
-              pk[2 * k] = T::pack(e0, e1);
-              pk[2 * k + 1] = T::pack(e2, e3);
+            for (int k = 0; k < 16; ++k) {
+              float a, b;
+              f2_unpack(x[k], a, b);
+              a = ex2_approx(a);
+              b = ex2_approx(b);
+              l2[q * 16 + k] = f2_add(l2[q * 16 + k], f2_pack(a, b));
+              pk[k] = T::pack(a, b);
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -591,28 +676,30 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (!valid) {
-          // a hidden V row may hold anything, and 0 x NaN is NaN: it is cleared
-          uint8_t* vr = smem + C::kOffKV + sv * C::kSlotBytes + key * 128;
+          // a hidden V row may hold anything, and 0 x NaN is NaN: it is cleared. The issuer,
+          // which waits for the slots in their order, says when V is there
+          const int64_t sv = C::seq_v(p.shared, gc, chunks);
+          mbar_wait(&v_ready[w], gw & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+          uint8_t* vr = smem + C::kOffKV + (sv % C::kSlots) * C::kSlotBytes + key * 128;
 #pragma unroll
           for (int x = 0; x < C::kHalves * 8; ++x)
             st_shared_v4(smem_u32(vr + (x >> 3) * kBox + (x & 7) * 16), 0u, 0u, 0u, 0u);
         }
+        __syncwarp();
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(&p_full[w]);
         ++gw;
         fresh = false;
       }
-      if (!ok) break;
       // ---- the piece's partial of this warpgroup
       const int64_t piece = static_cast<int64_t>(blockIdx.x) + static_cast<int64_t>(wk.b) * p.hk + wk.kvh;
       float2* ml = p.part_ml + (piece * 2 + w) * p.g;
       if (fresh) {  // it had no chunk
-        for (int x = key; x < p.g; x += 128) ml[x] = make_float2(kNone, 0.f);
+        if (key < p.g) ml[key] = make_float2(kNone, 0.f);
         continue;
       }
-      ok = wait_all(&o_done[w], (gw - 1) & 1);
-      if (!ok) break;
+      wait(&o_done[w], (gw - 1) & 1);
       tc_fence_after();
 #pragma unroll
       for (int q = 0; q < NM / 32; ++q) {
@@ -620,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // sums over the warp's 32 keys of 32 heads: lane k ends with head k
           float a[32];
 #pragma unroll
-          for (int k = 0; k < 32; ++k) a[k] = l[q * 32 + k];
+          for (int k = 0; k < 16; ++k) f2_unpack(l2[q * 16 + k], a[2 * k], a[2 * k + 1]);
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) {
             const bool up = (lane & o) != 0;
@@ -645,7 +732,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_arrive(&o_empty[w]);
       named_bar_sync(bar, 128);
       if (key < p.g)
-        ml[key] = make_float2(ref[key], (wmax[key] + wmax[NM + key]) +
+        ml[key] = make_float2(-nref[key], (wmax[key] + wmax[NM + key]) +
                                             (wmax[2 * NM + key] + wmax[3 * NM + key]));
       named_bar_sync(bar, 128);  // the next piece writes the references and maxima
     }
@@ -660,57 +747,84 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the pieces of one (sequence, head): a block of D threads, a column each.
+// Joins the pieces of one (sequence, head): a block of D threads, a column each. The
+// pieces' maxima and sums are read at once, then the outputs eight at a time; latency
+// bound (a few MB at most).
 template <typename T, int D>
 __global__ void __launch_bounds__(D) paged_join_kernel(const Params p) {
+  extern __shared__ float weight[];  // [2 (units + 1)]
+  __shared__ float red[2][D / 32];
   const int head = blockIdx.x % p.h;
   const int b = blockIdx.x / p.h;
   const int kvh = head / p.g, gi = head - kvh * p.g;
-  const int x = threadIdx.x;
+  const int x = threadIdx.x, warp = x >> 5;
   int64_t before, all;
   chunk_sums(p, b, &before, &all);
   const int64_t n = seq_chunks(p, b);
   const int64_t first = before * p.hk + kvh * n, last = first + n;
   all *= p.hk;
   const float sink2 = p.sink != nullptr ? __ldg(p.sink + head) * kLog2e : -INFINITY;
-  float top = sink2, sum = 0.f, acc = 0.f;
+  int64_t u0 = 0;
+  int parts = 0;  // two (warpgroups) per piece
   if (n > 0) {
     // CTA u takes chunks [all u / units, all (u + 1) / units)
-    int64_t u0 = first * p.units / all;
+    u0 = first * p.units / all;
     while (u0 > 0 && all * u0 / p.units > first) --u0;
     while (all * (u0 + 1) / p.units <= first) ++u0;
-    int64_t u1 = u0;
-    while (all * (u1 + 1) / p.units < last) ++u1;
-    const int64_t bh = static_cast<int64_t>(b) * p.hk + kvh;
-    for (int64_t u = u0; u <= u1; ++u) {
-      if (all * u / p.units == all * (u + 1) / p.units) continue;  // an empty stretch
-      for (int w = 0; w < 2; ++w) {
-        const int64_t at = ((u + bh) * 2 + w) * p.g + gi;
-        const float2 ml = p.part_ml[at];
-        if (ml.y == 0.f) continue;  // no visible key
-        const float o = p.part_o[at * D + x];
-        const float now = fmaxf(top, ml.x);
-        const float f = top == now ? 1.f : ex2_approx(top - now), g = ex2_approx(ml.x - now);
-        acc = acc * f + o * g;
-        sum = sum * f + ml.y * g;
-        top = now;
-      }
-    }
+    int64_t u1 = (last - 1) * p.units / all;
+    while (all * u1 / p.units > last - 1) --u1;
+    while (all * (u1 + 1) / p.units <= last - 1) ++u1;
+    parts = static_cast<int>(u1 - u0 + 1) * 2;
   }
-  const float ref = top == -INFINITY ? 0.f : top;
-  const float total = sum + (p.sink != nullptr ? ex2_approx(sink2 - ref) : 0.f);
+  // piece u of (sequence, kv head) is number u + b hk + kvh
+  const int64_t piece = (u0 + static_cast<int64_t>(b) * p.hk + kvh) * 2;
+  auto part = [&](int i) -> float2 {
+    const int64_t u = u0 + (i >> 1);
+    if (all * u / p.units == all * (u + 1) / p.units) return make_float2(kNone, 0.f);  // no chunk
+    return p.part_ml[(piece + i) * p.g + gi];
+  };
+  float top = kNone;
+  for (int i = x; i < parts; i += D) top = fmaxf(top, part(i).x);
+  top = warp_max(top);
+  if ((x & 31) == 0) red[0][warp] = top;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) top = fmaxf(top, red[0][i]);
+  top = fmaxf(top, sink2);
+  float sum = 0.f;
+  for (int i = x; i < parts; i += D) {
+    const float2 ml = part(i);
+    // a part without a visible key (sum 0) is not read below
+    const float f = ml.y == 0.f ? 0.f : ex2_approx(ml.x - top);
+    weight[i] = f;
+    sum += ml.y * f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+  if ((x & 31) == 0) red[1][warp] = sum;
+  __syncthreads();
+  sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) sum += red[1][i];
+  float acc = 0.f;
+  const float* o = p.part_o + (piece * p.g + gi) * D + x;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i)
+    if (weight[i] != 0.f) acc = fmaf(o[static_cast<int64_t>(i) * p.g * D], weight[i], acc);
+  const float total = sum + (p.sink != nullptr ? ex2_approx(sink2 - top) : 0.f);
   const float v = total == 0.f ? 0.f : acc / total;
   const uint32_t bits = T::pack(v, 0.f);
   static_cast<uint16_t*>(p.out)[static_cast<int64_t>(blockIdx.x) * D + x] =
       static_cast<uint16_t>(bits & 0xFFFFu);
   if (x == 0) {
-    const float l2 = ref + log2f(total);
-    p.lse2[blockIdx.x] = l2;
-    if (p.lse != nullptr) p.lse[blockIdx.x] = l2 * kLn2;
+    const float lse2 = total == 0.f ? -INFINITY : top + log2f(total);
+    p.lse2[blockIdx.x] = lse2;
+    if (p.lse != nullptr) p.lse[blockIdx.x] = lse2 * kLn2;
   }
 }
 
-// weights[slot of key] += sum over heads of 2^(z - lse): a thread a key, heads in order.
+// weights[slot of key] += sum over heads of 2^(z - lse): a thread a key, heads in order,
+// four at a time where the group's size and the scores' rows allow.
 __global__ void __launch_bounds__(kKeys) paged_weights_kernel(const Params p) {
   const int b = blockIdx.y, c = blockIdx.x;
   const Seq s = make_seq(p, b);
@@ -723,11 +837,23 @@ __global__ void __launch_bounds__(kKeys) paged_weights_kernel(const Params p) {
   if (page < 0) return;
   const int64_t cap = (static_cast<int64_t>(p.max_pages) * p.page + kKeys - 1) / kKeys + 2;
   const float* lse = p.lse2 + static_cast<int64_t>(b) * p.h;
+  const float* z = p.scores + ((static_cast<int64_t>(b) * p.hk * cap + c) * kKeys + threadIdx.x) * p.g;
+  const int64_t step = cap * kKeys * p.g;  // to the next kv head
   float sum = 0.f;
-  for (int kvh = 0; kvh < p.hk; ++kvh) {
-    const float* z = p.scores +
-                     (((static_cast<int64_t>(b) * p.hk + kvh) * cap + c) * kKeys + threadIdx.x) * p.g;
-    for (int k = 0; k < p.g; ++k) sum += ex2_approx(z[k] - __ldg(lse + kvh * p.g + k));
+  if (p.g % 4 == 0) {
+    const int n4 = p.h / 4, g4 = p.g / 4;
+#pragma unroll 8
+    for (int i = 0; i < n4; ++i) {
+      const int kvh = i / g4;
+      const float4 a = *reinterpret_cast<const float4*>(z + kvh * step + (i - kvh * g4) * 4);
+      const float4 m = __ldg(reinterpret_cast<const float4*>(lse) + i);
+      sum += (ex2_approx(a.x - m.x) + ex2_approx(a.y - m.y)) +
+             (ex2_approx(a.z - m.z) + ex2_approx(a.w - m.w));
+    }
+  } else {
+    for (int kvh = 0; kvh < p.hk; ++kvh)
+      for (int k = 0; k < p.g; ++k)
+        sum += ex2_approx(z[kvh * step + k] - __ldg(lse + kvh * p.g + k));
   }
   // one add per slot; pages that sequences share get one from each
   atomicAdd(p.weights + static_cast<int64_t>(page) * p.page + row % p.page, sum);
@@ -779,10 +905,12 @@ int launch_split(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& 
 template <typename T, int D>
 int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p,
            cudaStream_t stream) {
-  int st = p.g <= 64 ? launch_split<T, D, 64>(q, k, v, p, stream)
-                     : launch_split<T, D, 128>(q, k, v, p, stream);
+  int st = p.g <= 32   ? launch_split<T, D, 32>(q, k, v, p, stream)
+           : p.g <= 64 ? launch_split<T, D, 64>(q, k, v, p, stream)
+                       : launch_split<T, D, 128>(q, k, v, p, stream);
   if (st != DSA_OK) return st;
-  paged_join_kernel<T, D><<<static_cast<unsigned>(p.batch * p.h), D, 0, stream>>>(p);
+  paged_join_kernel<T, D><<<static_cast<unsigned>(p.batch * p.h), D, 2 * (p.units + 1) * sizeof(float),
+                            stream>>>(p);
   st = cuda_status(cudaGetLastError());
   if (st != DSA_OK || p.weights == nullptr) return st;
   paged_weights_kernel<<<dim3(static_cast<unsigned>(max_chunks(p.max_pages, p.page)),
@@ -861,9 +989,7 @@ extern "C" int dsa_paged_attn_fwd(const void* q, const int64_t* q_strides, const
   DeviceInfo di;
   int st = current_device_info(&di);
   if (st != DSA_OK) return st;
-  const int need = g <= 64 ? (head_dim == 128 ? Cfg<128, 64>::kSmemBytes : Cfg<64, 64>::kSmemBytes)
-                           : (head_dim == 128 ? Cfg<128, 128>::kSmemBytes : Cfg<64, 128>::kSmemBytes);
-  if (di.max_smem_optin < need) return DSA_ERR_UNSUPPORTED;
+  if (di.max_smem_optin < kMaxSmem) return DSA_ERR_UNSUPPORTED;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   Params p;
   p.batch = static_cast<int>(batch);

@@ -415,8 +415,8 @@ int dsa_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* k_pa
  * elements, NULL for contiguous: k_strides, v_strides (batch, token, head), kp_strides,
  * vp_strides (page, slot, head). A row outside the table's room, or of a page that
  * does not exist, is not written (DSA_DEVERR_CACHE). Two rows of one call must not
- * name one slot. Supported: head_dim a multiple of 8 and <= 1024, strides multiples
- * of 8. No counterpart in the reference. */
+ * name one slot. Supported: head_dim a multiple of 8 and <= 1024, n_kv_heads *
+ * head_dim < 131072, strides multiples of 8. No counterpart in the reference. */
 int dsa_cache_append(const void* k, const int64_t* k_strides, const void* v,
                      const int64_t* v_strides, void* k_pages, const int64_t* kp_strides,
                      void* v_pages, const int64_t* vp_strides, float* weights,
