@@ -74,16 +74,13 @@ struct Cfg {
   static constexpr int kColsO = kSBufs * NM;                  // TMEM: S^T buffers, then O^T
   static constexpr uint32_t kTmemCols = kColsO + 2 * NM <= 256 ? 256 : 512;
 
-  // Number in the CTA's sequence of slot loads of chunk i's K and V, of n chunks in all:
-  // V follows kLag chunks behind K, in the order in which the products use them, so a
-  // slot is given back soon after its data arrived.
-  static __device__ __forceinline__ int64_t seq_k(bool shared, int64_t i) {
-    return shared || i < kLag ? i : 2 * i - kLag;
-  }
-  static __device__ __forceinline__ int64_t seq_v(bool shared, int64_t i, int64_t n) {
-    if (shared) return i;
-    const int64_t x = 2 * i + kLag + 1;
-    return x < n + i ? x : n + i;
+  // V is loaded kLag chunks behind K, in the order in which the products use them, so a
+  // slot is given back soon after its data arrived. Slot of chunk i's V, of n chunks: the
+  // loads run K(0) .. K(kLag - 1), then K(i), V(i - kLag) in turn, then the last V.
+  static __device__ __forceinline__ int slot_v(bool shared, int i, int n) {
+    const int64_t x = shared ? i : 2 * static_cast<int64_t>(i) + kLag + 1;
+    const int64_t y = static_cast<int64_t>(n) + i;
+    return static_cast<int>((x < y ? x : y) % kSlots);
   }
 };
 
@@ -193,12 +190,35 @@ __device__ __forceinline__ bool walk_take(const Params& p, Walk& w) {
 }
 __device__ __forceinline__ void walk_next(Walk& w) { w.c0 = w.c1; }
 
-// max over the warp of a float (NaN is ignored)
-__device__ __forceinline__ float warp_max(float v) {
-  float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
-  return r;
+// Reduces 32 values of each lane over the lanes: lane k gets the result of a[k]. Each
+// step halves the values a lane carries, so it takes 31 shuffles and not 160.
+template <typename Op>
+__device__ __forceinline__ float warp_transposed(float (&a)[32], int lane, Op op) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const bool up = (lane & o) != 0;
+#pragma unroll
+    for (int k = 0; k < o; ++k) {
+      const float send = up ? a[k] : a[k + o];
+      const float keep = up ? a[k + o] : a[k];
+      a[k] = op(keep, __shfl_xor_sync(0xFFFFFFFFu, send, o));
+    }
+  }
+  return a[0];
 }
+
+// A position in a ring of N slots and the parity of its barriers' phase.
+template <int N>
+struct Ring {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      parity ^= 1u;
+    }
+  }
+};
 
 static_assert(Cfg<128, 32>::kSmemBytes <= kMaxSmem && Cfg<128, 64>::kSmemBytes <= kMaxSmem &&
                   Cfg<128, 128>::kSmemBytes <= kMaxSmem && Cfg<64, 32>::kSmemBytes <= kMaxSmem &&
@@ -319,14 +339,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   wk.kvh = walk_s[1];
   wk.c0 = walk_s[2];
   wk.left = *reinterpret_cast<const int64_t*>(walk_s + 4);
-  const int64_t chunks = wk.left;  // of the whole stretch
+  const int chunks = static_cast<int>(wk.left);  // of the whole stretch
 
   if (warp < 4) {
     win::set_max_regs_dec<kRegsAux>();
     if (warp == 0) {
       // ---------------------------------------------------------- producer
-      int64_t gc = 0, seq = 0;
-      int pieces = 0;
+      Ring<C::kSlots> at;
+      int gc = 0, loads = 0, pieces = 0;
       bool ok = true;
       // a lane's granule of a chunk: its page (-1: none), first slot of it, kv head
       struct Gran {
@@ -334,19 +354,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       Gran late[C::kLag];  // of the chunks whose V is not yet requested
       auto load = [&](const CUtensorMap* tm, const Gran& g, bool mine, int gi, int bytes) -> bool {
-        const int s = static_cast<int>(seq % C::kSlots);
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&kv_empty[s], static_cast<uint32_t>((seq / C::kSlots) & 1) ^ 1,
-                                               abort_flag, p.err, DSA_DEVERR_WIN_WAIT)))
+        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&kv_empty[at.slot], at.parity ^ 1u, abort_flag, p.err,
+                                               DSA_DEVERR_WIN_WAIT)))
           return false;
-        if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(bytes));
+        if (lane == 0) mbar_arrive_expect_tx(&kv_full[at.slot], static_cast<uint32_t>(bytes));
         __syncwarp();
         if (mine && g.page >= 0) {
-          uint8_t* dst = smem + C::kOffKV + s * C::kSlotBytes + gi * p.gran * 128;
+          uint8_t* dst = smem + C::kOffKV + at.slot * C::kSlotBytes + gi * p.gran * 128;
 #pragma unroll
           for (int half = 0; half < C::kHalves; ++half)
-            tma_load_4d(dst + half * kBox, tm, half * 64, g.slot, g.kvh, g.page, &kv_full[s]);
+            tma_load_4d(dst + half * kBox, tm, half * 64, g.slot, g.kvh, g.page, &kv_full[at.slot]);
         }
-        ++seq;
+        at.next();
+        ++loads;
         return true;
       };
       // a lane per granule of the next `ahead` chunks: their pages are looked up while the
@@ -372,19 +392,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             tma_load_3d(smem + C::kOffQ + half * NM * 128, &tm_q, half * 64, wk.kvh * p.g, wk.b,
                         q_full);
         }
-        int page = -1, row = 0, next_page = -1, next_row = 0;
+        int page = -1, slot = 0, next_page = -1, next_slot = 0;
         auto look = [&](int c) {
-          next_row = gran_row(p, wk.s, (c + sub) * gpc + gi);
-          next_page = c + sub < wk.c1 && next_row < wk.s.len
-                          ? __ldg(p.table + static_cast<int64_t>(wk.b) * p.max_pages + next_row / p.page)
+          const int row = gran_row(p, wk.s, (c + sub) * gpc + gi);
+          const int i = row / p.page;
+          next_slot = row - i * p.page;
+          next_page = c + sub < wk.c1 && row < wk.s.len
+                          ? __ldg(p.table + static_cast<int64_t>(wk.b) * p.max_pages + i)
                           : -2;  // nothing to read
         };
         look(wk.c0);
-        for (int c = wk.c0; ok && c < wk.c1; ++c, ++gc) {
-          const int turn = (c - wk.c0) % ahead;
+        for (int c = wk.c0, turn = 0; ok && c < wk.c1; ++c, ++gc, turn = turn + 1 == ahead ? 0 : turn + 1) {
           if (turn == 0) {
             page = next_page;
-            row = next_row;
+            slot = next_slot;
             if (page != -2 && (page < 0 || page >= p.num_pages)) {
               atomicOr(p.err, DSA_DEVERR_CACHE);
               page = -1;
@@ -392,7 +413,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             look(c + ahead);
           }
           const bool mine = sub == turn;
-          const Gran g = {mine ? max(page, -1) : -1, row % p.page, wk.kvh};
+          const Gran g = {mine ? max(page, -1) : -1, slot, wk.kvh};
           const uint32_t live = __ballot_sync(0xFFFFFFFFu, g.page >= 0);
           if (mine) meta[(gc & 15) * 16 + gi] = g.page >= 0 ? 1 : 0;
           __syncwarp();
@@ -409,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (ok && !p.shared) {
         // the last chunks' V
-        const int rest = gc < C::kLag ? static_cast<int>(gc) : C::kLag;
+        const int rest = min(gc, C::kLag);
 #pragma unroll
         for (int i = C::kLag - 1; i >= 0; --i) {
           if (i < rest && ok) {
@@ -419,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // copies in flight land before the CTA's shared memory goes away
-      for (int64_t i = (seq > C::kSlots ? seq - C::kSlots : 0); i < seq; ++i)
+      for (int i = max(loads - C::kSlots, 0); i < loads; ++i)
         mbar_drain(&kv_full[i % C::kSlots], static_cast<uint32_t>((i / C::kSlots) & 1));
       if (pieces > 0) mbar_drain(q_full, (pieces - 1) & 1);
     } else if (warp == 1 && lane == 0) {
@@ -435,21 +456,25 @@ __global__ void __launch_bounds__(kThreads, 1)
           smem_u32(smem + C::kOffKV), static_cast<uint32_t>(kBox), 1024u, kLayoutSW128));
       const uint32_t p_lo = static_cast<uint32_t>(make_smem_desc(
           smem_u32(smem + C::kOffP), static_cast<uint32_t>(kBox), 1024u, kLayoutSW128));
-      int64_t gc = 0;
-      int pieces = 0;
+      Ring<C::kSlots> at;       // the next slot in the order of the loads
+      Ring<C::kSlots> old;      // shared: the slot of chunk gc - kLag
+      int gc = 0, pieces = 0;
       int gp[2] = {0, 0};       // O^T products issued per warpgroup
       int drained[2] = {0, 0};  // pieces of the warpgroup whose O^T was to be read
       uint32_t fresh_bits = 0;  // bit k: chunk gc - 1 - k is its warpgroup's first of a piece
       bool ok = true;
-      auto wait_slot = [&](int64_t i) -> bool {
-        return mbar_wait(&kv_full[i % C::kSlots], static_cast<uint32_t>((i / C::kSlots) & 1), abort_flag,
-                         p.err, DSA_DEVERR_WIN_WAIT);
+      auto wait_slot = [&]() -> bool {
+        return mbar_wait(&kv_full[at.slot], at.parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
       };
-      auto issue_o = [&](int64_t i, bool fresh) -> bool {
-        const int w = static_cast<int>(i & 1);
-        const int64_t sv = C::seq_v(p.shared, i, chunks);
-        const int s = static_cast<int>(sv % C::kSlots);
-        if (!wait_slot(sv)) return false;
+      auto issue_o = [&](int w, bool fresh) -> bool {
+        int s = old.slot;
+        if (p.shared) {
+          old.next();
+        } else {
+          if (!wait_slot()) return false;
+          s = at.slot;
+          at.next();
+        }
         mbar_arrive(&v_ready[w]);  // the softmax may clear its hidden rows
         if (!mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) return false;
         if (fresh) {
@@ -478,13 +503,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; ok && j < n; ++j, ++gc) {
           // S^T runs ahead of the softmax: the buffer held S^T(gc - kSBufs), whose readers
           // arrived before O^T(gc - kSBufs) was issued
-          const int64_t sk = C::seq_k(p.shared, gc);
-          const int s = static_cast<int>(sk % C::kSlots);
-          ok = wait_slot(sk);
+          ok = wait_slot();
           if (!ok) break;
+          const int s = at.slot;
+          at.next();
           tc_fence_after();
           const uint32_t ka = k_lo + static_cast<uint32_t>(s * (C::kSlotBytes >> 4));
-          const uint32_t buf = static_cast<uint32_t>(gc % C::kSBufs);
+          const uint32_t buf = static_cast<uint32_t>(gc) % C::kSBufs;
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBox + (k & 3) * 32) >> 4);
@@ -495,12 +520,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_commit(&s_full[buf]);
           if (!p.shared) umma_commit(&kv_empty[s]);
           if (j == n - 1) umma_commit(q_empty);
-          if (gc >= C::kLag) ok = issue_o(gc - C::kLag, (fresh_bits >> (C::kLag - 1)) & 1u);
+          if (gc >= C::kLag) ok = issue_o((gc - C::kLag) & 1, (fresh_bits >> (C::kLag - 1)) & 1u);
           fresh_bits = (fresh_bits << 1) | (j < 2 ? 1u : 0u);
         }
       }
-      for (int64_t i = gc < C::kLag ? 0 : gc - C::kLag; ok && i < gc; ++i)
-        ok = issue_o(i, (fresh_bits >> (gc - 1 - i)) & 1u);
+      for (int i = max(gc - C::kLag, 0); ok && i < gc; ++i)
+        ok = issue_o(i & 1, (fresh_bits >> (gc - 1 - i)) & 1u);
       umma_commit(drain_bar);
       mbar_drain(drain_bar, 0);
     }
@@ -516,13 +541,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t od = tmem + lane_off + static_cast<uint32_t>(C::kColsO + w * NM);
     const uint32_t bar = 1 + static_cast<uint32_t>(w);
-    float* wmax = reinterpret_cast<float*>(smem + C::kOffMax) + w * 4 * NM;
-    float* nref = reinterpret_cast<float*>(smem + C::kOffRef) + w * 2 * NM;  // -reference
-    float* move = nref + NM;                                                 // its last step
+    // shared-memory addresses of the warpgroup's per-warp maxima [4][NM], the heads'
+    // negative references [NM] and their last steps [NM]
+    const uint32_t wmax = smem_u32(smem + C::kOffMax) + static_cast<uint32_t>(w * 4 * NM * 4);
+    const uint32_t nref = smem_u32(smem + C::kOffRef) + static_cast<uint32_t>(w * 2 * NM * 4);
+    const uint32_t move = nref + NM * 4;
+    const int gi = key / p.gran;  // the key's granule of a chunk and row of it
+    const int gr = key - gi * p.gran;
     const uint32_t prow = smem_u32(smem + C::kOffP) + static_cast<uint32_t>(w * C::kPBytes + key * 128);
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
-    int64_t gc = 0;
-    int gw = 0;
+    int gc = 0, gw = 0;
     uint32_t sp = 0;  // the chunk's S^T
     auto wait = [&](uint64_t* b, uint32_t parity) {  // whole warps
       mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
@@ -534,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld_32x32b_x32(sp + static_cast<uint32_t>(q * 32), v);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const float4 r = reinterpret_cast<const float4*>(nref)[q * 8 + k];
+        const float4 r = ld_shared_f4(nref + static_cast<uint32_t>(q * 128 + k * 16));
         d[2 * k] = f2_fma(f2_pack(__uint_as_float(v[4 * k]), __uint_as_float(v[4 * k + 1])), scale2,
                           f2_pack(r.x, r.y));
         d[2 * k + 1] = f2_fma(f2_pack(__uint_as_float(v[4 * k + 2]), __uint_as_float(v[4 * k + 3])),
@@ -547,15 +575,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = 0; k < NM / 2; ++k) l2[k] = 0ull;
       const int n = wk.c1 - wk.c0;
       bool fresh = true;
-      if (key < npad) nref[key] = 0.f;
+      if (key < npad) st_shared_f32(nref + key * 4, 0.f);
       named_bar_sync(bar, 128);
       for (int j = 0; j < n; ++j, ++gc) {
         if ((gc & 1) != w) continue;
         const int c = wk.c0 + j;
-        const int gi = key / p.gran;
-        const int row = gran_row(p, wk.s, c * gpc + gi) + (key - gi * p.gran);
-        sp = tmem + lane_off + static_cast<uint32_t>(gc % C::kSBufs) * NM;
-        wait(&s_full[gc % C::kSBufs], static_cast<uint32_t>((gc / C::kSBufs) & 1));
+        const int row = gran_row(p, wk.s, c * gpc + gi) + gr;
+        const uint32_t buf = static_cast<uint32_t>(gc) % C::kSBufs;
+        sp = tmem + lane_off + buf * NM;
+        wait(&s_full[buf], (static_cast<uint32_t>(gc) / C::kSBufs) & 1u);
         tc_fence_after();
         const bool valid = row_seen(wk.s, c * gpc + gi, row) && meta[(gc & 15) * 16 + gi] != 0;
         // up to 64 heads the scores stay in registers; beyond, they are loaded again
@@ -583,25 +611,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (q * 32 < npad) {
               uint64_t(&x)[16] = d[kHold ? q : 0];
               if (!kHold) load_scores(q, x);
-              float mine = 0.f;
+              float a[32];
 #pragma unroll
               for (int k = 0; k < 16; ++k) {
-                float a, b;
-                f2_unpack(x[k], a, b);
-                const float ma = warp_max(valid ? a : kNone), mb = warp_max(valid ? b : kNone);
-                if (lane == 2 * k) mine = ma;
-                if (lane == 2 * k + 1) mine = mb;
+                f2_unpack(x[k], a[2 * k], a[2 * k + 1]);
+                a[2 * k] = valid ? a[2 * k] : kNone;
+                a[2 * k + 1] = valid ? a[2 * k + 1] : kNone;
               }
-              wmax[quarter * NM + q * 32 + lane] = mine;
+              const float m = warp_transposed(a, lane, [](float u, float v) { return fmaxf(u, v); });
+              st_shared_f32(wmax + static_cast<uint32_t>((quarter * NM + q * 32 + lane) * 4), m);
             }
           }
           named_bar_sync(bar, 128);
           if (key < npad) {
-            const float m = fmaxf(fmaxf(wmax[key], wmax[NM + key]),
-                                  fmaxf(wmax[2 * NM + key], wmax[3 * NM + key]));
+            float m = ld_shared_f32(wmax + key * 4);
+#pragma unroll
+            for (int i = 1; i < 4; ++i)
+              m = fmaxf(m, ld_shared_f32(wmax + static_cast<uint32_t>((i * NM + key) * 4)));
             const float step = fresh || m > kRescaleLog2 ? m : 0.f;
-            nref[key] -= step;
-            move[key] = step;
+            st_shared_f32(nref + key * 4, ld_shared_f32(nref + key * 4) - step);
+            st_shared_f32(move + key * 4, step);
           }
           named_bar_sync(bar, 128);
           if (!fresh) {
@@ -615,7 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!fresh) tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
 #pragma unroll
               for (int k = 0; k < 16; ++k) {
-                const float s0 = move[q * 32 + 2 * k], s1 = move[q * 32 + 2 * k + 1];
+                const float s0 = ld_shared_f32(move + static_cast<uint32_t>((q * 32 + 2 * k) * 4));
+                const float s1 = ld_shared_f32(move + static_cast<uint32_t>((q * 32 + 2 * k) * 4 + 4));
                 if (kHold) d[q][k] = f2_sub(d[q][k], f2_pack(s0, s1));
                 if (!fresh) {
                   const float f0 = ex2_approx(-s0), f1 = ex2_approx(-s1);
@@ -652,8 +682,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int k = 0; k < 16; ++k) {
                 float a, b;
                 f2_unpack(x[k], a, b);
-                if (q * 32 + 2 * k < p.g) zrow[q * 32 + 2 * k] = a - nref[q * 32 + 2 * k];
-                if (q * 32 + 2 * k + 1 < p.g) zrow[q * 32 + 2 * k + 1] = b - nref[q * 32 + 2 * k + 1];
+                const int i = q * 32 + 2 * k;
+                if (i < p.g) zrow[i] = a - ld_shared_f32(nref + i * 4);
+                if (i + 1 < p.g) zrow[i + 1] = b - ld_shared_f32(nref + i * 4 + 4);
               }
             }
             uint32_t pk[16];
@@ -678,9 +709,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!valid) {
           // a hidden V row may hold anything, and 0 x NaN is NaN: it is cleared. The issuer,
           // which waits for the slots in their order, says when V is there
-          const int64_t sv = C::seq_v(p.shared, gc, chunks);
+          const int sv = C::slot_v(p.shared, gc, chunks);
           mbar_wait(&v_ready[w], gw & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
-          uint8_t* vr = smem + C::kOffKV + (sv % C::kSlots) * C::kSlotBytes + key * 128;
+          uint8_t* vr = smem + C::kOffKV + sv * C::kSlotBytes + key * 128;
 #pragma unroll
           for (int x = 0; x < C::kHalves * 8; ++x)
             st_shared_v4(smem_u32(vr + (x >> 3) * kBox + (x & 7) * 16), 0u, 0u, 0u, 0u);
@@ -704,20 +735,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int q = 0; q < NM / 32; ++q) {
         if (q * 32 < npad) {
-          // sums over the warp's 32 keys of 32 heads: lane k ends with head k
+          // sums over the warp's 32 keys of 32 heads
           float a[32];
 #pragma unroll
           for (int k = 0; k < 16; ++k) f2_unpack(l2[q * 16 + k], a[2 * k], a[2 * k + 1]);
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) {
-            const bool up = (lane & o) != 0;
-#pragma unroll
-            for (int k = 0; k < o; ++k) {
-              const float send = up ? a[k] : a[k + o];
-              a[k] = (up ? a[k + o] : a[k]) + __shfl_xor_sync(0xFFFFFFFFu, send, o);
-            }
-          }
-          wmax[quarter * NM + q * 32 + lane] = a[0];
+          const float sum = warp_transposed(a, lane, [](float u, float v) { return u + v; });
+          st_shared_f32(wmax + static_cast<uint32_t>((quarter * NM + q * 32 + lane) * 4), sum);
           uint32_t v[32];
           tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
           if (key < D) {
@@ -731,9 +754,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       mbar_arrive(&o_empty[w]);
       named_bar_sync(bar, 128);
-      if (key < p.g)
-        ml[key] = make_float2(-nref[key], (wmax[key] + wmax[NM + key]) +
-                                            (wmax[2 * NM + key] + wmax[3 * NM + key]));
+      if (key < p.g) {
+        float sum = ld_shared_f32(wmax + key * 4);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) sum += ld_shared_f32(wmax + static_cast<uint32_t>((i * NM + key) * 4));
+        ml[key] = make_float2(-ld_shared_f32(nref + key * 4), sum);
+      }
       named_bar_sync(bar, 128);  // the next piece writes the references and maxima
     }
   }
@@ -785,7 +811,8 @@ __global__ void __launch_bounds__(D) paged_join_kernel(const Params p) {
   };
   float top = kNone;
   for (int i = x; i < parts; i += D) top = fmaxf(top, part(i).x);
-  top = warp_max(top);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
   if ((x & 31) == 0) red[0][warp] = top;
   __syncthreads();
 #pragma unroll

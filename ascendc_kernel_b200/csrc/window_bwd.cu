@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int tok_b = min(max(end - p0, 0), p.tt);
         const int dup = (r % p.hb) == 0 ? 0 : p.hb * p.gb - p.s.g;
         const int ca = max(tok_a * p.gb, dup), cb = tok_b * p.gb;
-        const float4* stat4 = reinterpret_cast<const float4*>(stat_s + s * 2 * kStream);
+        const uint32_t stat4 = smem_u32(smem + C::kOffStat) + static_cast<uint32_t>(s * 2 * kStream * 4);
         // the statistics were written with ordinary stores: their barrier is waited
         // for here too (it completed before this tile's products were issued)
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&st_full[s], ((gs + i) / C::kStages) & 1, abort_flag,
@@ -419,7 +419,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           uint32_t pk[16], dk[16];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float4 nl = stat4[q * 8 + k], nd = stat4[16 + q * 8 + k];
+            const float4 nl = ld_shared_f4(stat4 + static_cast<uint32_t>((q * 8 + k) * 16));
+            const float4 nd = ld_shared_f4(stat4 + static_cast<uint32_t>((16 + q * 8 + k) * 16));
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int c = 4 * k + 2 * e;

@@ -76,6 +76,8 @@ CASES = [
     ([129, 1000, 63], 16, 12, 2, 100, 4), ([1500, 257], 128, 128, 1, 0, 0),
     ([900, 31], 64, 77, 1, 300, 130), ([513, 40], 40, 4, 4, 1, 1), ([200, 199], 32, 2, 1, 33, 200),
     ([3 + 7 * i for i in range(40)], 32, 33, 1, 17, 3), ([9000, 1, 0, 130], 40, 8, 2, 0, 0),
+    # several pieces and tens of chunks to each block of the split kernel
+    ([5000, 625, 4200, 3111, 2000, 901, 4999], 64, 32, 8, 0, 0), ([30000, 29000], 16, 64, 1, 0, 0),
 ]
 
 
