@@ -23,9 +23,9 @@
 //   warp 1      tcgen05 issuer
 //   warps 4..11 softmax: warpgroup w takes the chunks of parity w, with its own
 //               accumulator, reference and sums; S^T products run up to three chunks ahead
-// The reference of a head is set by a warpgroup's first chunk of a piece and
-// moves (O and the sums are rescaled) only when a score exceeds it by more than
-// 2^8, so the common chunk needs one vote and no reduction over keys; the sums
+// The reference of a head is the score of a warpgroup's first visible key of a
+// piece and moves (O and the sums are rescaled) only when a score exceeds it by more
+// than 2^14, so the common chunk needs one vote and no reduction over keys; the sums
 // stay per thread until the piece ends. P is rounded to the operands' type
 // (relative 2^-8 at most for bf16, the size of the output's own rounding); sums are fp32.
 // TMEM: kSBufs S^T buffers of NM columns, then O^T of the two warpgroups.
@@ -46,7 +46,7 @@ constexpr int kRegsAux = 88;        // 128 x 88 + 256 x 208 = 384 x 168 at launc
 constexpr int kRegsSoftmax = 208;
 constexpr int kKeys = 128;          // keys of a chunk
 constexpr int kBox = kKeys * 128;   // one [128 keys x 64 columns] SW128 box
-constexpr float kRescaleLog2 = 8.0f;
+constexpr float kRescaleLog2 = 14.0f;  // P <= 2^14 fits fp16
 constexpr int kMaxSmem = 232448;
 constexpr float kNone = -1.0e30f;   // reference of a piece without a visible key
 
@@ -86,7 +86,8 @@ struct Cfg {
 
 struct Params {
   int batch, h, hk, g;
-  int page, max_pages, gran;  // page size, table width, rows of a granule
+  int page, max_pages;        // page size, table width
+  int gran, gshift;           // rows of a granule, a power of two
   int64_t num_pages;
   int window, n_first;        // window 0: the whole sequence
   const int* table;           // [batch, max_pages]
@@ -121,11 +122,10 @@ __device__ __forceinline__ Seq make_seq(const Params& p, int b) {
   s.lo = p.window > 0 ? max(s.len - p.window, 0) : 0;
   s.nf = min(p.n_first, s.len);
   if (s.lo <= s.nf) s.lo = s.nf = 0;
-  s.start = s.lo - s.lo % p.gran;
-  s.nfg = (s.nf + p.gran - 1) / p.gran;
-  const int per = kKeys / p.gran;
-  const int n = s.nfg + (s.len - s.start + p.gran - 1) / p.gran;
-  s.chunks = (n + per - 1) / per;
+  s.start = s.lo & -p.gran;
+  s.nfg = (s.nf + p.gran - 1) >> p.gshift;
+  const int n = s.nfg + ((s.len - s.start + p.gran - 1) >> p.gshift);
+  s.chunks = ((n << p.gshift) + kKeys - 1) / kKeys;
   return s;
 }
 __device__ __forceinline__ int seq_chunks(const Params& p, int b) { return make_seq(p, b).chunks; }
@@ -143,28 +143,36 @@ __device__ __forceinline__ int page_of(const Params& p, int b, int row) {
   return page >= 0 && page < p.num_pages ? page : -1;
 }
 
-// Chunks of all sequences before b and of the whole batch, summed by one warp.
-__device__ __forceinline__ void chunk_sums(const Params& p, int b, int64_t* before, int64_t* all) {
-  int64_t x = 0, y = 0;
+// The line of all chunks cut into `units` stretches whose lengths differ by one at
+// most: the first `more` have each + 1 chunks.
+struct Line {
+  int each, more;
+  __device__ __forceinline__ Line(int all, int units) : each(all / units), more(all - each * units) {}
+  __device__ __forceinline__ int start(int u) const { return u * each + min(u, more); }
+  __device__ __forceinline__ int owner(int chunk) const {
+    const int longer = more * (each + 1);
+    return chunk < longer ? chunk / (each + 1) : more + (chunk - longer) / each;
+  }
+};
+
+// Chunks (of one kv head) of all sequences before b and of the whole batch, summed by
+// one warp.
+__device__ __forceinline__ void chunk_sums(const Params& p, int b, int* before, int* all) {
+  int x = 0, y = 0;
   for (int i = threadIdx.x & 31; i < p.batch; i += 32) {
     const int n = seq_chunks(p, i);
     y += n;
     if (i < b) x += n;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
-    y += __shfl_xor_sync(0xFFFFFFFFu, y, o);
-  }
-  *before = x;
-  *all = y;
+  *before = __reduce_add_sync(0xFFFFFFFFu, x);
+  *all = __reduce_add_sync(0xFFFFFFFFu, y);
 }
 
 // A CTA's stretch, walked piece by piece. The line orders the chunks by (sequence,
 // kv head, chunk).
 struct Walk {
   int b, kvh, c0, c1;   // the piece: chunks [c0, c1) of (b, kvh)
-  int64_t left;         // chunks of the stretch after this piece
+  int left;             // chunks of the stretch after this piece
   Seq s;
 };
 
@@ -181,8 +189,7 @@ __device__ __forceinline__ bool walk_take(const Params& p, Walk& w) {
       }
       continue;
     }
-    const int64_t n = w.s.chunks - w.c0;
-    w.c1 = w.c0 + static_cast<int>(n < w.left ? n : w.left);
+    w.c1 = w.c0 + min(w.s.chunks - w.c0, w.left);
     w.left -= w.c1 - w.c0;
     return true;
   }
@@ -246,13 +253,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain_bar = v_ready + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
-  int* walk_s = reinterpret_cast<int*>(smem + C::kOffMisc + 8);  // b, kvh, chunk, left (2 words)
+  int* walk_s = reinterpret_cast<int*>(smem + C::kOffMisc + 8);  // b, kvh, chunk, left
   int* meta = reinterpret_cast<int*>(smem + C::kOffMeta);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int npad = (p.g + 31) & ~31;
-  const int gpc = kKeys / p.gran;  // granules of a chunk
+  const int gpc = kKeys >> p.gshift;  // granules of a chunk
 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
@@ -276,40 +283,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_v);
   }
   // rows of q past the group stay 0: their scores are 0, their columns are not used
-  for (int i = threadIdx.x; i < C::kQBytes / 16; i += kThreads)
-    st_shared_v4(smem_u32(smem + C::kOffQ + i * 16), 0u, 0u, 0u, 0u);
-  fence_proxy_async_smem();
+  if (p.g < npad) {
+    for (int i = threadIdx.x; i < C::kQBytes / 16; i += kThreads)
+      st_shared_v4(smem_u32(smem + C::kOffQ + i * 16), 0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+  }
   if (warp == 1) {
     tmem_alloc(tmem_holder, C::kTmemCols);
     tmem_relinquish();
   }
   if (warp == 2) {
     // where this CTA's stretch [first, last) of the line starts
-    int64_t unused, all;
+    int unused, all;
     chunk_sums(p, 0, &unused, &all);
-    all *= p.hk;
-    const int64_t first = all * blockIdx.x / p.units;
-    const int64_t last = all * (blockIdx.x + 1) / p.units;
-    int64_t base = 0;  // chunks before the 32 sequences that the lanes hold
+    const Line line(all * p.hk, p.units);
+    const int first = line.start(blockIdx.x), last = line.start(blockIdx.x + 1);
+    int base = 0;  // chunks before the 32 sequences that the lanes hold
     int b = p.batch, kvh = 0, c = 0;
     bool found = first >= last;
     for (int i0 = 0; i0 < p.batch && !found; i0 += 32) {
-      const int64_t mine =
-          i0 + lane < p.batch ? static_cast<int64_t>(seq_chunks(p, i0 + lane)) * p.hk : 0;
-      int64_t sum = mine;  // inclusive prefix over the lanes
+      const int mine = i0 + lane < p.batch ? seq_chunks(p, i0 + lane) * p.hk : 0;
+      int sum = mine;  // inclusive prefix over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
+        const int y = __shfl_up_sync(0xFFFFFFFFu, sum, o);
         if (lane >= o) sum += y;
       }
       const uint32_t hit = __ballot_sync(0xFFFFFFFFu, first < base + sum && mine > 0);
       if (hit != 0) {
         const int l = __ffs(hit) - 1;
-        const int64_t begin = base + __shfl_sync(0xFFFFFFFFu, sum - mine, l);
-        const int64_t n = __shfl_sync(0xFFFFFFFFu, mine, l) / p.hk;
+        const int begin = base + __shfl_sync(0xFFFFFFFFu, sum - mine, l);
+        const int n = __shfl_sync(0xFFFFFFFFu, mine, l) / p.hk;
         b = i0 + l;
-        kvh = static_cast<int>((first - begin) / n);
-        c = static_cast<int>((first - begin) - static_cast<int64_t>(kvh) * n);
+        kvh = (first - begin) / n;
+        c = (first - begin) - kvh * n;
         found = true;
       }
       base += __shfl_sync(0xFFFFFFFFu, sum, 31);
@@ -318,16 +325,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       walk_s[0] = b;
       walk_s[1] = kvh;
       walk_s[2] = c;
-      *reinterpret_cast<int64_t*>(walk_s + 4) = last > first ? last - first : 0;
-      if (blockIdx.x == 0) {
-        // lengths outside the table's room are clamped and reported
-        bool bad = false;
-        for (int i = 0; i < p.batch; ++i) {
-          const int n = __ldg(p.lens + i);
-          bad = bad || n < 0 || n > static_cast<int64_t>(p.max_pages) * p.page;
-        }
-        if (bad) atomicOr(p.err, DSA_DEVERR_CACHE);
-      }
+      walk_s[3] = last - first;
+    }
+  }
+  if (warp == 3 && blockIdx.x == 0) {
+    // lengths outside the table's room are clamped and reported
+    for (int i = lane; i < p.batch; i += 32) {
+      const int n = __ldg(p.lens + i);
+      if (n < 0 || n > static_cast<int64_t>(p.max_pages) * p.page) atomicOr(p.err, DSA_DEVERR_CACHE);
     }
   }
   tc_fence_before();
@@ -338,8 +343,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   wk.b = walk_s[0];
   wk.kvh = walk_s[1];
   wk.c0 = walk_s[2];
-  wk.left = *reinterpret_cast<const int64_t*>(walk_s + 4);
-  const int chunks = static_cast<int>(wk.left);  // of the whole stretch
+  wk.left = walk_s[3];
+  const int chunks = wk.left;  // of the whole stretch
 
   if (warp < 4) {
     win::set_max_regs_dec<kRegsAux>();
@@ -443,8 +448,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = max(loads - C::kSlots, 0); i < loads; ++i)
         mbar_drain(&kv_full[i % C::kSlots], static_cast<uint32_t>((i / C::kSlots) & 1));
       if (pieces > 0) mbar_drain(q_full, (pieces - 1) & 1);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------- MMA issuer
+      // The whole warp walks and waits; one elected lane issues.
       const uint32_t idesc_s = win::make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(npad / 8) << 17);
       const uint32_t idesc_o = win::make_idesc<T>(128, 0, 1) | (1u << 15) |
                                (static_cast<uint32_t>(npad / 8) << 17);
@@ -463,8 +469,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       int drained[2] = {0, 0};  // pieces of the warpgroup whose O^T was to be read
       uint32_t fresh_bits = 0;  // bit k: chunk gc - 1 - k is its warpgroup's first of a piece
       bool ok = true;
+      auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
+        return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+      };
       auto wait_slot = [&]() -> bool {
-        return mbar_wait(&kv_full[at.slot], at.parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+        return wait_warp(&kv_full[at.slot], at.parity);
       };
       auto issue_o = [&](int w, bool fresh) -> bool {
         int s = old.slot;
@@ -475,30 +484,31 @@ __global__ void __launch_bounds__(kThreads, 1)
           s = at.slot;
           at.next();
         }
-        mbar_arrive(&v_ready[w]);  // the softmax may clear its hidden rows
-        if (!mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) return false;
+        if (lane == 0) mbar_arrive(&v_ready[w]);  // the softmax may clear its hidden rows
+        if (!wait_warp(&p_full[w], gp[w] & 1)) return false;
         if (fresh) {
-          if (drained[w] > 0 && !mbar_wait(&o_empty[w], (drained[w] - 1) & 1, abort_flag, p.err,
-                                           DSA_DEVERR_WIN_WAIT))
-            return false;
+          if (drained[w] > 0 && !wait_warp(&o_empty[w], (drained[w] - 1) & 1)) return false;
           ++drained[w];
         }
         tc_fence_after();
         const uint32_t va = v_lo + static_cast<uint32_t>(s * (C::kSlotBytes >> 4));
         const uint32_t pb = p_lo + static_cast<uint32_t>(w * (C::kPBytes >> 4));
         const uint32_t d = tmem + static_cast<uint32_t>(C::kColsO + w * NM);
+        if (elect_one()) {
 #pragma unroll
-        for (int st = 0; st < kKeys / 16; ++st)
-          umma_bf16(d, desc_from_words(va + static_cast<uint32_t>(st * 128), hi),
-                    desc_from_words(pb + static_cast<uint32_t>(st * 128), hi), idesc_o,
-                    (fresh && st == 0) ? 0u : 1u);
-        umma_commit(&o_done[w]);
-        umma_commit(&kv_empty[s]);
+          for (int st = 0; st < kKeys / 16; ++st)
+            umma_bf16(d, desc_from_words(va + static_cast<uint32_t>(st * 128), hi),
+                      desc_from_words(pb + static_cast<uint32_t>(st * 128), hi), idesc_o,
+                      (fresh && st == 0) ? 0u : 1u);
+          umma_commit(&o_done[w]);
+          umma_commit(&kv_empty[s]);
+        }
+        __syncwarp();
         ++gp[w];
         return true;
       };
       for (; ok && walk_take(p, wk); walk_next(wk), ++pieces) {
-        ok = mbar_wait(q_full, pieces & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+        ok = wait_warp(q_full, pieces & 1);
         const int n = wk.c1 - wk.c0;
         for (int j = 0; ok && j < n; ++j, ++gc) {
           // S^T runs ahead of the softmax: the buffer held S^T(gc - kSBufs), whose readers
@@ -510,24 +520,29 @@ __global__ void __launch_bounds__(kThreads, 1)
           tc_fence_after();
           const uint32_t ka = k_lo + static_cast<uint32_t>(s * (C::kSlotBytes >> 4));
           const uint32_t buf = static_cast<uint32_t>(gc) % C::kSBufs;
+          if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBox + (k & 3) * 32) >> 4);
-            const uint32_t bo = static_cast<uint32_t>(((k >> 2) * NM * 128 + (k & 3) * 32) >> 4);
-            umma_bf16(tmem + buf * NM, desc_from_words(ka + ao, hi), desc_from_words(q_lo + bo, hi),
-                      idesc_s, k > 0 ? 1u : 0u);
+            for (int k = 0; k < D / 16; ++k) {
+              const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBox + (k & 3) * 32) >> 4);
+              const uint32_t bo = static_cast<uint32_t>(((k >> 2) * NM * 128 + (k & 3) * 32) >> 4);
+              umma_bf16(tmem + buf * NM, desc_from_words(ka + ao, hi), desc_from_words(q_lo + bo, hi),
+                        idesc_s, k > 0 ? 1u : 0u);
+            }
+            umma_commit(&s_full[buf]);
+            if (!p.shared) umma_commit(&kv_empty[s]);
+            if (j == n - 1) umma_commit(q_empty);
           }
-          umma_commit(&s_full[buf]);
-          if (!p.shared) umma_commit(&kv_empty[s]);
-          if (j == n - 1) umma_commit(q_empty);
+          __syncwarp();
           if (gc >= C::kLag) ok = issue_o((gc - C::kLag) & 1, (fresh_bits >> (C::kLag - 1)) & 1u);
           fresh_bits = (fresh_bits << 1) | (j < 2 ? 1u : 0u);
         }
       }
       for (int i = max(gc - C::kLag, 0); ok && i < gc; ++i)
         ok = issue_o(i & 1, (fresh_bits >> (gc - 1 - i)) & 1u);
-      umma_commit(drain_bar);
+      if (elect_one()) umma_commit(drain_bar);
+      __syncwarp();
       mbar_drain(drain_bar, 0);
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ softmax
@@ -546,8 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t wmax = smem_u32(smem + C::kOffMax) + static_cast<uint32_t>(w * 4 * NM * 4);
     const uint32_t nref = smem_u32(smem + C::kOffRef) + static_cast<uint32_t>(w * 2 * NM * 4);
     const uint32_t move = nref + NM * 4;
-    const int gi = key / p.gran;  // the key's granule of a chunk and row of it
-    const int gr = key - gi * p.gran;
+    const int gi = key >> p.gshift;  // the key's granule of a chunk and row of it
+    const int gr = key & (p.gran - 1);
     const uint32_t prow = smem_u32(smem + C::kOffP) + static_cast<uint32_t>(w * C::kPBytes + key * 128);
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int gc = 0, gw = 0;
@@ -574,7 +589,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int k = 0; k < NM / 2; ++k) l2[k] = 0ull;
       const int n = wk.c1 - wk.c0;
-      bool fresh = true;
+      bool fresh = true;  // no chunk of the piece yet
+      bool unset = true;  // no visible key yet: the references stand at 0
       if (key < npad) st_shared_f32(nref + key * 4, 0.f);
       named_bar_sync(bar, 128);
       for (int j = 0; j < n; ++j, ++gc) {
@@ -589,12 +605,53 @@ __global__ void __launch_bounds__(kThreads, 1)
         // up to 64 heads the scores stay in registers; beyond, they are loaded again
         constexpr bool kHold = NM <= 64;
         uint64_t d[kHold ? NM / 32 : 1][16];
+#pragma unroll
+        for (int q = 0; q < NM / 32; ++q)
+          if (kHold && q * 32 < npad) load_scores(q, d[q]);
+        if (unset) {
+          // the references are the scores of the first visible key: any key does, as long
+          // as the vote below moves a reference that others exceed by far
+          const uint32_t seen = __ballot_sync(0xFFFFFFFFu, valid);
+          if (lane == 0) st_shared_f32(wmax + quarter * 4, __uint_as_float(seen));
+          named_bar_sync(bar, 128);
+          int owner = -1;
+#pragma unroll
+          for (int i = 3; i >= 0; --i)
+            if (__float_as_uint(ld_shared_f32(wmax + i * 4)) != 0u) owner = i;
+          if (owner >= 0) {
+            const bool mine = quarter == owner && lane == __ffs(seen) - 1;
+#pragma unroll
+            for (int q = 0; q < NM / 32; ++q) {
+              if (q * 32 < npad) {
+                uint64_t(&x)[16] = d[kHold ? q : 0];
+                if (!kHold) {
+                  named_bar_sync(bar, 128);  // all warps read the references of 0
+                  load_scores(q, x);
+                }
+                if (mine) {
+#pragma unroll
+                  for (int k = 0; k < 16; ++k) {
+                    float a, b;
+                    f2_unpack(x[k], a, b);
+                    st_shared_f32(nref + static_cast<uint32_t>((q * 32 + 2 * k) * 4), -a);
+                    st_shared_f32(nref + static_cast<uint32_t>((q * 32 + 2 * k) * 4 + 4), -b);
+                  }
+                }
+              }
+            }
+            named_bar_sync(bar, 128);
+#pragma unroll
+            for (int q = 0; q < NM / 32; ++q)
+              if (kHold && q * 32 < npad) load_scores(q, d[q]);
+            unset = false;
+          }
+        }
         float excess = -INFINITY;
 #pragma unroll
         for (int q = 0; q < NM / 32; ++q) {
           if (q * 32 < npad) {
             uint64_t(&x)[16] = d[kHold ? q : 0];
-            load_scores(q, x);
+            if (!kHold) load_scores(q, x);
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
               float a, b;
@@ -603,24 +660,24 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        // does any score exceed its head's reference by more than 2^8?
-        if (named_bar_or(bar, 128, fresh || (valid && excess > kRescaleLog2))) {
+        // does any score exceed its head's reference by more than 2^14? Rare: the code is
+        // kept short (rolled loops), so that it does not push the common path out of the
+        // instruction cache
+        if (named_bar_or(bar, 128, valid && excess > kRescaleLog2)) {
           // the heads' maxima over the chunk's keys: warps, then the warpgroup
+#pragma unroll 1
+          for (int q = 0; q * 32 < npad; ++q) {
+            uint64_t x[16];
+            load_scores(q, x);
+            float a[32];
 #pragma unroll
-          for (int q = 0; q < NM / 32; ++q) {
-            if (q * 32 < npad) {
-              uint64_t(&x)[16] = d[kHold ? q : 0];
-              if (!kHold) load_scores(q, x);
-              float a[32];
-#pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                f2_unpack(x[k], a[2 * k], a[2 * k + 1]);
-                a[2 * k] = valid ? a[2 * k] : kNone;
-                a[2 * k + 1] = valid ? a[2 * k + 1] : kNone;
-              }
-              const float m = warp_transposed(a, lane, [](float u, float v) { return fmaxf(u, v); });
-              st_shared_f32(wmax + static_cast<uint32_t>((quarter * NM + q * 32 + lane) * 4), m);
+            for (int k = 0; k < 16; ++k) {
+              f2_unpack(x[k], a[2 * k], a[2 * k + 1]);
+              a[2 * k] = valid ? a[2 * k] : kNone;
+              a[2 * k + 1] = valid ? a[2 * k + 1] : kNone;
             }
+            const float m = warp_transposed(a, lane, [](float u, float v) { return fmaxf(u, v); });
+            st_shared_f32(wmax + static_cast<uint32_t>((quarter * NM + q * 32 + lane) * 4), m);
           }
           named_bar_sync(bar, 128);
           if (key < npad) {
@@ -628,35 +685,40 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int i = 1; i < 4; ++i)
               m = fmaxf(m, ld_shared_f32(wmax + static_cast<uint32_t>((i * NM + key) * 4)));
-            const float step = fresh || m > kRescaleLog2 ? m : 0.f;
+            const float step = m > kRescaleLog2 ? m : 0.f;
             st_shared_f32(nref + key * 4, ld_shared_f32(nref + key * 4) - step);
-            st_shared_f32(move + key * 4, step);
+            st_shared_f32(move + key * 4, ex2_approx(-step));
           }
           named_bar_sync(bar, 128);
           if (!fresh) {
             wait(&o_done[w], (gw - 1) & 1);
             tc_fence_after();
-          }
-#pragma unroll
-          for (int q = 0; q < NM / 32; ++q) {
-            if (q * 32 < npad) {
+#pragma unroll 1
+            for (int q = 0; q * 32 < npad; ++q) {
               uint32_t v[32];
-              if (!fresh) tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
+              tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
 #pragma unroll
-              for (int k = 0; k < 16; ++k) {
-                const float s0 = ld_shared_f32(move + static_cast<uint32_t>((q * 32 + 2 * k) * 4));
-                const float s1 = ld_shared_f32(move + static_cast<uint32_t>((q * 32 + 2 * k) * 4 + 4));
-                if (kHold) d[q][k] = f2_sub(d[q][k], f2_pack(s0, s1));
-                if (!fresh) {
-                  const float f0 = ex2_approx(-s0), f1 = ex2_approx(-s1);
-                  l2[q * 16 + k] = f2_mul(l2[q * 16 + k], f2_pack(f0, f1));
-                  v[2 * k] = __float_as_uint(__uint_as_float(v[2 * k]) * f0);
-                  v[2 * k + 1] = __float_as_uint(__uint_as_float(v[2 * k + 1]) * f1);
-                }
+              for (int k = 0; k < 8; ++k) {
+                const float4 f = ld_shared_f4(move + static_cast<uint32_t>(q * 128 + k * 16));
+                v[4 * k] = __float_as_uint(__uint_as_float(v[4 * k]) * f.x);
+                v[4 * k + 1] = __float_as_uint(__uint_as_float(v[4 * k + 1]) * f.y);
+                v[4 * k + 2] = __float_as_uint(__uint_as_float(v[4 * k + 2]) * f.z);
+                v[4 * k + 3] = __float_as_uint(__uint_as_float(v[4 * k + 3]) * f.w);
               }
-              if (!fresh) tmem_st_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
+              tmem_st_32x32b_x32(od + static_cast<uint32_t>(q * 32), v);
+            }
+#pragma unroll
+            for (int k = 0; k < NM / 4; ++k) {
+              if (4 * k < npad) {
+                const float4 f = ld_shared_f4(move + static_cast<uint32_t>(k * 16));
+                l2[2 * k] = f2_mul(l2[2 * k], f2_pack(f.x, f.y));
+                l2[2 * k + 1] = f2_mul(l2[2 * k + 1], f2_pack(f.z, f.w));
+              }
             }
           }
+#pragma unroll
+          for (int q = 0; q < NM / 32; ++q)
+            if (kHold && q * 32 < npad) load_scores(q, d[q]);
         }
         // ---- P = 2^(z - reference), the key's weights of all heads
         if (gw > 0) wait(&o_done[w], (gw - 1) & 1);  // the previous product has read P
@@ -784,29 +846,20 @@ __global__ void __launch_bounds__(D) paged_join_kernel(const Params p) {
   const int b = blockIdx.x / p.h;
   const int kvh = head / p.g, gi = head - kvh * p.g;
   const int x = threadIdx.x, warp = x >> 5;
-  int64_t before, all;
+  int before, all;
   chunk_sums(p, b, &before, &all);
-  const int64_t n = seq_chunks(p, b);
-  const int64_t first = before * p.hk + kvh * n, last = first + n;
-  all *= p.hk;
+  const int n = seq_chunks(p, b);
+  const Line line(all * p.hk, p.units);
   const float sink2 = p.sink != nullptr ? __ldg(p.sink + head) * kLog2e : -INFINITY;
-  int64_t u0 = 0;
-  int parts = 0;  // two (warpgroups) per piece
+  int u0 = 0, parts = 0;  // two (warpgroups) per piece, none of which is empty
   if (n > 0) {
-    // CTA u takes chunks [all u / units, all (u + 1) / units)
-    u0 = first * p.units / all;
-    while (u0 > 0 && all * u0 / p.units > first) --u0;
-    while (all * (u0 + 1) / p.units <= first) ++u0;
-    int64_t u1 = (last - 1) * p.units / all;
-    while (all * u1 / p.units > last - 1) --u1;
-    while (all * (u1 + 1) / p.units <= last - 1) ++u1;
-    parts = static_cast<int>(u1 - u0 + 1) * 2;
+    const int first = before * p.hk + kvh * n;
+    u0 = line.owner(first);
+    parts = (line.owner(first + n - 1) - u0 + 1) * 2;
   }
   // piece u of (sequence, kv head) is number u + b hk + kvh
-  const int64_t piece = (u0 + static_cast<int64_t>(b) * p.hk + kvh) * 2;
+  const int64_t piece = (static_cast<int64_t>(u0) + static_cast<int64_t>(b) * p.hk + kvh) * 2;
   auto part = [&](int i) -> float2 {
-    const int64_t u = u0 + (i >> 1);
-    if (all * u / p.units == all * (u + 1) / p.units) return make_float2(kNone, 0.f);  // no chunk
     return p.part_ml[(piece + i) * p.g + gi];
   };
   float top = kNone;
@@ -856,9 +909,9 @@ __global__ void __launch_bounds__(kKeys) paged_weights_kernel(const Params p) {
   const int b = blockIdx.y, c = blockIdx.x;
   const Seq s = make_seq(p, b);
   if (c >= s.chunks) return;
-  const int per = kKeys / p.gran;
-  const int gi = threadIdx.x / p.gran;
-  const int row = gran_row(p, s, c * per + gi) + (threadIdx.x - gi * p.gran);
+  const int per = kKeys >> p.gshift;
+  const int gi = threadIdx.x >> p.gshift;
+  const int row = gran_row(p, s, c * per + gi) + (threadIdx.x & (p.gran - 1));
   if (!row_seen(s, c * per + gi, row)) return;
   const int page = page_of(p, b, row);
   if (page < 0) return;
@@ -1001,7 +1054,8 @@ extern "C" int dsa_paged_attn_fwd(const void* q, const int64_t* q_strides, const
   const int g = n_heads / n_kv_heads;
   if (g > 128 || page_size % 8 != 0 || page_size > (1 << 20) || num_pages > 0x7FFFFFFF ||
       max_pages > (int64_t{1} << 28) || max_pages * page_size > (int64_t{1} << 28) ||
-      batch > 65535 || batch * n_heads > (int64_t{1} << 28))
+      batch > 65535 || batch * n_heads > (int64_t{1} << 28) ||
+      batch * n_kv_heads * max_chunks(max_pages, page_size) > 0x7FFFFFFF)
     return DSA_ERR_UNSUPPORTED;
   if (batch == 0) return DSA_OK;
   if (q == nullptr || k_pages == nullptr || v_pages == nullptr || block_table == nullptr ||
@@ -1026,6 +1080,7 @@ extern "C" int dsa_paged_attn_fwd(const void* q, const int64_t* q_strides, const
   p.page = static_cast<int>(page_size);
   p.max_pages = static_cast<int>(max_pages);
   p.gran = granule(page_size);
+  p.gshift = p.gran == 32 ? 5 : (p.gran == 16 ? 4 : 3);
   p.num_pages = num_pages;
   const int64_t room = max_pages * page_size;
   p.window = static_cast<int>(window < room ? window : 0);  // at least the room: everything
