@@ -275,8 +275,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (uses > 0) mbar_drain(kv_full, (uses - 1) & 1);
       for (int i = (gs > C::kStages ? gs - C::kStages : 0); i < gs; ++i)
         mbar_drain(&st_full[i % C::kStages], (i / C::kStages) & 1);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------- MMA issuer
+      // the whole warp walks and waits; one elected lane issues
       constexpr uint32_t idesc_s = make_idesc<T>(128, kStream, 0);
       constexpr uint32_t idesc_o = make_idesc<T>(128, D, 1);
       const uint64_t dk0 = make_smem_desc(smem_u32(smem + C::kOffK), 16u, 1024u, kLayoutSW128);
@@ -289,52 +290,62 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int gs = 0, uses = 0;
       int gp[2] = {0, 0};
       bool ok = true;
+      auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
+        return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+      };
+      auto commit = [&](uint64_t* b) {
+        if (elect_one()) umma_commit(b);
+        __syncwarp();
+      };
       auto issue_s = [&](int i) -> bool {  // i: global tile number; buffer i & 1
         const int w = i & 1, s = i % C::kStages;
-        if (!mbar_wait(&st_full[s], (i / C::kStages) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
-          return false;
-        if (gp[w] >= 1 && !mbar_wait(&o_done[w], (gp[w] - 1) & 1, abort_flag, p.err,
-                                     DSA_DEVERR_WIN_WAIT))
-          return false;
+        if (!wait_warp(&st_full[s], (i / C::kStages) & 1)) return false;
+        if (gp[w] >= 1 && !wait_warp(&o_done[w], (gp[w] - 1) & 1)) return false;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 128);
         const uint32_t qb = s_lo + static_cast<uint32_t>(s * (C::kStageBytes >> 4));
         const uint32_t ob = qb + static_cast<uint32_t>(C::kStageBytes >> 5);
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
-          const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
-          umma_bf16(d, desc_from_words(k_lo + ao, hi), desc_from_words(qb + bo, hi), idesc_s,
-                    k > 0 ? 1u : 0u);
-        }
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+            const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
+            umma_bf16(d, desc_from_words(k_lo + ao, hi), desc_from_words(qb + bo, hi), idesc_s,
+                      k > 0 ? 1u : 0u);
+          }
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
-          const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
-          umma_bf16(d + 64u, desc_from_words(v_lo + ao, hi), desc_from_words(ob + bo, hi), idesc_s,
-                    k > 0 ? 1u : 0u);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+            const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
+            umma_bf16(d + 64u, desc_from_words(v_lo + ao, hi), desc_from_words(ob + bo, hi), idesc_s,
+                      k > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[w]);
         }
-        umma_commit(&s_full[w]);
+        __syncwarp();
         return true;
       };
       auto issue_o = [&](int i, bool fresh) -> bool {
         const int w = i & 1, s = i % C::kStages;
-        if (!mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) return false;
+        if (!wait_warp(&p_full[w], gp[w] & 1)) return false;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 128);
         const uint32_t qb = mn_lo + static_cast<uint32_t>(s * (C::kStageBytes >> 4));
         const uint32_t ob = qb + static_cast<uint32_t>(C::kStageBytes >> 5);
+        if (elect_one()) {
 #pragma unroll
-        for (int st = 0; st < kStream / 16; ++st) {
-          const uint32_t acc = (fresh && st == 0) ? 0u : 1u;
-          const uint32_t bo = static_cast<uint32_t>(st * 128);
-          umma_bf16_tmem_a(tmem + 384u, d + static_cast<uint32_t>(st * 8), desc_from_words(ob + bo, hi),
-                           idesc_o, acc);
-          umma_bf16_tmem_a(tmem + 256u, d + 64u + static_cast<uint32_t>(st * 8),
-                           desc_from_words(qb + bo, hi), idesc_o, acc);
+          for (int st = 0; st < kStream / 16; ++st) {
+            const uint32_t acc = (fresh && st == 0) ? 0u : 1u;
+            const uint32_t bo = static_cast<uint32_t>(st * 128);
+            umma_bf16_tmem_a(tmem + 384u, d + static_cast<uint32_t>(st * 8),
+                             desc_from_words(ob + bo, hi), idesc_o, acc);
+            umma_bf16_tmem_a(tmem + 256u, d + 64u + static_cast<uint32_t>(st * 8),
+                             desc_from_words(qb + bo, hi), idesc_o, acc);
+          }
+          umma_commit(&o_done[w]);
+          umma_commit(&st_empty[s]);
         }
-        umma_commit(&o_done[w]);
-        umma_commit(&st_empty[s]);
+        __syncwarp();
         ++gp[w];
         return true;
       };
@@ -342,25 +353,25 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const Unit u = make_unit(p, x);
         const int nt = u.r1 - u.r0;
         if (nt <= 0) continue;
-        ok = mbar_wait(kv_full, uses & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+        ok = wait_warp(kv_full, uses & 1);
         ok = ok && issue_s(gs) && (nt < 2 || issue_s(gs + 1));
-        if (ok && nt <= 2) umma_commit(kv_empty);
-        ok = ok && (uses == 0 || mbar_wait(acc_empty, (uses - 1) & 1, abort_flag, p.err,
-                                           DSA_DEVERR_WIN_WAIT));
+        if (ok && nt <= 2) commit(kv_empty);
+        ok = ok && (uses == 0 || wait_warp(acc_empty, (uses - 1) & 1));
         for (int i = 0; i < nt && ok; ++i) {
           ok = issue_o(gs + i, i == 0);
           if (ok && i + 2 < nt) {
             ok = issue_s(gs + i + 2);
-            if (ok && i + 3 == nt) umma_commit(kv_empty);  // the key tile is no longer read
+            if (ok && i + 3 == nt) commit(kv_empty);  // the key tile is no longer read
           }
         }
         if (!ok) break;
-        umma_commit(acc_full);
+        commit(acc_full);
         gs += nt;
         ++uses;
       }
-      umma_commit(drain_bar);
+      commit(drain_bar);
       mbar_drain(drain_bar, 0);
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ P^T and dS^T
@@ -704,8 +715,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         mbar_drain(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
       for (int w = 0; w < 2; ++w)
         if (uses[w] > 0) mbar_drain(&q_full[w], (uses[w] - 1) & 1);
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1) {
       // ---------------------------------------------------------- MMA issuer
+      // the whole warp walks and waits; one elected lane issues
       constexpr uint32_t idesc_o = make_idesc<T>(128, D, 1);
       const uint64_t dq0 = make_smem_desc(smem_u32(smem + C::kOffQ), 16u, 1024u, kLayoutSW128);
       const uint32_t hi = static_cast<uint32_t>(dq0 >> 32);
@@ -718,10 +730,15 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int uses[2] = {0, 0};
       int first[2] = {0, 0}, last[2] = {-1, -1};
       bool ok = true;
+      auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
+        return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+      };
+      auto commit = [&](uint64_t* b) {
+        if (elect_one()) umma_commit(b);
+        __syncwarp();
+      };
       auto issue_s = [&](int w, int c, int ks, int vs, int nb) -> bool {
-        if (gp[w] >= 1 && !mbar_wait(&o_done[w], (gp[w] - 1) & 1, abort_flag, p.err,
-                                     DSA_DEVERR_WIN_WAIT))
-          return false;
+        if (gp[w] >= 1 && !wait_warp(&o_done[w], (gp[w] - 1) & 1)) return false;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 256);
         const uint32_t qa = q_lo + static_cast<uint32_t>(2 * w * (C::kTileBytes >> 4));
@@ -730,43 +747,49 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const uint32_t vb = k_lo + static_cast<uint32_t>(vs * (C::kSlotBytes >> 4));
         const uint32_t idesc_s =
             make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(nb * kBlk / 8) << 17);
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
-          const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
-          umma_bf16(d, desc_from_words(qa + ao, hi), desc_from_words(kb + bo, hi), idesc_s,
-                    k > 0 ? 1u : 0u);
-        }
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+            const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
+            umma_bf16(d, desc_from_words(qa + ao, hi), desc_from_words(kb + bo, hi), idesc_s,
+                      k > 0 ? 1u : 0u);
+          }
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
-          const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
-          umma_bf16(d + 64u, desc_from_words(oa + ao, hi), desc_from_words(vb + bo, hi), idesc_s,
-                    k > 0 ? 1u : 0u);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+            const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
+            umma_bf16(d + 64u, desc_from_words(oa + ao, hi), desc_from_words(vb + bo, hi), idesc_s,
+                      k > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[w]);
+          if (c == last[w]) umma_commit(&q_empty[w]);
         }
-        umma_commit(&s_full[w]);
-        if (c == last[w]) umma_commit(&q_empty[w]);
+        __syncwarp();
         return true;
       };
       auto issue_o = [&](int w, int c, int slot, int nb) -> bool {
-        if (!mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) return false;
-        if (c == first[w] && uses[w] > 1 &&
-            !mbar_wait(&o_empty[w], (uses[w] - 2) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
-          return false;
+        if (!wait_warp(&p_full[w], gp[w] & 1)) return false;
+        if (c == first[w] && uses[w] > 1 && !wait_warp(&o_empty[w], (uses[w] - 2) & 1)) return false;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 256);
         const uint32_t kb = mn_lo + static_cast<uint32_t>(slot * (C::kSlotBytes >> 4));
-        for (int st = 0; st < nb * 2; ++st)
-          umma_bf16_tmem_a(d + 128u, d + static_cast<uint32_t>(st * 8),
-                           desc_from_words(kb + static_cast<uint32_t>(st * 128), hi), idesc_o,
-                           (c > first[w] || st > 0) ? 1u : 0u);
-        umma_commit(&o_done[w]);
+        const uint32_t more = c > first[w] ? 1u : 0u;
+        if (elect_one()) {
+#pragma unroll
+          for (int st = 0; st < kCB * 2; ++st)
+            if (st < nb * 2)
+              umma_bf16_tmem_a(d + 128u, d + static_cast<uint32_t>(st * 8),
+                               desc_from_words(kb + static_cast<uint32_t>(st * 128), hi), idesc_o,
+                               st > 0 ? 1u : more);
+          umma_commit(&o_done[w]);
+        }
+        __syncwarp();
         ++gp[w];
         return true;
       };
       auto wait_slot = [&](int i) -> bool {
-        return mbar_wait(&kv_full[i % C::kSlots], (i / C::kSlots) & 1, abort_flag, p.err,
-                         DSA_DEVERR_WIN_WAIT);
+        return wait_warp(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
       };
       // K rows at or past kv_len may hold anything, and 0 x NaN is NaN: cleared before
       // the product that sums over them
@@ -777,19 +800,20 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           const int key = it.r.key(c * kCB + i);
           for (int r = max(it.kv_len - key, 0); r < kBlk; ++r) {
             wrote = true;
-            for (int x = 0; x < C::kHalves * 8; ++x)
+            if (int x = lane; x < C::kHalves * 8)
               st_shared_v4(smem_u32(base + (x >> 3) * kHalfBox + (i * kBlk + r) * 128 + (x & 7) * 16),
                            0u, 0u, 0u, 0u);
           }
         }
         if (wrote) fence_proxy_async_smem();
+        __syncwarp();
       };
       for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
         const Item it = make_item(p.s, p.grid, item);
         for (int w = 0; w < 2 && ok; ++w) {
           it.span<kCB>(p.s, w, &first[w], &last[w]);
           if (last[w] < 0) continue;
-          ok = mbar_wait(&q_full[w], uses[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+          ok = wait_warp(&q_full[w], uses[w] & 1);
           ++uses[w];
         }
         if (!ok) break;
@@ -801,7 +825,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           for (int w = 0; w < 2 && ok; ++w)
             if (it.active<kCB>(p.s, w, 0))
               ok = issue_s(w, 0, k_slot(0) % C::kSlots, v_slot(0) % C::kSlots, it.blocks<kCB>(0));
-          if (ok && !p.shared) umma_commit(&kv_empty[v_slot(0) % C::kSlots]);
+          if (ok && !p.shared) commit(&kv_empty[v_slot(0) % C::kSlots]);
         }
         for (int c = 0; c < chunks && ok; ++c) {
           const int nb = it.blocks<kCB>(c);
@@ -816,13 +840,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                            it.blocks<kCB>(c + 1));
           }
           if (!ok) break;
-          umma_commit(&kv_empty[sk]);
-          if (more && !p.shared) umma_commit(&kv_empty[v_slot(c + 1) % C::kSlots]);
+          commit(&kv_empty[sk]);
+          if (more && !p.shared) commit(&kv_empty[v_slot(c + 1) % C::kSlots]);
         }
         seq += chunks * per;
       }
-      umma_commit(drain_bar);
+      commit(drain_bar);
       mbar_drain(drain_bar, 0);
+      __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ dS

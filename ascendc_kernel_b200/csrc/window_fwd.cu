@@ -175,7 +175,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
+    // the whole warp walks and waits; one elected lane issues
+    {
       constexpr uint32_t idesc_o = make_idesc<T>(128, D, 1);
       const uint64_t dq = make_smem_desc(smem_u32(smem + C::kOffQ), 16u, 1024u, kLayoutSW128);
       const uint64_t dk = make_smem_desc(smem_u32(smem + C::kOffKV), 16u, 1024u, kLayoutSW128);
@@ -190,46 +191,57 @@ __global__ void __launch_bounds__(kThreads, 1)
       int uses[2] = {0, 0};    // items per tile
       int first[2] = {0, 0}, last[2] = {-1, -1};
       bool ok = true;
+      auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
+        return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+      };
       auto issue_s = [&](int w, int c, int slot, int nb) -> bool {
         // the S/P columns are free once the tile's previous PV product completed
-        if (gp[w] >= 1 && !mbar_wait(&o_done[w], (gp[w] - 1) & 1, abort_flag, p.err,
-                                     DSA_DEVERR_WIN_WAIT))
-          return false;
+        if (gp[w] >= 1 && !wait_warp(&o_done[w], (gp[w] - 1) & 1)) return false;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 256);
         const uint32_t qa = q_lo + static_cast<uint32_t>(w * (C::kTileBytes >> 4));
         const uint32_t kb = k_lo + static_cast<uint32_t>(slot * (C::kTileBytes >> 4));
         const uint32_t idesc_s = make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(nb * kBlk / 8) << 17);
+        if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t o = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
-          umma_bf16(d, desc_from_words(qa + o, hi), desc_from_words(kb + o, hi), idesc_s,
-                    k > 0 ? 1u : 0u);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t o = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+            umma_bf16(d, desc_from_words(qa + o, hi), desc_from_words(kb + o, hi), idesc_s,
+                      k > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[w]);
+          if (c == last[w]) umma_commit(&q_empty[w]);
         }
-        umma_commit(&s_full[w]);
-        if (c == last[w]) umma_commit(&q_empty[w]);
+        __syncwarp();
         ++gs[w];
         return true;
       };
       auto issue_pv = [&](int w, int c, int slot, int nb) -> bool {
-        if (!mbar_wait(&p_full[w], gp[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) return false;
-        if (c == first[w] && uses[w] > 1 &&
-            !mbar_wait(&o_empty[w], (uses[w] - 2) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
-          return false;
+        if (!wait_warp(&p_full[w], gp[w] & 1)) return false;
+        if (c == first[w] && uses[w] > 1 && !wait_warp(&o_empty[w], (uses[w] - 2) & 1)) return false;
         tc_fence_after();
         const uint32_t sp = tmem + static_cast<uint32_t>(w * 256);
         const uint32_t vb = v_lo + static_cast<uint32_t>(slot * (C::kTileBytes >> 4));
-        for (int st = 0; st < nb * 2; ++st)  // 16 keys a step, 8 TMEM columns of P
-          umma_bf16_tmem_a(sp + 128u, sp + static_cast<uint32_t>(st * 8),
-                           desc_from_words(vb + static_cast<uint32_t>(st * 128), hi), idesc_o,
-                           (c > first[w] || st > 0) ? 1u : 0u);
-        umma_commit(&o_done[w]);
+        const uint32_t more = c > first[w] ? 1u : 0u;
+        if (elect_one()) {
+#pragma unroll
+          for (int st = 0; st < kChunkBlks * 2; ++st)  // 16 keys a step, 8 TMEM columns of P
+            if (st < nb * 2)
+              umma_bf16_tmem_a(sp + 128u, sp + static_cast<uint32_t>(st * 8),
+                               desc_from_words(vb + static_cast<uint32_t>(st * 128), hi), idesc_o,
+                               st > 0 ? 1u : more);
+          umma_commit(&o_done[w]);
+        }
+        __syncwarp();
         ++gp[w];
         return true;
       };
+      auto commit = [&](uint64_t* b) {
+        if (elect_one()) umma_commit(b);
+        __syncwarp();
+      };
       auto wait_slot = [&](int i) -> bool {
-        return mbar_wait(&kv_full[i % C::kSlots], (i / C::kSlots) & 1, abort_flag, p.err,
-                         DSA_DEVERR_WIN_WAIT);
+        return wait_warp(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
       };
       // V rows at or past kv_len may hold anything, and 0 x NaN is NaN: they are
       // cleared before the product that reads them (at most 31 rows of a block)
@@ -240,19 +252,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int key = it.r.key(c * kChunkBlks + i);
           for (int r = max(it.kv_len - key, 0); r < kBlk; ++r) {
             wrote = true;
-            for (int x = 0; x < C::kHalves * 8; ++x)
+            if (int x = lane; x < C::kHalves * 8)
               st_shared_v4(smem_u32(base + (x >> 3) * kBoxBytes + (i * kBlk + r) * 128 + (x & 7) * 16),
                            0u, 0u, 0u, 0u);
           }
         }
         if (wrote) fence_proxy_async_smem();
+        __syncwarp();
       };
       for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
         const Item it = make_item(p.s, p.grid, item);
         for (int w = 0; w < 2 && ok; ++w) {
           it.span<kChunkBlks>(p.s, w, &first[w], &last[w]);
           if (last[w] < 0) continue;
-          ok = mbar_wait(&q_full[w], uses[w] & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+          ok = wait_warp(&q_full[w], uses[w] & 1);
           ++uses[w];
         }
         if (!ok) break;
@@ -263,7 +276,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = wait_slot(k_slot(0));
           for (int w = 0; w < 2 && ok; ++w)
             if (it.active<kChunkBlks>(p.s, w, 0)) ok = issue_s(w, 0, k_slot(0) % C::kSlots, nb);
-          if (ok && !p.shared) umma_commit(&kv_empty[k_slot(0) % C::kSlots]);
+          if (ok && !p.shared) commit(&kv_empty[k_slot(0) % C::kSlots]);
         }
         for (int c = 0; c < it.chunks<kChunkBlks>() && ok; ++c) {
           const int nb = it.blocks<kChunkBlks>(c);
@@ -279,13 +292,14 @@ __global__ void __launch_bounds__(kThreads, 1)
               ok = issue_s(w, c + 1, k_slot(c + 1) % C::kSlots, nbn);
           }
           if (!ok) break;
-          umma_commit(&kv_empty[sv]);
-          if (more && !p.shared) umma_commit(&kv_empty[k_slot(c + 1) % C::kSlots]);
+          commit(&kv_empty[sv]);
+          if (more && !p.shared) commit(&kv_empty[k_slot(c + 1) % C::kSlots]);
         }
         seq += it.chunks<kChunkBlks>() * per;
       }
-      umma_commit(drain_bar);
+      commit(drain_bar);
       mbar_drain(drain_bar, 0);
+      __syncwarp();
     }
   }
   } else {
