@@ -76,7 +76,8 @@ struct DkvCfg {
   static constexpr int kOffV = kTileBytes;
   static constexpr int kOffS = 2 * kTileBytes;
   static constexpr int kOffStat = kOffS + kStages * kStageBytes;  // [stage][2][64] f32
-  static constexpr int kOffBar = kOffStat + kStages * 2 * kStream * 4;
+  static constexpr int kOffStage = kOffStat + kStages * 2 * kStream * 4;  // [8 warps] 2 KB
+  static constexpr int kOffBar = kOffStage + 8 * 2048;
   static constexpr int kNumBars = 2 + 2 * kStages + 2 + 2 + 2 + 1 + 1 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
@@ -381,6 +382,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const int row = quarter * 32 + lane;  // key of the tile
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t sp = tmem + lane_off + static_cast<uint32_t>(w * 128);
+    const uint32_t stage = smem_u32(smem + C::kOffStage) + static_cast<uint32_t>((warp - 4) * 2048);
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int gs = 0, gw = 0, uses = 0;
     bool ok = true;
@@ -505,18 +507,17 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               reinterpret_cast<float4*>(dst + kRows * D)[k] =
                   make_float4(fv[4 * k], fv[4 * k + 1], fv[4 * k + 2], fv[4 * k + 3]);
           }
-        } else if (key < p.s.n) {
+        } else {
           const int64_t at =
               ((static_cast<int64_t>(u.b) * p.s.n + key) * p.s.hk + u.kvh) * D + c0 + q * 32;
+          uint32_t y[16];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            reinterpret_cast<uint4*>(p.dk + at)[k] =
-                make_uint4(T::pack(fk[8 * k], fk[8 * k + 1]), T::pack(fk[8 * k + 2], fk[8 * k + 3]),
-                           T::pack(fk[8 * k + 4], fk[8 * k + 5]), T::pack(fk[8 * k + 6], fk[8 * k + 7]));
-            if (p.dv != nullptr)
-              reinterpret_cast<uint4*>(p.dv + at)[k] = make_uint4(
-                  T::pack(fv[8 * k], fv[8 * k + 1]), T::pack(fv[8 * k + 2], fv[8 * k + 3]),
-                  T::pack(fv[8 * k + 4], fv[8 * k + 5]), T::pack(fv[8 * k + 6], fv[8 * k + 7]));
+          for (int k = 0; k < 16; ++k) y[k] = T::pack(fk[2 * k], fk[2 * k + 1]);
+          store_rows(stage, y, key < p.s.n ? p.dk + at : nullptr, lane);
+          if (p.dv != nullptr) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) y[k] = T::pack(fv[2 * k], fv[2 * k + 1]);
+            store_rows(stage, y, key < p.s.n ? p.dv + at : nullptr, lane);
           }
         }
       }
@@ -582,10 +583,11 @@ struct DqCfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kRows * D * 2;
   static constexpr int kSlotBytes = kCB * kBlk * D * 2;
-  static constexpr int kSlots = D == 128 ? 6 : 8;
+  static constexpr int kSlots = D == 128 ? 5 : 8;
   static constexpr int kOffQ = 0;                      // [2 tiles] q, dout
   static constexpr int kOffKV = 4 * kTileBytes;
-  static constexpr int kOffBar = kOffKV + kSlots * kSlotBytes;
+  static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;  // [8 warps] 2 KB, dq rows
+  static constexpr int kOffBar = kOffStage + 8 * 2048;
   static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 2 + 2 + 2 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
@@ -666,12 +668,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int seq = 0;
       int uses[2] = {0, 0};
       bool ok = true;
-      auto load_slot = [&](const Item& it, const CUtensorMap* tm, int c) -> bool {
+      auto load_slot = [&](const Item<kCB>& it, const CUtensorMap* tm, int c) -> bool {
         const int s = seq % C::kSlots;
         if (!mbar_wait(&kv_empty[s], ((seq / C::kSlots) & 1) ^ 1, abort_flag, p.err,
                        DSA_DEVERR_WIN_WAIT))
           return false;
-        const int nb = it.blocks<kCB>(c);
+        const int nb = it.blocks(c);
         uint8_t* dst = smem + C::kOffKV + s * C::kSlotBytes;
         mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(nb * kBlk * D * 2));
         for (int i = 0; i < nb; ++i) {
@@ -684,12 +686,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ++seq;
         return true;
       };
-      for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
-        const Item it = make_item(p.s, p.grid, item);
+      for (int item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
+        const Item<kCB> it = make_item<kCB>(p.s, p.grid, item);
         for (int w = 0; w < 2 && ok; ++w) {
-          int f, l;
-          it.span<kCB>(p.s, w, &f, &l);
-          if (l < 0) continue;
+          if (it.last(w) < 0) continue;
           if (!mbar_wait(&q_empty[w], (uses[w] & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) {
             ok = false;
             break;
@@ -698,14 +698,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           mbar_arrive_expect_tx(&q_full[w], static_cast<uint32_t>(2 * p.grid.tt * p.s.g * D * 2));
 #pragma unroll
           for (int half = 0; half < C::kHalves; ++half) {
-            tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0[w], it.b,
+            tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0(w), it.b,
                         &q_full[w]);
             tma_load_4d(qs + C::kTileBytes + half * kBoxBytes, &tm_do, half * 64, it.kvh * p.s.g,
-                        it.t0[w], it.b, &q_full[w]);
+                        it.t0(w), it.b, &q_full[w]);
           }
           ++uses[w];
         }
-        const int chunks = it.chunks<kCB>();
+        const int chunks = it.chunks;
         for (int c = 0; c < chunks && ok; ++c) {
           ok = load_slot(it, &tm_k, c);
           if (ok && !p.shared) ok = load_slot(it, &tm_v, c);
@@ -793,7 +793,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       };
       // K rows at or past kv_len may hold anything, and 0 x NaN is NaN: cleared before
       // the product that sums over them
-      auto clear_tail = [&](const Item& it, int c, int slot, int nb) {
+      auto clear_tail = [&](const Item<kCB>& it, int c, int slot, int nb) {
         uint8_t* base = smem + C::kOffKV + slot * C::kSlotBytes;
         bool wrote = false;
         for (int i = 0; i < nb; ++i) {
@@ -808,36 +808,37 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (wrote) fence_proxy_async_smem();
         __syncwarp();
       };
-      for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
-        const Item it = make_item(p.s, p.grid, item);
+      for (int item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
+        const Item<kCB> it = make_item<kCB>(p.s, p.grid, item);
         for (int w = 0; w < 2 && ok; ++w) {
-          it.span<kCB>(p.s, w, &first[w], &last[w]);
+          first[w] = it.first(w);
+          last[w] = it.last(w);
           if (last[w] < 0) continue;
           ok = wait_warp(&q_full[w], uses[w] & 1);
           ++uses[w];
         }
         if (!ok) break;
-        const int chunks = it.chunks<kCB>();
+        const int chunks = it.chunks;
         auto k_slot = [&](int c) { return seq + c * per; };
         auto v_slot = [&](int c) { return seq + c * per + per - 1; };
         if (chunks > 0) {
           ok = wait_slot(k_slot(0)) && wait_slot(v_slot(0));
           for (int w = 0; w < 2 && ok; ++w)
-            if (it.active<kCB>(p.s, w, 0))
-              ok = issue_s(w, 0, k_slot(0) % C::kSlots, v_slot(0) % C::kSlots, it.blocks<kCB>(0));
+            if (it.active(w, 0))
+              ok = issue_s(w, 0, k_slot(0) % C::kSlots, v_slot(0) % C::kSlots, it.blocks(0));
           if (ok && !p.shared) commit(&kv_empty[v_slot(0) % C::kSlots]);
         }
         for (int c = 0; c < chunks && ok; ++c) {
-          const int nb = it.blocks<kCB>(c);
+          const int nb = it.blocks(c);
           const bool more = c + 1 < chunks;
           const int sk = k_slot(c) % C::kSlots;
           if (p.s.kv_lens != nullptr) clear_tail(it, c, sk, nb);
           if (more) ok = wait_slot(k_slot(c + 1)) && wait_slot(v_slot(c + 1));
           for (int w = 0; w < 2 && ok; ++w) {
-            if (it.active<kCB>(p.s, w, c)) ok = issue_o(w, c, sk, nb);
-            if (ok && more && it.active<kCB>(p.s, w, c + 1))
+            if (it.active(w, c)) ok = issue_o(w, c, sk, nb);
+            if (ok && more && it.active(w, c + 1))
               ok = issue_s(w, c + 1, k_slot(c + 1) % C::kSlots, v_slot(c + 1) % C::kSlots,
-                           it.blocks<kCB>(c + 1));
+                           it.blocks(c + 1));
           }
           if (!ok) break;
           commit(&kv_empty[sk]);
@@ -860,23 +861,23 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t sp = tmem + lane_off + static_cast<uint32_t>(w * 256);
     const uint32_t od = sp + 128u;
+    const uint32_t stage = smem_u32(smem + C::kOffStage) + static_cast<uint32_t>((warp - 4) * 2048);
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int gc = 0;
     bool ok = true;
-    for (int64_t item = blockIdx.x; item < p.grid.items; item += gridDim.x) {
-      const Item it = make_item(p.s, p.grid, item);
-      int first, last;
-      it.span<kCB>(p.s, w, &first, &last);
-      const int t = it.t0[w] + tok;
-      const bool valid = tok < p.grid.tt && t < it.t1[w];
-      const int pos = min(t, it.t1[w] - 1) + p.s.n - p.s.m;
+    for (int item = blockIdx.x; item < p.grid.items; item += gridDim.x) {
+      const Item<kCB> it = make_item<kCB>(p.s, p.grid, item);
+      const int first = it.first(w), last = it.last(w);
+      const int t = it.t0(w) + tok;
+      const bool valid = tok < p.grid.tt && t < it.t1(w);
+      const int pos = min(t, it.t1(w) - 1) + p.s.n - p.s.m;
       const int64_t orow = (static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + it.kvh * p.s.g + head;
       const float2 st = valid ? __ldg(p.stat + orow) : make_float2(-INFINITY, 0.f);
       const uint64_t l2 = f2_pack(st.x, st.x), d2 = f2_pack(st.y, st.y);
       uint64_t psum[2] = {0ull, 0ull};  // sum_j P_j dP_j
       for (int c = first; c <= last; ++c) {
-        if (!it.active<kCB>(p.s, w, c)) continue;
-        const int nb = it.blocks<kCB>(c);
+        if (!it.active(w, c)) continue;
+        const int nb = it.blocks(c);
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[w], gc & 1, abort_flag, p.err,
                                                DSA_DEVERR_WIN_WAIT));
         if (!ok) break;
@@ -946,18 +947,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
           for (int k = 0; k < 32; ++k) ov[k] = 0u;
         }
-        if (valid) {
-          uint4* dst = reinterpret_cast<uint4*>(p.dq + orow * D + q * 32);
+        uint32_t x[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              x[u] = T::pack(__uint_as_float(ov[8 * j + 2 * u]) * p.scale,
-                             __uint_as_float(ov[8 * j + 2 * u + 1]) * p.scale);
-            dst[j] = make_uint4(x[0], x[1], x[2], x[3]);
-          }
-        }
+        for (int k = 0; k < 16; ++k)
+          x[k] = T::pack(__uint_as_float(ov[2 * k]) * p.scale, __uint_as_float(ov[2 * k + 1]) * p.scale);
+        store_rows(stage, x, valid ? p.dq + orow * D + q * 32 : nullptr, lane);
       }
       if (last >= 0) {
         tc_fence_before();
@@ -1128,7 +1122,7 @@ int launch_bwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   }
   DqParams p;
   p.s = s;
-  p.grid = tile_grid(s, batch);
+  if (!tile_grid(s, batch, &p.grid)) return DSA_ERR_UNSUPPORTED;
   p.scale = scale;
   p.scale_log2 = scale * kLog2e;
   p.stat = stat;
@@ -1146,7 +1140,7 @@ int launch_bwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   auto kernel = window_dq_kernel<T, D>;
   st = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), DqCfg<D>::kSmemBytes);
   if (st != DSA_OK) return st;
-  const int64_t grid = p.grid.items < di.num_sms ? p.grid.items : di.num_sms;
+  const int grid = p.grid.items < di.num_sms ? p.grid.items : di.num_sms;
   kernel<<<static_cast<unsigned>(grid), kBwdThreads, DqCfg<D>::kSmemBytes, stream>>>(tm_q, tm_do, tm_k,
                                                                                     tm_v, p);
   st = cuda_status(cudaGetLastError());

@@ -146,70 +146,84 @@ __device__ __forceinline__ void tmem_st_x16_nowait(uint32_t taddr, const uint32_
 struct TileGrid {
   int tt;               // tokens of a tile
   int items_per_head;   // pairs of tiles
-  int64_t items;
+  int items;
 };
-
-inline TileGrid tile_grid(const Shape& s, int64_t batch) {
-  TileGrid g;
-  g.tt = kRows / s.g;
-  g.items_per_head = ((s.m + g.tt - 1) / g.tt + 1) / 2;
-  g.items = batch * s.hk * g.items_per_head;
-  return g;
-}
 
 // The item's keys are read in chunks of CB blocks (the last one may be shorter).
+// Tile w sees keys of chunk c only if c <= last[w] and (c < head or c >= tail[w]):
+// chunks with first tokens, and those from its own window's start on.
+template <int CB>
 struct Item {
   int b, kvh, kv_len;
-  int t0[2], t1[2];  // tokens of each tile, empty when t1 <= t0
+  int t00, t10;      // first tokens of the tiles
+  int t01, t11;      // past their last ones; a tile is empty when t_1 <= t_0
   Range r;
+  int chunks, head;
+  int tail0, tail1, last0, last1;
 
-  template <int CB>
-  __device__ __forceinline__ int chunks() const {
-    return (r.nblk + CB - 1) / CB;
+  __device__ __forceinline__ int t0(int w) const { return w ? t10 : t00; }
+  __device__ __forceinline__ int t1(int w) const { return w ? t11 : t01; }
+  __device__ __forceinline__ int last(int w) const { return w ? last1 : last0; }
+  __device__ __forceinline__ int blocks(int c) const { return min(CB, r.nblk - c * CB); }
+  __device__ __forceinline__ bool active(int w, int c) const {
+    return c <= last(w) && (c < head || c >= (w ? tail1 : tail0));
   }
-  template <int CB>
-  __device__ __forceinline__ int blocks(int c) const {
-    return min(CB, r.nblk - c * CB);
-  }
-  // Whether any row of tile w sees a key of chunk c.
-  template <int CB>
-  __device__ __forceinline__ bool active(const Shape& s, int w, int c) const {
-    if (t1[w] <= t0[w]) return false;
-    const int off = s.n - s.m;
-    const int hi = min(t1[w] + off, kv_len);
-    const int lo = t0[w] + off - s.window + 1;
-    const int nb = blocks<CB>(c);
-    bool any = false;
-    for (int i = 0; i < nb; ++i) {
-      const int k = r.key(c * CB + i);
-      any = any || (k < hi && (c * CB + i < r.nfb || k + kBlk > lo || k < s.n_first));
-    }
-    return any;
-  }
-  // First and last active chunk of tile w (last = -1 when none).
-  template <int CB>
-  __device__ __forceinline__ void span(const Shape& s, int w, int* first, int* last) const {
-    int f = 0, l = chunks<CB>() - 1;
-    while (l >= 0 && !active<CB>(s, w, l)) --l;
-    while (f <= l && !active<CB>(s, w, f)) ++f;
-    *first = f;
-    *last = l;
-  }
+  __device__ __forceinline__ int first(int w) const { return head > 0 ? 0 : (w ? tail1 : tail0); }
 };
 
-__device__ __forceinline__ Item make_item(const Shape& s, const TileGrid& g, int64_t item) {
-  Item it;
-  const int64_t bh = item / g.items_per_head;
-  const int pair = static_cast<int>(item - bh * g.items_per_head);
-  it.b = static_cast<int>(bh / s.hk);
-  it.kvh = static_cast<int>(bh - static_cast<int64_t>(it.b) * s.hk);
+template <int CB>
+__device__ __forceinline__ void tile_span(const Shape& s, const Item<CB>& it, int t0, int t1,
+                                          int* tail, int* last) {
+  const int off = s.n - s.m;
+  const int hi = min(t1 + off, it.kv_len);
+  const int lo = t0 + off - s.window + 1;
+  // blocks of the window range that lie below hi, and those wholly below lo
+  const int below = max(hi - it.r.lo + kBlk - 1, 0) / kBlk;
+  const int end = min(it.r.nfb + below, it.r.nblk);
+  *last = t1 > t0 && hi > 0 && end > 0 ? (end - 1) / CB : -1;
+  *tail = (it.r.nfb + max(lo - it.r.lo, 0) / kBlk) / CB;
+}
+
+template <int CB>
+__device__ __forceinline__ Item<CB> make_item(const Shape& s, const TileGrid& g, int item) {
+  Item<CB> it;
+  const int bh = item / g.items_per_head;
+  const int t = (item - bh * g.items_per_head) * 2 * g.tt;
+  it.b = bh / s.hk;
+  it.kvh = bh - it.b * s.hk;
   it.kv_len = kv_len_of(s, it.b);
-  for (int w = 0; w < 2; ++w) {
-    it.t0[w] = min((2 * pair + w) * g.tt, s.m);
-    it.t1[w] = min((2 * pair + w + 1) * g.tt, s.m);
-  }
-  it.r = key_range(s, it.t0[0], max(it.t1[0], it.t1[1]), it.kv_len);
+  it.t00 = t;
+  it.t01 = it.t10 = min(t + g.tt, s.m);
+  it.t11 = min(t + 2 * g.tt, s.m);
+  it.r = key_range(s, it.t00, it.t11, it.kv_len);
+  it.chunks = (it.r.nblk + CB - 1) / CB;
+  // chunks with first tokens: of their own blocks, or of the one range from key 0
+  const int heads = it.r.nfb > 0 ? it.r.nfb : (it.r.lo == 0 ? (s.n_first + kBlk - 1) / kBlk : 0);
+  it.head = (heads + CB - 1) / CB;
+  tile_span<CB>(s, it, it.t00, it.t01, &it.tail0, &it.last0);
+  tile_span<CB>(s, it, it.t10, it.t11, &it.tail1, &it.last1);
   return it;
+}
+
+// Stores 32 columns (16 packed words) of one row per lane to global memory: through
+// 2 KB of the warp's own shared memory, so that each store instruction writes whole
+// 64-byte pieces of 8 rows and not 16 bytes of 32. `row` is the lane's row (null: not
+// stored).
+__device__ __forceinline__ void store_rows(uint32_t stage, const uint32_t (&x)[16], uint16_t* row,
+                                           int lane) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    st_shared_v4(stage + static_cast<uint32_t>(lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)), x[4 * j],
+                 x[4 * j + 1], x[4 * j + 2], x[4 * j + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 8 + (lane >> 2), j = lane & 3;
+    const float4 v = ld_shared_f4(stage + static_cast<uint32_t>(r * 64 + ((j ^ ((r >> 1) & 3)) << 4)));
+    const uint64_t at = __shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(row), r);
+    if (at != 0) reinterpret_cast<float4*>(at)[j] = v;
+  }
+  __syncwarp();
 }
 
 }  // namespace win

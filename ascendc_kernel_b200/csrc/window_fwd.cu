@@ -46,7 +46,8 @@ struct FwdCfg {
   static constexpr int kSlots = D == 128 ? 4 : 6;
   static constexpr int kOffQ = 0;
   static constexpr int kOffKV = 2 * kTileBytes;
-  static constexpr int kOffBar = kOffKV + kSlots * kTileBytes;
+  static constexpr int kOffStage = kOffKV + kSlots * kTileBytes;  // [8 warps] 2 KB, out rows
+  static constexpr int kOffBar = kOffStage + 8 * 2048;
   static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 2 + 2 + 2 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
@@ -125,12 +126,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       int seq = 0;
       int uses[2] = {0, 0};
       bool ok = true;
-      auto load_slot = [&](const Item& it, const CUtensorMap* tm, int c) -> bool {
+      auto load_slot = [&](const Item<kChunkBlks>& it, const CUtensorMap* tm, int c) -> bool {
         const int s = seq % C::kSlots;
         if (!mbar_wait(&kv_empty[s], ((seq / C::kSlots) & 1) ^ 1, abort_flag, p.err,
                        DSA_DEVERR_WIN_WAIT))
           return false;
-        const int nb = it.blocks<kChunkBlks>(c);
+        const int nb = it.blocks(c);
         uint8_t* dst = smem + C::kOffKV + s * C::kTileBytes;
         mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(nb * kBlk * D * 2));
         for (int i = 0; i < nb; ++i) {
@@ -143,12 +144,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++seq;
         return true;
       };
-      for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
-        const Item it = make_item(p.s, p.grid, item);
+      for (int item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
+        const Item<kChunkBlks> it = make_item<kChunkBlks>(p.s, p.grid, item);
         for (int w = 0; w < 2 && ok; ++w) {
-          int f, l;
-          it.span<kChunkBlks>(p.s, w, &f, &l);
-          if (l < 0) continue;
+          if (it.last(w) < 0) continue;
           if (!mbar_wait(&q_empty[w], (uses[w] & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) {
             ok = false;
             break;
@@ -158,11 +157,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 static_cast<uint32_t>(p.grid.tt * p.s.g * D * 2));
 #pragma unroll
           for (int half = 0; half < C::kHalves; ++half)
-            tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0[w], it.b,
+            tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0(w), it.b,
                         &q_full[w]);
           ++uses[w];
         }
-        for (int c = 0; c < it.chunks<kChunkBlks>() && ok; ++c) {
+        for (int c = 0; c < it.chunks && ok; ++c) {
           ok = load_slot(it, &tm_k, c);
           if (ok && !p.shared) ok = load_slot(it, &tm_v, c);
         }
@@ -245,7 +244,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       // V rows at or past kv_len may hold anything, and 0 x NaN is NaN: they are
       // cleared before the product that reads them (at most 31 rows of a block)
-      auto clear_tail = [&](const Item& it, int c, int slot, int nb) {
+      auto clear_tail = [&](const Item<kChunkBlks>& it, int c, int slot, int nb) {
         uint8_t* base = smem + C::kOffKV + slot * C::kTileBytes;
         bool wrote = false;
         for (int i = 0; i < nb; ++i) {
@@ -260,10 +259,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (wrote) fence_proxy_async_smem();
         __syncwarp();
       };
-      for (int64_t item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
-        const Item it = make_item(p.s, p.grid, item);
+      for (int item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
+        const Item<kChunkBlks> it = make_item<kChunkBlks>(p.s, p.grid, item);
         for (int w = 0; w < 2 && ok; ++w) {
-          it.span<kChunkBlks>(p.s, w, &first[w], &last[w]);
+          first[w] = it.first(w);
+          last[w] = it.last(w);
           if (last[w] < 0) continue;
           ok = wait_warp(&q_full[w], uses[w] & 1);
           ++uses[w];
@@ -271,31 +271,31 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         auto k_slot = [&](int c) { return seq + c * per; };
         auto v_slot = [&](int c) { return seq + c * per + per - 1; };
-        if (it.chunks<kChunkBlks>() > 0) {
-          const int nb = it.blocks<kChunkBlks>(0);
+        if (it.chunks > 0) {
+          const int nb = it.blocks(0);
           ok = wait_slot(k_slot(0));
           for (int w = 0; w < 2 && ok; ++w)
-            if (it.active<kChunkBlks>(p.s, w, 0)) ok = issue_s(w, 0, k_slot(0) % C::kSlots, nb);
+            if (it.active(w, 0)) ok = issue_s(w, 0, k_slot(0) % C::kSlots, nb);
           if (ok && !p.shared) commit(&kv_empty[k_slot(0) % C::kSlots]);
         }
-        for (int c = 0; c < it.chunks<kChunkBlks>() && ok; ++c) {
-          const int nb = it.blocks<kChunkBlks>(c);
-          const bool more = c + 1 < it.chunks<kChunkBlks>();
-          const int nbn = more ? it.blocks<kChunkBlks>(c + 1) : 0;
+        for (int c = 0; c < it.chunks && ok; ++c) {
+          const int nb = it.blocks(c);
+          const bool more = c + 1 < it.chunks;
+          const int nbn = more ? it.blocks(c + 1) : 0;
           const int sv = v_slot(c) % C::kSlots;
           ok = wait_slot(v_slot(c));
           if (ok && p.s.kv_lens != nullptr) clear_tail(it, c, sv, nb);
           if (ok && more) ok = wait_slot(k_slot(c + 1));
           for (int w = 0; w < 2 && ok; ++w) {
-            if (it.active<kChunkBlks>(p.s, w, c)) ok = issue_pv(w, c, sv, nb);
-            if (ok && more && it.active<kChunkBlks>(p.s, w, c + 1))
+            if (it.active(w, c)) ok = issue_pv(w, c, sv, nb);
+            if (ok && more && it.active(w, c + 1))
               ok = issue_s(w, c + 1, k_slot(c + 1) % C::kSlots, nbn);
           }
           if (!ok) break;
           commit(&kv_empty[sv]);
           if (more && !p.shared) commit(&kv_empty[k_slot(c + 1) % C::kSlots]);
         }
-        seq += it.chunks<kChunkBlks>() * per;
+        seq += it.chunks * per;
       }
       commit(drain_bar);
       mbar_drain(drain_bar, 0);
@@ -313,22 +313,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t sp = tmem + lane_off + static_cast<uint32_t>(w * 256);
     const uint32_t od = sp + 128u;
+    const uint32_t stage = smem_u32(smem + C::kOffStage) + static_cast<uint32_t>((warp - 4) * 2048);
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int gc = 0;  // chunks processed (all items)
     bool ok = true;
-    for (int64_t item = blockIdx.x; item < p.grid.items; item += gridDim.x) {
-      const Item it = make_item(p.s, p.grid, item);
-      int first, last;
-      it.span<kChunkBlks>(p.s, w, &first, &last);
-      const int t = it.t0[w] + tok;
-      const bool valid = tok < p.grid.tt && t < it.t1[w];
+    for (int item = blockIdx.x; item < p.grid.items; item += gridDim.x) {
+      const Item<kChunkBlks> it = make_item<kChunkBlks>(p.s, p.grid, item);
+      const int first = it.first(w), last = it.last(w);
+      const int t = it.t0(w) + tok;
+      const bool valid = tok < p.grid.tt && t < it.t1(w);
       // rows past the tile's tokens follow its last one: their values are not used
-      const int pos = min(t, it.t1[w] - 1) + p.s.n - p.s.m;
+      const int pos = min(t, it.t1(w) - 1) + p.s.n - p.s.m;
       const int gh = it.kvh * p.s.g + head;
       float m = -INFINITY, l = 0.f;
       for (int c = first; c <= last; ++c) {
-        if (!it.active<kChunkBlks>(p.s, w, c)) continue;
-        const int nb = it.blocks<kChunkBlks>(c);
+        if (!it.active(w, c)) continue;
+        const int nb = it.blocks(c);
         ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[w], gc & 1, abort_flag, p.err,
                                                DSA_DEVERR_WIN_WAIT));
         if (!ok) break;
@@ -435,18 +435,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int k = 0; k < 32; ++k) ov[k] = 0u;
         }
-        if (valid) {
-          uint4* dst = reinterpret_cast<uint4*>(p.out + orow * D + q * 32);
+        uint32_t x[16];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t x[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-              x[u] = T::pack(__uint_as_float(ov[8 * j + 2 * u]) * inv,
-                             __uint_as_float(ov[8 * j + 2 * u + 1]) * inv);
-            dst[j] = make_uint4(x[0], x[1], x[2], x[3]);
-          }
-        }
+        for (int k = 0; k < 16; ++k)
+          x[k] = T::pack(__uint_as_float(ov[2 * k]) * inv, __uint_as_float(ov[2 * k + 1]) * inv);
+        store_rows(stage, x, valid ? p.out + orow * D + q * 32 : nullptr, lane);
       }
       if (last >= 0) {
         tc_fence_before();
@@ -478,7 +471,7 @@ int launch_fwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   if (st != DSA_OK) return st;
   FwdParams p;
   p.s = s;
-  p.grid = tile_grid(s, batch);
+  if (!tile_grid(s, batch, &p.grid)) return DSA_ERR_UNSUPPORTED;
   p.scale_log2 = scale * kLog2e;
   p.sink = sink;
   p.out = static_cast<uint16_t*>(out);
@@ -493,7 +486,7 @@ int launch_fwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   auto kernel = window_fwd_kernel<T, D>;
   st = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), C::kSmemBytes);
   if (st != DSA_OK) return st;
-  const int64_t grid = p.grid.items < di.num_sms ? p.grid.items : di.num_sms;
+  const int grid = p.grid.items < di.num_sms ? p.grid.items : di.num_sms;
   kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmemBytes, stream>>>(tm_q, tm_k, tm_v, p);
   return cuda_status(cudaGetLastError());
 }

@@ -75,6 +75,15 @@ inline int map_head_by_rows(CUtensorMap* tm, uint32_t fmt, const void* base, con
                            CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
+// False when the items do not fit 31 bits.
+inline bool tile_grid(const Shape& s, int64_t batch, TileGrid* g) {
+  g->tt = kRows / s.g;
+  g->items_per_head = ((s.m + g->tt - 1) / g->tt + 1) / 2;
+  const int64_t items = batch * s.hk * g->items_per_head;
+  g->items = static_cast<int>(items);
+  return items <= 0x7FFFFF00;
+}
+
 // Checks shared by the forward and the backward; fills `x` and `s`.
 inline int check_window_args(const void* q, const int64_t* q_strides, const void* k,
                              const int64_t* k_strides, const void* v, const int64_t* v_strides,
