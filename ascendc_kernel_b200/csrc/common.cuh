@@ -141,6 +141,19 @@ __device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t nthreads, boo
   return out != 0u;
 }
 
+// A position in a ring of N slots and the parity of its barriers' phase.
+template <int N>
+struct Ring {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == N) {
+      slot = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
 // ---------------------------------------------------------------- proxies
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");

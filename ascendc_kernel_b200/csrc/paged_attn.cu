@@ -214,19 +214,6 @@ __device__ __forceinline__ float warp_transposed(float (&a)[32], int lane, Op op
   return a[0];
 }
 
-// A position in a ring of N slots and the parity of its barriers' phase.
-template <int N>
-struct Ring {
-  int slot = 0;
-  uint32_t parity = 0;
-  __device__ __forceinline__ void next() {
-    if (++slot == N) {
-      slot = 0;
-      parity ^= 1u;
-    }
-  }
-};
-
 static_assert(Cfg<128, 32>::kSmemBytes <= kMaxSmem && Cfg<128, 64>::kSmemBytes <= kMaxSmem &&
                   Cfg<128, 128>::kSmemBytes <= kMaxSmem && Cfg<64, 32>::kSmemBytes <= kMaxSmem &&
                   Cfg<64, 64>::kSmemBytes <= kMaxSmem && Cfg<64, 128>::kSmemBytes <= kMaxSmem,

@@ -686,8 +686,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ++seq;
         return true;
       };
-      for (int item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
-        const Item<kCB> it = make_item<kCB>(p.s, p.grid, item);
+      for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid)) {
+        const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
         for (int w = 0; w < 2 && ok; ++w) {
           if (it.last(w) < 0) continue;
           if (!mbar_wait(&q_empty[w], (uses[w] & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) {
@@ -808,8 +808,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (wrote) fence_proxy_async_smem();
         __syncwarp();
       };
-      for (int item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
-        const Item<kCB> it = make_item<kCB>(p.s, p.grid, item);
+      for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid)) {
+        const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
         for (int w = 0; w < 2 && ok; ++w) {
           first[w] = it.first(w);
           last[w] = it.last(w);
@@ -865,8 +865,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int gc = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < p.grid.items; item += gridDim.x) {
-      const Item<kCB> it = make_item<kCB>(p.s, p.grid, item);
+    for (ItemWalk wk(p.s, p.grid); wk.item < p.grid.items; wk.next(p.s, p.grid)) {
+      const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
       const int first = it.first(w), last = it.last(w);
       const int t = it.t0(w) + tok;
       const bool valid = tok < p.grid.tt && t < it.t1(w);
@@ -897,11 +897,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             tmem_wait_ld_dep(dv[i]);
           }
         }
+        const bool full = chunk_full<kCB>(p.s, it, it.t0(w), it.t1(w), c);
 #pragma unroll
         for (int i = 0; i < kCB; ++i) {
           if (i < nb) {
-            const uint32_t seen = seen_bits(p.s, it.r, c * kCB + i, pos, it.kv_len);
-            if (!__all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu)) {
+            if (!full) {
+              const uint32_t seen = seen_bits(p.s, it.r, c * kCB + i, pos, it.kv_len);
 #pragma unroll
               for (int k = 0; k < 32; ++k)
                 if (!((seen >> k) & 1u)) {
@@ -938,25 +939,24 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
       }
-#pragma unroll 1
+      // the row is rounded as it is read, so that O is given back before the stores
+      uint32_t x[D / 32][16];
+#pragma unroll
       for (int q = 0; q < D / 32; ++q) {
         uint32_t ov[32];
-        if (last >= 0) {
-          tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) ov[k] = 0u;
-        }
-        uint32_t x[16];
+        if (last >= 0) tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          x[k] = T::pack(__uint_as_float(ov[2 * k]) * p.scale, __uint_as_float(ov[2 * k + 1]) * p.scale);
-        store_rows(stage, x, valid ? p.dq + orow * D + q * 32 : nullptr, lane);
+          x[q][k] = last < 0 ? 0u
+                             : T::pack(__uint_as_float(ov[2 * k]) * p.scale, __uint_as_float(ov[2 * k + 1]) * p.scale);
       }
       if (last >= 0) {
         tc_fence_before();
         mbar_arrive(&o_empty[w]);
       }
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q)
+        store_rows(stage, x[q], valid ? p.dq + orow * D + q * 32 : nullptr, lane);
       if (valid && p.sink != nullptr) {
         float a0, a1, b0, b1;
         f2_unpack(psum[0], a0, a1);

@@ -180,17 +180,48 @@ __device__ __forceinline__ void tile_span(const Shape& s, const Item<CB>& it, in
   // blocks of the window range that lie below hi, and those wholly below lo
   const int below = max(hi - it.r.lo + kBlk - 1, 0) / kBlk;
   const int end = min(it.r.nfb + below, it.r.nblk);
-  *last = t1 > t0 && hi > 0 && end > 0 ? (end - 1) / CB : -1;
   *tail = (it.r.nfb + max(lo - it.r.lo, 0) / kBlk) / CB;
+  int l = t1 > t0 && hi > 0 && end > 0 ? (end - 1) / CB : -1;
+  // a window that starts past the valid keys: first tokens only
+  if (l >= it.head && l < *tail) l = it.head - 1;
+  *last = l;
 }
 
+// The items of one CTA: blockIdx.x, blockIdx.x + gridDim.x, ... as (batch, kv head, pair
+// of tiles), stepped without divisions.
+struct ItemWalk {
+  int item, b, kvh, pair;
+  int step_bh, step_pair;
+  __device__ __forceinline__ ItemWalk(const Shape& s, const TileGrid& g) {
+    item = blockIdx.x;
+    const int bh = item / g.items_per_head;
+    pair = item - bh * g.items_per_head;
+    b = bh / s.hk;
+    kvh = bh - b * s.hk;
+    step_bh = gridDim.x / g.items_per_head;
+    step_pair = gridDim.x - step_bh * g.items_per_head;
+  }
+  __device__ __forceinline__ void next(const Shape& s, const TileGrid& g) {
+    item += gridDim.x;
+    pair += step_pair;
+    kvh += step_bh;
+    if (pair >= g.items_per_head) {
+      pair -= g.items_per_head;
+      ++kvh;
+    }
+    while (kvh >= s.hk) {
+      kvh -= s.hk;
+      ++b;
+    }
+  }
+};
+
 template <int CB>
-__device__ __forceinline__ Item<CB> make_item(const Shape& s, const TileGrid& g, int item) {
+__device__ __forceinline__ Item<CB> make_item(const Shape& s, const TileGrid& g, const ItemWalk& w) {
   Item<CB> it;
-  const int bh = item / g.items_per_head;
-  const int t = (item - bh * g.items_per_head) * 2 * g.tt;
-  it.b = bh / s.hk;
-  it.kvh = bh - it.b * s.hk;
+  const int t = w.pair * 2 * g.tt;
+  it.b = w.b;
+  it.kvh = w.kvh;
   it.kv_len = kv_len_of(s, it.b);
   it.t00 = t;
   it.t01 = it.t10 = min(t + g.tt, s.m);
@@ -203,6 +234,16 @@ __device__ __forceinline__ Item<CB> make_item(const Shape& s, const TileGrid& g,
   tile_span<CB>(s, it, it.t00, it.t01, &it.tail0, &it.last0);
   tile_span<CB>(s, it, it.t10, it.t11, &it.tail1, &it.last1);
   return it;
+}
+
+// Whether every row of the tile with tokens [t0, t1) sees all keys of chunk c.
+template <int CB>
+__device__ __forceinline__ bool chunk_full(const Shape& s, const Item<CB>& it, int t0, int t1, int c) {
+  const int off = s.n - s.m;
+  const int key = it.r.key(c * CB);
+  const int end = key + it.blocks(c) * kBlk;
+  return c * CB >= it.r.nfb && key > t1 - 1 + off - s.window && end <= t0 + off + 1 &&
+         end <= it.kv_len;
 }
 
 // Stores 32 columns (16 packed words) of one row per lane to global memory: through

@@ -8,20 +8,22 @@
 // One pass over the keys with a running reference (maximum) and sum in fp32.
 // Per CTA (one per SM, persistent, 384 threads), a work item is two 128-row
 // tiles (consecutive tokens, all heads of a group) that share every key chunk of
-// up to 128 keys:
+// up to 64 keys:
 //   warp 0      TMA: q tiles, K and V chunks into a ring of slots (one slot a
 //               chunk when K and V are the same tensor).
-//   warp 1      tcgen05 issuer: S = Q K^T, then O += P V with P read from TMEM.
-//               Per chunk PV(c) of a tile, then S(c+1) of the same tile into the
-//               columns PV(c) read: one tile's products run under the other
-//               tile's softmax.
+//   warps 1, 2  tcgen05 issuers, one per tile: S = Q K^T, then O += P V with P read
+//               from TMEM.
 //   warps 4..11 softmax: a warpgroup per tile, a thread per row: no exchange
 //               between threads for the row's maximum and sum.
+// Each tile has two S buffers (P overwrites its S): PV(c) is followed by S(c + 2) into
+// the buffer that it frees while the softmax is at chunk c + 1, so the scores are there
+// when the softmax gets to them. One issuer for both tiles was the bottleneck: its
+// waits and commits took 2,000 of the 3,400 cycles of a chunk.
 // P is rounded to the operands' 16-bit type for the second product (its sum is
 // taken before the rounding, in fp32): a relative 2^-8 (2^-11 for fp16) a term at most,
 // the size of the output's own rounding. The reference moves, and O is rescaled,
 // only when a row's maximum exceeds it by more than 2^8, so P stays within fp16.
-// TMEM per tile w: S/P columns [256w, 256w+128), O columns [256w+128, 256w+128+D).
+// TMEM per tile w: S/P buffers [256w, +64), [256w+64, +64), O [256w+128, +D).
 #include "host_util.h"
 #include "window_common.cuh"
 #include "window_host.h"
@@ -31,24 +33,26 @@ namespace win {
 
 constexpr int kThreads = 384;
 // The launch holds 384 x 168 registers; the softmax warpgroups, whose threads keep
-// a chunk's 128 scores, take 208 each and the warpgroup of TMA and MMA keeps 88:
+// a chunk's scores and their row's results, take 208 each and the warpgroup of TMA and MMA keeps 88:
 // 128 x 88 + 256 x 208 = 384 x 168.
 constexpr int kRegsAux = 88;
 constexpr int kRegsSoftmax = 208;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.0f;
-constexpr int kChunkBlks = 4;  // blocks of a chunk
+constexpr int kCB = 2;  // key blocks of a chunk
+constexpr int kHalfBox = kCB * kBlk * 128;  // one [64 keys x 64 columns] SW128 box
 
 template <int D>
 struct FwdCfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kRows * D * 2;
-  static constexpr int kSlots = D == 128 ? 4 : 6;
+  static constexpr int kSlotBytes = kCB * kBlk * D * 2;
+  static constexpr int kSlots = 8;
   static constexpr int kOffQ = 0;
   static constexpr int kOffKV = 2 * kTileBytes;
-  static constexpr int kOffStage = kOffKV + kSlots * kTileBytes;  // [8 warps] 2 KB, out rows
+  static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;  // [8 warps] 2 KB, out rows
   static constexpr int kOffBar = kOffStage + 8 * 2048;
-  static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 2 + 2 + 2 + 2 + 1;
+  static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 4 + 4 + 4 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
 };
@@ -76,11 +80,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = bars;                  // [2] TMA -> MMA
   uint64_t* q_empty = q_full + 2;           // [2] last S of the tile done -> TMA
   uint64_t* kv_full = q_empty + 2;          // [kSlots]
-  uint64_t* kv_empty = kv_full + C::kSlots; // [kSlots]
-  uint64_t* s_full = kv_empty + C::kSlots;  // [2] S of a chunk in TMEM
-  uint64_t* p_full = s_full + 2;            // [2] P written (128 arrivals)
-  uint64_t* o_done = p_full + 2;            // [2] PV of a chunk completed
-  uint64_t* o_empty = o_done + 2;           // [2] O read by the epilogue (128 arrivals)
+  uint64_t* kv_empty = kv_full + C::kSlots; // [kSlots] both issuers
+  uint64_t* s_full = kv_empty + C::kSlots;  // [2 tiles][2] S of a chunk in TMEM
+  uint64_t* p_full = s_full + 4;            // [2 tiles][2] P written (128 arrivals)
+  uint64_t* o_done = p_full + 4;            // [2 tiles][2] PV of a chunk completed
+  uint64_t* o_empty = o_done + 4;           // [2] O read by the epilogue (128 arrivals)
   uint64_t* drain_bar = o_empty + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + C::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::kOffMisc + 4);
@@ -93,16 +97,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int w = 0; w < 2; ++w) {
       mbar_init(&q_full[w], 1);
       mbar_init(&q_empty[w], 1);
-      mbar_init(&s_full[w], 1);
-      mbar_init(&p_full[w], 128);
-      mbar_init(&o_done[w], 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[2 * w + i], 1);
+        mbar_init(&p_full[2 * w + i], 128);
+        mbar_init(&o_done[2 * w + i], 1);
+      }
       mbar_init(&o_empty[w], 128);
     }
     for (int s = 0; s < C::kSlots; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], 2);
     }
-    mbar_init(drain_bar, 1);
+    mbar_init(drain_bar, 2);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_q);
@@ -123,59 +129,62 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      int seq = 0;
-      int uses[2] = {0, 0};
+      Ring<C::kSlots> at;
+      int loads = 0;
+      int uses0 = 0, uses1 = 0;
       bool ok = true;
-      auto load_slot = [&](const Item<kChunkBlks>& it, const CUtensorMap* tm, int c) -> bool {
-        const int s = seq % C::kSlots;
-        if (!mbar_wait(&kv_empty[s], ((seq / C::kSlots) & 1) ^ 1, abort_flag, p.err,
-                       DSA_DEVERR_WIN_WAIT))
+      auto load_slot = [&](const Item<kCB>& it, const CUtensorMap* tm, int c) -> bool {
+        if (!mbar_wait(&kv_empty[at.slot], at.parity ^ 1u, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
           return false;
         const int nb = it.blocks(c);
-        uint8_t* dst = smem + C::kOffKV + s * C::kTileBytes;
-        mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(nb * kBlk * D * 2));
+        uint8_t* dst = smem + C::kOffKV + at.slot * C::kSlotBytes;
+        mbar_arrive_expect_tx(&kv_full[at.slot], static_cast<uint32_t>(nb * kBlk * D * 2));
         for (int i = 0; i < nb; ++i) {
-          const int key = it.r.key(c * kChunkBlks + i);
+          const int key = it.r.key(c * kCB + i);
 #pragma unroll
           for (int half = 0; half < C::kHalves; ++half)
-            tma_load_4d(dst + half * kBoxBytes + i * kBlk * 128, tm, half * 64, key, it.kvh, it.b,
-                        &kv_full[s]);
+            tma_load_4d(dst + half * kHalfBox + i * kBlk * 128, tm, half * 64, key, it.kvh, it.b,
+                        &kv_full[at.slot]);
         }
-        ++seq;
+        at.next();
+        ++loads;
         return true;
       };
-      for (int item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
-        const Item<kChunkBlks> it = make_item<kChunkBlks>(p.s, p.grid, item);
-        for (int w = 0; w < 2 && ok; ++w) {
-          if (it.last(w) < 0) continue;
-          if (!mbar_wait(&q_empty[w], (uses[w] & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) {
-            ok = false;
-            break;
-          }
-          uint8_t* qs = smem + C::kOffQ + w * C::kTileBytes;
-          mbar_arrive_expect_tx(&q_full[w],
-                                static_cast<uint32_t>(p.grid.tt * p.s.g * D * 2));
+      auto load_q = [&](const Item<kCB>& it, int w, int& uses) -> bool {
+        if (it.last(w) < 0) return true;
+        if (!mbar_wait(&q_empty[w], (uses & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
+          return false;
+        uint8_t* qs = smem + C::kOffQ + w * C::kTileBytes;
+        mbar_arrive_expect_tx(&q_full[w], static_cast<uint32_t>(p.grid.tt * p.s.g * D * 2));
 #pragma unroll
-          for (int half = 0; half < C::kHalves; ++half)
-            tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0(w), it.b,
-                        &q_full[w]);
-          ++uses[w];
-        }
+        for (int half = 0; half < C::kHalves; ++half)
+          tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0(w), it.b,
+                      &q_full[w]);
+        ++uses;
+        return true;
+      };
+      for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid)) {
+        const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
+        // the order in which the products use them: K(0), q, K(1), V(0), K(2), V(1), ...
+        if (it.chunks > 0) ok = load_slot(it, &tm_k, 0);
+        ok = ok && load_q(it, 0, uses0) && load_q(it, 1, uses1);
+        if (ok && it.chunks > 1) ok = load_slot(it, &tm_k, 1);
         for (int c = 0; c < it.chunks && ok; ++c) {
-          ok = load_slot(it, &tm_k, c);
-          if (ok && !p.shared) ok = load_slot(it, &tm_v, c);
+          if (!p.shared) ok = load_slot(it, &tm_v, c);
+          if (ok && c + 2 < it.chunks) ok = load_slot(it, &tm_k, c + 2);
         }
       }
       // copies in flight land before the CTA's shared memory goes away
-      for (int i = (seq > C::kSlots ? seq - C::kSlots : 0); i < seq; ++i)
+      for (int i = max(loads - C::kSlots, 0); i < loads; ++i)
         mbar_drain(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
-      for (int w = 0; w < 2; ++w)
-        if (uses[w] > 0) mbar_drain(&q_full[w], (uses[w] - 1) & 1);
+      if (uses0 > 0) mbar_drain(&q_full[0], (uses0 - 1) & 1);
+      if (uses1 > 0) mbar_drain(&q_full[1], (uses1 - 1) & 1);
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------ MMA issuers
     // the whole warp walks and waits; one elected lane issues
     {
+      const int w = warp - 1;
       constexpr uint32_t idesc_o = make_idesc<T>(128, D, 1);
       const uint64_t dq = make_smem_desc(smem_u32(smem + C::kOffQ), 16u, 1024u, kLayoutSW128);
       const uint64_t dk = make_smem_desc(smem_u32(smem + C::kOffKV), 16u, 1024u, kLayoutSW128);
@@ -183,119 +192,120 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t q_lo = static_cast<uint32_t>(dq);
       const uint32_t k_lo = static_cast<uint32_t>(dk);
       const uint32_t v_lo = static_cast<uint32_t>(make_smem_desc(
-          smem_u32(smem + C::kOffKV), static_cast<uint32_t>(kBoxBytes), 1024u, kLayoutSW128));
-      int seq = 0;             // slot number of the item's first chunk
-      int gs[2] = {0, 0};      // S products issued per tile
-      int gp[2] = {0, 0};      // PV products issued per tile
-      int uses[2] = {0, 0};    // items per tile
-      int first[2] = {0, 0}, last[2] = {-1, -1};
+          smem_u32(smem + C::kOffKV), static_cast<uint32_t>(kHalfBox), 1024u, kLayoutSW128));
+      Ring<C::kSlots> at;  // the next slot in the order of the loads
       bool ok = true;
       auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
         return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
-      };
-      auto issue_s = [&](int w, int c, int slot, int nb) -> bool {
-        // the S/P columns are free once the tile's previous PV product completed
-        if (gp[w] >= 1 && !wait_warp(&o_done[w], (gp[w] - 1) & 1)) return false;
-        tc_fence_after();
-        const uint32_t d = tmem + static_cast<uint32_t>(w * 256);
-        const uint32_t qa = q_lo + static_cast<uint32_t>(w * (C::kTileBytes >> 4));
-        const uint32_t kb = k_lo + static_cast<uint32_t>(slot * (C::kTileBytes >> 4));
-        const uint32_t idesc_s = make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(nb * kBlk / 8) << 17);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t o = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
-            umma_bf16(d, desc_from_words(qa + o, hi), desc_from_words(kb + o, hi), idesc_s,
-                      k > 0 ? 1u : 0u);
-          }
-          umma_commit(&s_full[w]);
-          if (c == last[w]) umma_commit(&q_empty[w]);
-        }
-        __syncwarp();
-        ++gs[w];
-        return true;
-      };
-      auto issue_pv = [&](int w, int c, int slot, int nb) -> bool {
-        if (!wait_warp(&p_full[w], gp[w] & 1)) return false;
-        if (c == first[w] && uses[w] > 1 && !wait_warp(&o_empty[w], (uses[w] - 2) & 1)) return false;
-        tc_fence_after();
-        const uint32_t sp = tmem + static_cast<uint32_t>(w * 256);
-        const uint32_t vb = v_lo + static_cast<uint32_t>(slot * (C::kTileBytes >> 4));
-        const uint32_t more = c > first[w] ? 1u : 0u;
-        if (elect_one()) {
-#pragma unroll
-          for (int st = 0; st < kChunkBlks * 2; ++st)  // 16 keys a step, 8 TMEM columns of P
-            if (st < nb * 2)
-              umma_bf16_tmem_a(sp + 128u, sp + static_cast<uint32_t>(st * 8),
-                               desc_from_words(vb + static_cast<uint32_t>(st * 128), hi), idesc_o,
-                               st > 0 ? 1u : more);
-          umma_commit(&o_done[w]);
-        }
-        __syncwarp();
-        ++gp[w];
-        return true;
       };
       auto commit = [&](uint64_t* b) {
         if (elect_one()) umma_commit(b);
         __syncwarp();
       };
-      auto wait_slot = [&](int i) -> bool {
-        return wait_warp(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
+      // waits for the next slot and returns its number
+      auto take = [&]() -> int {
+        const int s = at.slot;
+        ok = ok && wait_warp(&kv_full[s], at.parity);
+        at.next();
+        return s;
+      };
+      int gs = 0, go = 0, uses = 0;  // S and PV products issued, items
+      auto issue_s = [&](const Item<kCB>& it, int c, int slot) {
+        if (!ok || !it.active(w, c)) return;
+        // the buffer's P was read by the PV product before the last one
+        const int buf = 2 * w + (gs & 1);
+        if (gs >= 2) ok = wait_warp(&o_done[buf], ((gs - 2) >> 1) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t d = tmem + static_cast<uint32_t>(w * 256 + (gs & 1) * 64);
+        const uint32_t qa = q_lo + static_cast<uint32_t>(w * (C::kTileBytes >> 4));
+        const uint32_t kb = k_lo + static_cast<uint32_t>(slot * (C::kSlotBytes >> 4));
+        const uint32_t idesc_s =
+            make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(it.blocks(c) * kBlk / 8) << 17);
+        const bool end = c == it.last(w);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
+            const uint32_t bo = static_cast<uint32_t>(((k >> 2) * kHalfBox + (k & 3) * 32) >> 4);
+            umma_bf16(d, desc_from_words(qa + ao, hi), desc_from_words(kb + bo, hi), idesc_s,
+                      k > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[buf]);
+          if (end) umma_commit(&q_empty[w]);
+        }
+        __syncwarp();
+        ++gs;
+      };
+      auto issue_pv = [&](const Item<kCB>& it, int c, int slot) {
+        if (!ok || !it.active(w, c)) return;
+        const bool fresh = c == it.first(w);
+        const int buf = 2 * w + (go & 1);
+        ok = wait_warp(&p_full[buf], (go >> 1) & 1);
+        if (ok && fresh && uses > 1) ok = wait_warp(&o_empty[w], (uses - 2) & 1);
+        if (!ok) return;
+        tc_fence_after();
+        const uint32_t sp = tmem + static_cast<uint32_t>(w * 256 + (go & 1) * 64);
+        const uint32_t od = tmem + static_cast<uint32_t>(w * 256 + 128);
+        const uint32_t vb = v_lo + static_cast<uint32_t>(slot * (C::kSlotBytes >> 4));
+        const int nb = it.blocks(c);
+        const uint32_t more = fresh ? 0u : 1u;
+        if (elect_one()) {
+#pragma unroll
+          for (int st = 0; st < kCB * 2; ++st)  // 16 keys a step, 8 TMEM columns of P
+            if (st < nb * 2)
+              umma_bf16_tmem_a(od, sp + static_cast<uint32_t>(st * 8),
+                               desc_from_words(vb + static_cast<uint32_t>(st * 128), hi), idesc_o,
+                               st > 0 ? 1u : more);
+          umma_commit(&o_done[buf]);
+        }
+        __syncwarp();
+        ++go;
       };
       // V rows at or past kv_len may hold anything, and 0 x NaN is NaN: they are
-      // cleared before the product that reads them (at most 31 rows of a block)
-      auto clear_tail = [&](const Item<kChunkBlks>& it, int c, int slot, int nb) {
-        uint8_t* base = smem + C::kOffKV + slot * C::kTileBytes;
+      // cleared before the product that reads them (by both issuers, to the same zeros)
+      auto clear_tail = [&](const Item<kCB>& it, int c, int slot) {
+        uint8_t* base = smem + C::kOffKV + slot * C::kSlotBytes;
         bool wrote = false;
-        for (int i = 0; i < nb; ++i) {
-          const int key = it.r.key(c * kChunkBlks + i);
+        for (int i = 0; i < it.blocks(c); ++i) {
+          const int key = it.r.key(c * kCB + i);
           for (int r = max(it.kv_len - key, 0); r < kBlk; ++r) {
             wrote = true;
             if (int x = lane; x < C::kHalves * 8)
-              st_shared_v4(smem_u32(base + (x >> 3) * kBoxBytes + (i * kBlk + r) * 128 + (x & 7) * 16),
+              st_shared_v4(smem_u32(base + (x >> 3) * kHalfBox + (i * kBlk + r) * 128 + (x & 7) * 16),
                            0u, 0u, 0u, 0u);
           }
         }
         if (wrote) fence_proxy_async_smem();
         __syncwarp();
       };
-      for (int item = blockIdx.x; ok && item < p.grid.items; item += gridDim.x) {
-        const Item<kChunkBlks> it = make_item<kChunkBlks>(p.s, p.grid, item);
-        for (int w = 0; w < 2 && ok; ++w) {
-          first[w] = it.first(w);
-          last[w] = it.last(w);
-          if (last[w] < 0) continue;
-          ok = wait_warp(&q_full[w], uses[w] & 1);
-          ++uses[w];
+      for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid)) {
+        const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
+        const int n = it.chunks;
+        if (n == 0) continue;
+        // slots of K(c), K(c + 1) and K(c + 2); the other issuer takes the same
+        int k0 = take(), k1 = 0, k2 = 0;
+        if (it.last(w) >= 0) ok = ok && wait_warp(&q_full[w], uses++ & 1);
+        issue_s(it, 0, k0);
+        if (!p.shared) commit(&kv_empty[k0]);
+        if (n > 1) {
+          k1 = take();
+          issue_s(it, 1, k1);
+          if (!p.shared) commit(&kv_empty[k1]);
         }
-        if (!ok) break;
-        auto k_slot = [&](int c) { return seq + c * per; };
-        auto v_slot = [&](int c) { return seq + c * per + per - 1; };
-        if (it.chunks > 0) {
-          const int nb = it.blocks(0);
-          ok = wait_slot(k_slot(0));
-          for (int w = 0; w < 2 && ok; ++w)
-            if (it.active(w, 0)) ok = issue_s(w, 0, k_slot(0) % C::kSlots, nb);
-          if (ok && !p.shared) commit(&kv_empty[k_slot(0) % C::kSlots]);
-        }
-        for (int c = 0; c < it.chunks && ok; ++c) {
-          const int nb = it.blocks(c);
-          const bool more = c + 1 < it.chunks;
-          const int nbn = more ? it.blocks(c + 1) : 0;
-          const int sv = v_slot(c) % C::kSlots;
-          ok = wait_slot(v_slot(c));
-          if (ok && p.s.kv_lens != nullptr) clear_tail(it, c, sv, nb);
-          if (ok && more) ok = wait_slot(k_slot(c + 1));
-          for (int w = 0; w < 2 && ok; ++w) {
-            if (it.active(w, c)) ok = issue_pv(w, c, sv, nb);
-            if (ok && more && it.active(w, c + 1))
-              ok = issue_s(w, c + 1, k_slot(c + 1) % C::kSlots, nbn);
+        for (int c = 0; c < n && ok; ++c) {
+          const int v = p.shared ? k0 : take();
+          if (ok && p.s.kv_lens != nullptr) clear_tail(it, c, v);
+          issue_pv(it, c, v);
+          commit(&kv_empty[v]);
+          if (c + 2 < n) {
+            k2 = take();
+            issue_s(it, c + 2, k2);
+            if (!p.shared) commit(&kv_empty[k2]);
           }
-          if (!ok) break;
-          commit(&kv_empty[sv]);
-          if (more && !p.shared) commit(&kv_empty[k_slot(c + 1) % C::kSlots]);
+          k0 = k1;
+          k1 = k2;
         }
-        seq += it.chunks * per;
       }
       commit(drain_bar);
       mbar_drain(drain_bar, 0);
@@ -311,14 +321,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tok = row / p.s.g;
     const int head = row - tok * p.s.g;
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
-    const uint32_t sp = tmem + lane_off + static_cast<uint32_t>(w * 256);
-    const uint32_t od = sp + 128u;
+    const uint32_t st = tmem + lane_off + static_cast<uint32_t>(w * 256);
+    const uint32_t od = st + 128u;
     const uint32_t stage = smem_u32(smem + C::kOffStage) + static_cast<uint32_t>((warp - 4) * 2048);
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int gc = 0;  // chunks processed (all items)
     bool ok = true;
-    for (int item = blockIdx.x; item < p.grid.items; item += gridDim.x) {
-      const Item<kChunkBlks> it = make_item<kChunkBlks>(p.s, p.grid, item);
+    for (ItemWalk wk(p.s, p.grid); wk.item < p.grid.items; wk.next(p.s, p.grid)) {
+      const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
       const int first = it.first(w), last = it.last(w);
       const int t = it.t0(w) + tok;
       const bool valid = tok < p.grid.tt && t < it.t1(w);
@@ -329,33 +339,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int c = first; c <= last; ++c) {
         if (!it.active(w, c)) continue;
         const int nb = it.blocks(c);
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[w], gc & 1, abort_flag, p.err,
+        const uint32_t buf = static_cast<uint32_t>(gc) & 1u;
+        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[2 * w + buf], (gc >> 1) & 1, abort_flag, p.err,
                                                DSA_DEVERR_WIN_WAIT));
         if (!ok) break;
         tc_fence_after();
-        uint32_t v[kChunkBlks][32];
+        const uint32_t sp = st + buf * 64u;
+        uint32_t v[kCB][32];
 #pragma unroll
-        for (int i = 0; i < kChunkBlks; ++i)
+        for (int i = 0; i < kCB; ++i)
           if (i < nb) tmem_ld_32x32b_x32_nowait(sp + static_cast<uint32_t>(i * kBlk), v[i]);
+        const bool full = chunk_full<kCB>(p.s, it, it.t0(w), it.t1(w), c);
         float mx = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kChunkBlks; ++i) {
+        for (int i = 0; i < kCB; ++i) {
           if (i < nb) {
             tmem_wait_ld_dep(v[i]);
-            const uint32_t seen = seen_bits(p.s, it.r, c * kChunkBlks + i, pos, it.kv_len);
-            if (!__all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu)) {
+            if (!full) {
+              const uint32_t seen = seen_bits(p.s, it.r, c * kCB + i, pos, it.kv_len);
 #pragma unroll
               for (int k = 0; k < 32; ++k)
                 if (!((seen >> k) & 1u)) v[i][k] = 0xFF800000u;
             }
-            float a = fmaxf(__uint_as_float(v[i][0]), __uint_as_float(v[i][1]));
-            float b = fmaxf(__uint_as_float(v[i][2]), __uint_as_float(v[i][3]));
+            float a[4];
 #pragma unroll
-            for (int k = 4; k < 32; k += 4) {
-              a = fmax3(a, __uint_as_float(v[i][k]), __uint_as_float(v[i][k + 1]));
-              b = fmax3(b, __uint_as_float(v[i][k + 2]), __uint_as_float(v[i][k + 3]));
+            for (int k = 0; k < 4; ++k)
+              a[k] = fmaxf(__uint_as_float(v[i][k]), __uint_as_float(v[i][k + 4]));
+#pragma unroll
+            for (int k = 8; k < 32; k += 8) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                a[j] = fmax3(a[j], __uint_as_float(v[i][k + j]), __uint_as_float(v[i][k + j + 4]));
             }
-            mx = fmax3(mx, a, b);
+            mx = fmax3(mx, fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
           }
         }
         const float mz = mx * p.scale_log2;
@@ -369,7 +385,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             l *= factor;
           }
           if (__any_sync(0xFFFFFFFFu, factor != 1.f)) {
-            // this chunk's S was issued after the previous PV product completed
+            // O holds the previous chunk's product once that completed (the one before
+            // it completed before this chunk's S was issued)
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&o_done[2 * w + (buf ^ 1u)], ((gc - 1) >> 1) & 1,
+                                                   abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+            if (!ok) break;
+            tc_fence_after();
 #pragma unroll 1
             for (int q = 0; q < D / 32; ++q) {
               uint32_t ov[32];
@@ -384,7 +405,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint64_t neg2 = f2_pack(-ref, -ref);
         uint64_t sum2[2] = {0ull, 0ull};
 #pragma unroll
-        for (int i = 0; i < kChunkBlks; ++i) {
+        for (int i = 0; i < kCB; ++i) {
           if (i < nb) {
             uint32_t pk[16];
 #pragma unroll
@@ -406,7 +427,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += (a0 + a1) + (b0 + b1);
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[w]);
+        mbar_arrive(&p_full[2 * w + buf]);
         ++gc;
       }
       if (!ok) break;
@@ -421,30 +442,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = total == 0.f ? 0.f : mine / total;
       const int64_t orow = (static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + gh;
       if (last >= 0) {
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&o_done[w], (gc - 1) & 1, abort_flag, p.err,
-                                               DSA_DEVERR_WIN_WAIT));
+        ok = __all_sync(0xFFFFFFFFu,
+                        mbar_wait(&o_done[2 * w + ((gc - 1) & 1)], ((gc - 1) >> 1) & 1, abort_flag,
+                                  p.err, DSA_DEVERR_WIN_WAIT));
         if (!ok) break;
         tc_fence_after();
       }
-#pragma unroll 1
+      // the row is rounded as it is read, so that O is given back before the stores
+      uint32_t x[D / 32][16];
+#pragma unroll
       for (int q = 0; q < D / 32; ++q) {
         uint32_t ov[32];
-        if (last >= 0) {
-          tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) ov[k] = 0u;
-        }
-        uint32_t x[16];
+        if (last >= 0) tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          x[k] = T::pack(__uint_as_float(ov[2 * k]) * inv, __uint_as_float(ov[2 * k + 1]) * inv);
-        store_rows(stage, x, valid ? p.out + orow * D + q * 32 : nullptr, lane);
+          x[q][k] = last < 0 ? 0u
+                             : T::pack(__uint_as_float(ov[2 * k]) * inv, __uint_as_float(ov[2 * k + 1]) * inv);
       }
       if (last >= 0) {
         tc_fence_before();
         mbar_arrive(&o_empty[w]);
       }
+#pragma unroll
+      for (int q = 0; q < D / 32; ++q)
+        store_rows(stage, x[q], valid ? p.out + orow * D + q * 32 : nullptr, lane);
       if (valid && p.lse != nullptr) p.lse[orow] = (ref + log2f(total)) * kLn2;
     }
   }
