@@ -346,8 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       Gran late[C::kLag];  // of the chunks whose V is not yet requested
       auto load = [&](const CUtensorMap* tm, const Gran& g, bool mine, int gi, int bytes) -> bool {
-        if (!__all_sync(0xFFFFFFFFu, mbar_wait(&kv_empty[at.slot], at.parity ^ 1u, abort_flag, p.err,
-                                               DSA_DEVERR_WIN_WAIT)))
+        if (!mbar_wait_warp(&kv_empty[at.slot], at.parity ^ 1u, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
           return false;
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[at.slot], static_cast<uint32_t>(bytes));
         __syncwarp();
@@ -374,8 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         late[0] = g;
       };
       for (; ok && walk_take(p, wk); walk_next(wk), ++pieces) {
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(q_empty, (pieces & 1) ^ 1, abort_flag, p.err,
-                                               DSA_DEVERR_WIN_WAIT));
+        ok = mbar_wait_warp(q_empty, (pieces & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.g * D * 2));
@@ -457,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t fresh_bits = 0;  // bit k: chunk gc - 1 - k is its warpgroup's first of a piece
       bool ok = true;
       auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
-        return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+        return mbar_wait_warp(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
       };
       auto wait_slot = [&]() -> bool {
         return wait_warp(&kv_full[at.slot], at.parity);

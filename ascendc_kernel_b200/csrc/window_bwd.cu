@@ -222,8 +222,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int64_t x = blockIdx.x; ok && x < p.units; x += gridDim.x) {
         const Unit u = make_unit(p, x);
         if (u.r1 <= u.r0) continue;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(kv_empty, (uses & 1) ^ 1, abort_flag, p.err,
-                                               DSA_DEVERR_WIN_WAIT));
+        ok = mbar_wait_warp(kv_empty, (uses & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(kv_full, 2 * C::kTileBytes);
@@ -250,8 +249,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               st[i] = __ldg(p.stat + (static_cast<int64_t>(u.b) * p.s.m + t0 + tok) * p.s.h + h0 +
                             (row - tok * p.gb));
           }
-          ok = __all_sync(0xFFFFFFFFu, mbar_wait(&st_empty[s], ((gs / C::kStages) & 1) ^ 1, abort_flag,
-                                                 p.err, DSA_DEVERR_WIN_WAIT));
+          ok = mbar_wait_warp(&st_empty[s], ((gs / C::kStages) & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
           if (!ok) break;
           if (lane == 0) {
             uint8_t* dst = smem + C::kOffS + s * C::kStageBytes;
@@ -292,7 +290,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int gp[2] = {0, 0};
       bool ok = true;
       auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
-        return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+        return mbar_wait_warp(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
       };
       auto commit = [&](uint64_t* b) {
         if (elect_one()) umma_commit(b);
@@ -398,8 +396,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int i = 0; i < nt; ++i) {
         if (((gs + i) & 1) != w) continue;
         const int s = (gs + i) % C::kStages;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[w], gw & 1, abort_flag, p.err,
-                                               DSA_DEVERR_WIN_WAIT));
+        ok = mbar_wait_warp(&s_full[w], gw & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+        if (!ok) break;
+        // the statistics were written with ordinary stores: their barrier is waited
+        // for here too (it completed before this tile's products were issued)
+        ok = mbar_wait_warp(&st_full[s], ((gs + i) / C::kStages) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         tc_fence_after();
         uint32_t sv[2][32], dv[2][32];
@@ -416,11 +417,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int dup = (r % p.hb) == 0 ? 0 : p.hb * p.gb - p.s.g;
         const int ca = max(tok_a * p.gb, dup), cb = tok_b * p.gb;
         const uint32_t stat4 = smem_u32(smem + C::kOffStat) + static_cast<uint32_t>(s * 2 * kStream * 4);
-        // the statistics were written with ordinary stores: their barrier is waited
-        // for here too (it completed before this tile's products were issued)
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&st_full[s], ((gs + i) / C::kStages) & 1, abort_flag,
-                                               p.err, DSA_DEVERR_WIN_WAIT));
-        if (!ok) break;
         tmem_wait_ld_dep(sv[0]);
         tmem_wait_ld_dep(dv[0]);
         tmem_wait_ld_dep(sv[1]);
@@ -474,8 +470,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       gs += nt;
       // ---- epilogue: warpgroup 0 the first half of the columns, 1 the second
       if (nt > 0) {
-        ok = __all_sync(0xFFFFFFFFu,
-                        mbar_wait(acc_full, uses & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+        ok = mbar_wait_warp(acc_full, uses & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         tc_fence_after();
         ++uses;
@@ -629,7 +624,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int per = p.shared ? 1 : 2;
 
   if (threadIdx.x == 0) {
     for (int w = 0; w < 2; ++w) {
@@ -642,9 +636,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     for (int s = 0; s < C::kSlots; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], 2);
     }
-    mbar_init(drain_bar, 1);
+    mbar_init(drain_bar, 2);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_q);
@@ -665,59 +659,59 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     set_max_regs_dec<kBwdRegsAux>();
     if (warp == 0 && lane == 0) {
       // ---------------------------------------------------------- producer
-      int seq = 0;
-      int uses[2] = {0, 0};
+      Ring<C::kSlots> at;
+      int loads = 0;
+      int uses0 = 0, uses1 = 0;
       bool ok = true;
       auto load_slot = [&](const Item<kCB>& it, const CUtensorMap* tm, int c) -> bool {
-        const int s = seq % C::kSlots;
-        if (!mbar_wait(&kv_empty[s], ((seq / C::kSlots) & 1) ^ 1, abort_flag, p.err,
-                       DSA_DEVERR_WIN_WAIT))
+        if (!mbar_wait(&kv_empty[at.slot], at.parity ^ 1u, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
           return false;
         const int nb = it.blocks(c);
-        uint8_t* dst = smem + C::kOffKV + s * C::kSlotBytes;
-        mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(nb * kBlk * D * 2));
+        uint8_t* dst = smem + C::kOffKV + at.slot * C::kSlotBytes;
+        mbar_arrive_expect_tx(&kv_full[at.slot], static_cast<uint32_t>(nb * kBlk * D * 2));
         for (int i = 0; i < nb; ++i) {
           const int key = it.r.key(c * kCB + i);
 #pragma unroll
           for (int half = 0; half < C::kHalves; ++half)
             tma_load_4d(dst + half * kHalfBox + i * kBlk * 128, tm, half * 64, key, it.kvh, it.b,
-                        &kv_full[s]);
+                        &kv_full[at.slot]);
         }
-        ++seq;
+        at.next();
+        ++loads;
+        return true;
+      };
+      auto load_rows = [&](const Item<kCB>& it, int w, int& uses) -> bool {
+        if (it.last(w) < 0) return true;
+        if (!mbar_wait(&q_empty[w], (uses & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
+          return false;
+        uint8_t* qs = smem + C::kOffQ + 2 * w * C::kTileBytes;
+        mbar_arrive_expect_tx(&q_full[w], static_cast<uint32_t>(2 * p.grid.tt * p.s.g * D * 2));
+#pragma unroll
+        for (int half = 0; half < C::kHalves; ++half) {
+          tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0(w), it.b,
+                      &q_full[w]);
+          tma_load_4d(qs + C::kTileBytes + half * kBoxBytes, &tm_do, half * 64, it.kvh * p.s.g,
+                      it.t0(w), it.b, &q_full[w]);
+        }
+        ++uses;
         return true;
       };
       for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid)) {
         const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
-        for (int w = 0; w < 2 && ok; ++w) {
-          if (it.last(w) < 0) continue;
-          if (!mbar_wait(&q_empty[w], (uses[w] & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT)) {
-            ok = false;
-            break;
-          }
-          uint8_t* qs = smem + C::kOffQ + 2 * w * C::kTileBytes;
-          mbar_arrive_expect_tx(&q_full[w], static_cast<uint32_t>(2 * p.grid.tt * p.s.g * D * 2));
-#pragma unroll
-          for (int half = 0; half < C::kHalves; ++half) {
-            tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0(w), it.b,
-                        &q_full[w]);
-            tma_load_4d(qs + C::kTileBytes + half * kBoxBytes, &tm_do, half * 64, it.kvh * p.s.g,
-                        it.t0(w), it.b, &q_full[w]);
-          }
-          ++uses[w];
-        }
-        const int chunks = it.chunks;
-        for (int c = 0; c < chunks && ok; ++c) {
+        ok = load_rows(it, 0, uses0) && load_rows(it, 1, uses1);
+        for (int c = 0; c < it.chunks && ok; ++c) {
           ok = load_slot(it, &tm_k, c);
           if (ok && !p.shared) ok = load_slot(it, &tm_v, c);
         }
       }
-      for (int i = (seq > C::kSlots ? seq - C::kSlots : 0); i < seq; ++i)
+      for (int i = max(loads - C::kSlots, 0); i < loads; ++i)
         mbar_drain(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
-      for (int w = 0; w < 2; ++w)
-        if (uses[w] > 0) mbar_drain(&q_full[w], (uses[w] - 1) & 1);
-    } else if (warp == 1) {
-      // ---------------------------------------------------------- MMA issuer
+      if (uses0 > 0) mbar_drain(&q_full[0], (uses0 - 1) & 1);
+      if (uses1 > 0) mbar_drain(&q_full[1], (uses1 - 1) & 1);
+    } else if (warp == 1 || warp == 2) {
+      // ---------------------------------------------------------- MMA issuers, one per tile
       // the whole warp walks and waits; one elected lane issues
+      const int w = warp - 1;
       constexpr uint32_t idesc_o = make_idesc<T>(128, D, 1);
       const uint64_t dq0 = make_smem_desc(smem_u32(smem + C::kOffQ), 16u, 1024u, kLayoutSW128);
       const uint32_t hi = static_cast<uint32_t>(dq0 >> 32);
@@ -725,20 +719,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const uint32_t k_lo = q_lo + static_cast<uint32_t>((C::kOffKV - C::kOffQ) >> 4);
       const uint32_t mn_lo = static_cast<uint32_t>(make_smem_desc(
           smem_u32(smem + C::kOffKV), static_cast<uint32_t>(kHalfBox), 1024u, kLayoutSW128));
-      int seq = 0;
-      int gp[2] = {0, 0};
-      int uses[2] = {0, 0};
-      int first[2] = {0, 0}, last[2] = {-1, -1};
+      Ring<C::kSlots> at;  // the next slot in the order of the loads
+      int gp = 0, uses = 0;
       bool ok = true;
       auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
-        return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+        return mbar_wait_warp(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
       };
       auto commit = [&](uint64_t* b) {
         if (elect_one()) umma_commit(b);
         __syncwarp();
       };
-      auto issue_s = [&](int w, int c, int ks, int vs, int nb) -> bool {
-        if (gp[w] >= 1 && !wait_warp(&o_done[w], (gp[w] - 1) & 1)) return false;
+      // waits for the next slot and returns its number
+      auto take = [&]() -> int {
+        const int s = at.slot;
+        ok = ok && wait_warp(&kv_full[s], at.parity);
+        at.next();
+        return s;
+      };
+      auto issue_s = [&](const Item<kCB>& it, int c, int ks, int vs) {
+        if (!ok || !it.active(w, c)) return;
+        if (gp >= 1) ok = wait_warp(&o_done[w], (gp - 1) & 1);
+        if (!ok) return;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 256);
         const uint32_t qa = q_lo + static_cast<uint32_t>(2 * w * (C::kTileBytes >> 4));
@@ -746,7 +747,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const uint32_t kb = k_lo + static_cast<uint32_t>(ks * (C::kSlotBytes >> 4));
         const uint32_t vb = k_lo + static_cast<uint32_t>(vs * (C::kSlotBytes >> 4));
         const uint32_t idesc_s =
-            make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(nb * kBlk / 8) << 17);
+            make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(it.blocks(c) * kBlk / 8) << 17);
+        const bool end = c == it.last(w);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
@@ -763,18 +765,21 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
                       k > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[w]);
-          if (c == last[w]) umma_commit(&q_empty[w]);
+          if (end) umma_commit(&q_empty[w]);
         }
         __syncwarp();
-        return true;
       };
-      auto issue_o = [&](int w, int c, int slot, int nb) -> bool {
-        if (!wait_warp(&p_full[w], gp[w] & 1)) return false;
-        if (c == first[w] && uses[w] > 1 && !wait_warp(&o_empty[w], (uses[w] - 2) & 1)) return false;
+      auto issue_o = [&](const Item<kCB>& it, int c, int slot) {
+        if (!ok || !it.active(w, c)) return;
+        const bool fresh = c == it.first(w);
+        ok = wait_warp(&p_full[w], gp & 1);
+        if (ok && fresh && uses > 1) ok = wait_warp(&o_empty[w], (uses - 2) & 1);
+        if (!ok) return;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 256);
         const uint32_t kb = mn_lo + static_cast<uint32_t>(slot * (C::kSlotBytes >> 4));
-        const uint32_t more = c > first[w] ? 1u : 0u;
+        const int nb = it.blocks(c);
+        const uint32_t more = fresh ? 0u : 1u;
         if (elect_one()) {
 #pragma unroll
           for (int st = 0; st < kCB * 2; ++st)
@@ -785,14 +790,10 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           umma_commit(&o_done[w]);
         }
         __syncwarp();
-        ++gp[w];
-        return true;
-      };
-      auto wait_slot = [&](int i) -> bool {
-        return wait_warp(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
+        ++gp;
       };
       // K rows at or past kv_len may hold anything, and 0 x NaN is NaN: cleared before
-      // the product that sums over them
+      // the product that sums over them (by both issuers, to the same zeros)
       auto clear_tail = [&](const Item<kCB>& it, int c, int slot, int nb) {
         uint8_t* base = smem + C::kOffKV + slot * C::kSlotBytes;
         bool wrote = false;
@@ -810,41 +811,27 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       };
       for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid)) {
         const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
-        for (int w = 0; w < 2 && ok; ++w) {
-          first[w] = it.first(w);
-          last[w] = it.last(w);
-          if (last[w] < 0) continue;
-          ok = wait_warp(&q_full[w], uses[w] & 1);
-          ++uses[w];
-        }
-        if (!ok) break;
-        const int chunks = it.chunks;
-        auto k_slot = [&](int c) { return seq + c * per; };
-        auto v_slot = [&](int c) { return seq + c * per + per - 1; };
-        if (chunks > 0) {
-          ok = wait_slot(k_slot(0)) && wait_slot(v_slot(0));
-          for (int w = 0; w < 2 && ok; ++w)
-            if (it.active(w, 0))
-              ok = issue_s(w, 0, k_slot(0) % C::kSlots, v_slot(0) % C::kSlots, it.blocks(0));
-          if (ok && !p.shared) commit(&kv_empty[v_slot(0) % C::kSlots]);
-        }
-        for (int c = 0; c < chunks && ok; ++c) {
-          const int nb = it.blocks(c);
-          const bool more = c + 1 < chunks;
-          const int sk = k_slot(c) % C::kSlots;
-          if (p.s.kv_lens != nullptr) clear_tail(it, c, sk, nb);
-          if (more) ok = wait_slot(k_slot(c + 1)) && wait_slot(v_slot(c + 1));
-          for (int w = 0; w < 2 && ok; ++w) {
-            if (it.active(w, c)) ok = issue_o(w, c, sk, nb);
-            if (ok && more && it.active(w, c + 1))
-              ok = issue_s(w, c + 1, k_slot(c + 1) % C::kSlots, v_slot(c + 1) % C::kSlots,
-                           it.blocks(c + 1));
+        const int n = it.chunks;
+        if (n == 0) continue;
+        if (it.last(w) >= 0) ok = wait_warp(&q_full[w], uses++ & 1);
+        int ks = take();
+        int vs = p.shared ? ks : take();
+        issue_s(it, 0, ks, vs);
+        if (!p.shared) commit(&kv_empty[vs]);
+        for (int c = 0; c < n && ok; ++c) {
+          const int now = ks;
+          if (p.s.kv_lens != nullptr) clear_tail(it, c, now, it.blocks(c));
+          if (c + 1 < n) {
+            ks = take();
+            vs = p.shared ? ks : take();
           }
-          if (!ok) break;
-          commit(&kv_empty[sk]);
-          if (more && !p.shared) commit(&kv_empty[v_slot(c + 1) % C::kSlots]);
+          issue_o(it, c, now);
+          if (c + 1 < n) {
+            issue_s(it, c + 1, ks, vs);
+            if (!p.shared) commit(&kv_empty[vs]);
+          }
+          commit(&kv_empty[now]);
         }
-        seq += chunks * per;
       }
       commit(drain_bar);
       mbar_drain(drain_bar, 0);
@@ -878,8 +865,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       for (int c = first; c <= last; ++c) {
         if (!it.active(w, c)) continue;
         const int nb = it.blocks(c);
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[w], gc & 1, abort_flag, p.err,
-                                               DSA_DEVERR_WIN_WAIT));
+        ok = mbar_wait_warp(&s_full[w], gc & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         tc_fence_after();
         uint32_t sv[kCB][32], dv[kCB][32];
@@ -934,29 +920,25 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       }
       if (!ok) break;
       if (last >= 0) {
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&o_done[w], (gc - 1) & 1, abort_flag, p.err,
-                                               DSA_DEVERR_WIN_WAIT));
+        ok = mbar_wait_warp(&o_done[w], (gc - 1) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         tc_fence_after();
       }
-      // the row is rounded as it is read, so that O is given back before the stores
-      uint32_t x[D / 32][16];
-#pragma unroll
+#pragma unroll 1
       for (int q = 0; q < D / 32; ++q) {
-        uint32_t ov[32];
+        uint32_t ov[32], x[16];
         if (last >= 0) tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
 #pragma unroll
         for (int k = 0; k < 16; ++k)
-          x[q][k] = last < 0 ? 0u
-                             : T::pack(__uint_as_float(ov[2 * k]) * p.scale, __uint_as_float(ov[2 * k + 1]) * p.scale);
+          x[k] = last < 0 ? 0u
+                          : T::pack(__uint_as_float(ov[2 * k]) * p.scale,
+                                    __uint_as_float(ov[2 * k + 1]) * p.scale);
+        if (last >= 0 && q == D / 32 - 1) {
+          tc_fence_before();
+          mbar_arrive(&o_empty[w]);
+        }
+        store_rows(stage, x, valid ? p.dq + orow * D + q * 32 : nullptr, lane);
       }
-      if (last >= 0) {
-        tc_fence_before();
-        mbar_arrive(&o_empty[w]);
-      }
-#pragma unroll
-      for (int q = 0; q < D / 32; ++q)
-        store_rows(stage, x[q], valid ? p.dq + orow * D + q * 32 : nullptr, lane);
       if (valid && p.sink != nullptr) {
         float a0, a1, b0, b1;
         f2_unpack(psum[0], a0, a1);

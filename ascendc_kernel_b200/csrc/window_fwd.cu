@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (uses0 > 0) mbar_drain(&q_full[0], (uses0 - 1) & 1);
       if (uses1 > 0) mbar_drain(&q_full[1], (uses1 - 1) & 1);
     }
-  } else if (warp <= 2) {
+  } else if (warp == 1 || warp == 2) {
     // ------------------------------------------------------------ MMA issuers
     // the whole warp walks and waits; one elected lane issues
     {
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Ring<C::kSlots> at;  // the next slot in the order of the loads
       bool ok = true;
       auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
-        return __all_sync(0xFFFFFFFFu, mbar_wait(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+        return mbar_wait_warp(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
       };
       auto commit = [&](uint64_t* b) {
         if (elect_one()) umma_commit(b);
@@ -340,8 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!it.active(w, c)) continue;
         const int nb = it.blocks(c);
         const uint32_t buf = static_cast<uint32_t>(gc) & 1u;
-        ok = __all_sync(0xFFFFFFFFu, mbar_wait(&s_full[2 * w + buf], (gc >> 1) & 1, abort_flag, p.err,
-                                               DSA_DEVERR_WIN_WAIT));
+        ok = mbar_wait_warp(&s_full[2 * w + buf], (gc >> 1) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         tc_fence_after();
         const uint32_t sp = st + buf * 64u;
@@ -387,8 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (__any_sync(0xFFFFFFFFu, factor != 1.f)) {
             // O holds the previous chunk's product once that completed (the one before
             // it completed before this chunk's S was issued)
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(&o_done[2 * w + (buf ^ 1u)], ((gc - 1) >> 1) & 1,
-                                                   abort_flag, p.err, DSA_DEVERR_WIN_WAIT));
+            ok = mbar_wait_warp(&o_done[2 * w + (buf ^ 1u)], ((gc - 1) >> 1) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
@@ -442,9 +440,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float inv = total == 0.f ? 0.f : mine / total;
       const int64_t orow = (static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + gh;
       if (last >= 0) {
-        ok = __all_sync(0xFFFFFFFFu,
-                        mbar_wait(&o_done[2 * w + ((gc - 1) & 1)], ((gc - 1) >> 1) & 1, abort_flag,
-                                  p.err, DSA_DEVERR_WIN_WAIT));
+        ok = mbar_wait_warp(&o_done[2 * w + ((gc - 1) & 1)], ((gc - 1) >> 1) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         tc_fence_after();
       }
