@@ -162,13 +162,14 @@ __device__ __forceinline__ bool named_bar_or(uint32_t id, uint32_t nthreads, boo
   return out != 0u;
 }
 
-// A position in a ring of N slots and the parity of its barriers' phase.
+// A position in a ring of N slots and the parity of its barriers' phase (N = 0: the
+// number of slots is given at run time).
 template <int N>
 struct Ring {
   int slot = 0;
   uint32_t parity = 0;
-  __device__ __forceinline__ void next() {
-    if (++slot == N) {
+  __device__ __forceinline__ void next(int n = N) {
+    if (++slot == n) {
       slot = 0;
       parity ^= 1u;
     }

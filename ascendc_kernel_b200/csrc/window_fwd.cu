@@ -9,8 +9,8 @@
 // Per CTA (one per SM, persistent, 384 threads), a work item is two 128-row
 // tiles (consecutive tokens, all heads of a group) that share every key chunk of
 // up to 64 keys:
-//   warp 0      TMA: q tiles, K and V chunks into a ring of slots (one slot a
-//               chunk when K and V are the same tensor).
+//   warp 0      TMA: q tiles, K and V chunks into a ring of stages (twice as many when
+//               K and V are the same tensor and a stage holds it once).
 //   warps 1, 2  tcgen05 issuers, one per tile: S = Q K^T, then O += P V with P read
 //               from TMEM.
 //   warps 4..11 softmax: a warpgroup per tile, a thread per row: no exchange
@@ -47,7 +47,7 @@ struct FwdCfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kRows * D * 2;
   static constexpr int kSlotBytes = kCB * kBlk * D * 2;
-  static constexpr int kSlots = 8;
+  static constexpr int kSlots = 8;  // 8 stages of one slot (K = V) or 4 of two (K, V)
   static constexpr int kOffQ = 0;
   static constexpr int kOffKV = 2 * kTileBytes;
   static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;  // [8 warps] 2 KB, out rows
@@ -79,8 +79,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* q_full = bars;                  // [2] TMA -> MMA
   uint64_t* q_empty = q_full + 2;           // [2] last S of the tile done -> TMA
-  uint64_t* kv_full = q_empty + 2;          // [kSlots]
-  uint64_t* kv_empty = kv_full + C::kSlots; // [kSlots] both issuers
+  uint64_t* kv_full = q_empty + 2;          // [stages]
+  uint64_t* kv_empty = kv_full + C::kSlots; // [stages] both issuers
   uint64_t* s_full = kv_empty + C::kSlots;  // [2 tiles][2] S of a chunk in TMEM
   uint64_t* p_full = s_full + 4;            // [2 tiles][2] P written (128 arrivals)
   uint64_t* o_done = p_full + 4;            // [2 tiles][2] PV of a chunk completed
@@ -91,7 +91,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
-  const int per = p.shared ? 1 : 2;  // slots of a chunk
+  const int stages = p.shared ? C::kSlots : C::kSlots / 2;
+  const int stage_bytes = p.shared ? C::kSlotBytes : 2 * C::kSlotBytes;
 
   if (threadIdx.x == 0) {
     for (int w = 0; w < 2; ++w) {
@@ -129,24 +130,28 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      Ring<C::kSlots> at;
+      Ring<0> at;
       int loads = 0;
       int uses0 = 0, uses1 = 0;
       bool ok = true;
-      auto load_slot = [&](const Item<kCB>& it, const CUtensorMap* tm, int c) -> bool {
+      auto load = [&](const Item<kCB>& it, int c) -> bool {
         if (!mbar_wait(&kv_empty[at.slot], at.parity ^ 1u, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
           return false;
         const int nb = it.blocks(c);
-        uint8_t* dst = smem + C::kOffKV + at.slot * C::kSlotBytes;
-        mbar_arrive_expect_tx(&kv_full[at.slot], static_cast<uint32_t>(nb * kBlk * D * 2));
-        for (int i = 0; i < nb; ++i) {
-          const int key = it.r.key(c * kCB + i);
+        uint8_t* dst = smem + C::kOffKV + at.slot * stage_bytes;
+        mbar_arrive_expect_tx(&kv_full[at.slot],
+                              static_cast<uint32_t>(nb * kBlk * D * 2 * (p.shared ? 1 : 2)));
+        for (int kind = 0; kind < (p.shared ? 1 : 2); ++kind) {
+          const CUtensorMap* tm = kind == 0 ? &tm_k : &tm_v;
+          for (int i = 0; i < nb; ++i) {
+            const int key = it.r.key(c * kCB + i);
 #pragma unroll
-          for (int half = 0; half < C::kHalves; ++half)
-            tma_load_4d(dst + half * kHalfBox + i * kBlk * 128, tm, half * 64, key, it.kvh, it.b,
-                        &kv_full[at.slot]);
+            for (int half = 0; half < C::kHalves; ++half)
+              tma_load_4d(dst + kind * C::kSlotBytes + half * kHalfBox + i * kBlk * 128, tm, half * 64,
+                          key, it.kvh, it.b, &kv_full[at.slot]);
+          }
         }
-        at.next();
+        at.next(stages);
         ++loads;
         return true;
       };
@@ -165,18 +170,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid)) {
         const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
-        // the order in which the products use them: K(0), q, K(1), V(0), K(2), V(1), ...
-        if (it.chunks > 0) ok = load_slot(it, &tm_k, 0);
+        if (it.chunks > 0) ok = load(it, 0);
         ok = ok && load_q(it, 0, uses0) && load_q(it, 1, uses1);
-        if (ok && it.chunks > 1) ok = load_slot(it, &tm_k, 1);
-        for (int c = 0; c < it.chunks && ok; ++c) {
-          if (!p.shared) ok = load_slot(it, &tm_v, c);
-          if (ok && c + 2 < it.chunks) ok = load_slot(it, &tm_k, c + 2);
-        }
+        for (int c = 1; c < it.chunks && ok; ++c) ok = load(it, c);
       }
       // copies in flight land before the CTA's shared memory goes away
-      for (int i = max(loads - C::kSlots, 0); i < loads; ++i)
-        mbar_drain(&kv_full[i % C::kSlots], (i / C::kSlots) & 1);
+      for (int i = max(loads - stages, 0); i < loads; ++i)
+        mbar_drain(&kv_full[i % stages], (i / stages) & 1);
       if (uses0 > 0) mbar_drain(&q_full[0], (uses0 - 1) & 1);
       if (uses1 > 0) mbar_drain(&q_full[1], (uses1 - 1) & 1);
     }
@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t k_lo = static_cast<uint32_t>(dk);
       const uint32_t v_lo = static_cast<uint32_t>(make_smem_desc(
           smem_u32(smem + C::kOffKV), static_cast<uint32_t>(kHalfBox), 1024u, kLayoutSW128));
-      Ring<C::kSlots> at;  // the next slot in the order of the loads
+      Ring<0> at;  // the next stage
       bool ok = true;
       auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
         return mbar_wait_warp(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
@@ -202,11 +202,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (elect_one()) umma_commit(b);
         __syncwarp();
       };
-      // waits for the next slot and returns its number
+      // waits for the next stage and returns its number
       auto take = [&]() -> int {
         const int s = at.slot;
         ok = ok && wait_warp(&kv_full[s], at.parity);
-        at.next();
+        at.next(stages);
         return s;
       };
       int gs = 0, go = 0, uses = 0;  // S and PV products issued, items
@@ -219,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 256 + (gs & 1) * 64);
         const uint32_t qa = q_lo + static_cast<uint32_t>(w * (C::kTileBytes >> 4));
-        const uint32_t kb = k_lo + static_cast<uint32_t>(slot * (C::kSlotBytes >> 4));
+        const uint32_t kb = k_lo + static_cast<uint32_t>(slot * (stage_bytes >> 4));
         const uint32_t idesc_s =
             make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(it.blocks(c) * kBlk / 8) << 17);
         const bool end = c == it.last(w);
@@ -237,8 +237,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         ++gs;
       };
+      // PV of chunk c; the stage is given back
       auto issue_pv = [&](const Item<kCB>& it, int c, int slot) {
-        if (!ok || !it.active(w, c)) return;
+        if (!ok) return;
+        if (!it.active(w, c)) {
+          commit(&kv_empty[slot]);
+          return;
+        }
         const bool fresh = c == it.first(w);
         const int buf = 2 * w + (go & 1);
         ok = wait_warp(&p_full[buf], (go >> 1) & 1);
@@ -247,7 +252,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         const uint32_t sp = tmem + static_cast<uint32_t>(w * 256 + (go & 1) * 64);
         const uint32_t od = tmem + static_cast<uint32_t>(w * 256 + 128);
-        const uint32_t vb = v_lo + static_cast<uint32_t>(slot * (C::kSlotBytes >> 4));
+        const uint32_t vb =
+            v_lo + static_cast<uint32_t>((slot * stage_bytes + stage_bytes - C::kSlotBytes) >> 4);
         const int nb = it.blocks(c);
         const uint32_t more = fresh ? 0u : 1u;
         if (elect_one()) {
@@ -258,6 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                desc_from_words(vb + static_cast<uint32_t>(st * 128), hi), idesc_o,
                                st > 0 ? 1u : more);
           umma_commit(&o_done[buf]);
+          umma_commit(&kv_empty[slot]);
         }
         __syncwarp();
         ++go;
@@ -265,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // V rows at or past kv_len may hold anything, and 0 x NaN is NaN: they are
       // cleared before the product that reads them (by both issuers, to the same zeros)
       auto clear_tail = [&](const Item<kCB>& it, int c, int slot) {
-        uint8_t* base = smem + C::kOffKV + slot * C::kSlotBytes;
+        uint8_t* base = smem + C::kOffKV + slot * stage_bytes + stage_bytes - C::kSlotBytes;
         bool wrote = false;
         for (int i = 0; i < it.blocks(c); ++i) {
           const int key = it.r.key(c * kCB + i);
@@ -283,28 +290,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
         const int n = it.chunks;
         if (n == 0) continue;
-        // slots of K(c), K(c + 1) and K(c + 2); the other issuer takes the same
-        int k0 = take(), k1 = 0, k2 = 0;
+        // stages of chunks c, c + 1 and c + 2; the other issuer takes the same
+        int s0 = take(), s1 = 0, s2 = 0;
         if (it.last(w) >= 0) ok = ok && wait_warp(&q_full[w], uses++ & 1);
-        issue_s(it, 0, k0);
-        if (!p.shared) commit(&kv_empty[k0]);
+        issue_s(it, 0, s0);
         if (n > 1) {
-          k1 = take();
-          issue_s(it, 1, k1);
-          if (!p.shared) commit(&kv_empty[k1]);
+          s1 = take();
+          issue_s(it, 1, s1);
         }
         for (int c = 0; c < n && ok; ++c) {
-          const int v = p.shared ? k0 : take();
-          if (ok && p.s.kv_lens != nullptr) clear_tail(it, c, v);
-          issue_pv(it, c, v);
-          commit(&kv_empty[v]);
+          if (p.s.kv_lens != nullptr) clear_tail(it, c, s0);
+          issue_pv(it, c, s0);
           if (c + 2 < n) {
-            k2 = take();
-            issue_s(it, c + 2, k2);
-            if (!p.shared) commit(&kv_empty[k2]);
+            s2 = take();
+            issue_s(it, c + 2, s2);
           }
-          k0 = k1;
-          k1 = k2;
+          s0 = s1;
+          s1 = s2;
         }
       }
       commit(drain_bar);

@@ -112,6 +112,8 @@ SHAPES = [
     (2, 65, 411, 12, 2, 200, 130), (2, 100, 60, 8, 2, 20, 2), (1, 400, 400, 1, 1, 128, 200),
     (2, 64, 64, 14, 2, 9, 0), (1, 70, 90, 77, 1, 50, 3), (1, 257, 257, 2, 1, 129, 33),
     (1, 1, 385, 8, 1, 127, 32), (2, 7, 0, 4, 2, 5, 2),
+    # ragged: the second tile's window starts past the valid keys
+    (1, 540, 540, 1, 1, 20, 0), (1, 540, 540, 1, 1, 20, 5),
 ]
 
 
