@@ -131,6 +131,19 @@ def call(fn: str, *args) -> None:
     check(fn, getattr(lib(), fn)(*args))
 
 
+def bind(fn: str):
+    """Entry point `fn` as a function that raises DsaError on a non-zero status; for calls
+    short enough that the name lookup of :func:`call` shows."""
+    entry = getattr(lib(), fn)
+
+    def run(*args):
+        status = entry(*args)
+        if status != 0:
+            check(fn, status)
+
+    return run
+
+
 def device_error(device: int, clear: bool = True) -> int:
     """Synchronizes `device` and returns (then clears) its device error word."""
     code = ctypes.c_uint(0)

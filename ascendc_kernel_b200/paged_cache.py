@@ -16,42 +16,50 @@ Shape preconditions are checked with ``assert``; CUDA-level failures raise DsaEr
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
-from ._native import call, lib
-from .window_attn import DTYPES, _ptr, _sink_on, _strided, _strides
+from ._native import lib
+from .window_attn import DTYPES, _ptr, _run, _sink_on, _strided, _strides
 
 
 def _check_pool(k_pages, v_pages, weights, block_table):
+    """Checks what the operators share; returns num_pages, page_size, hk, d and the device."""
     assert k_pages.is_cuda and k_pages.dtype in DTYPES and k_pages.dim() == 4, \
         "k_pages must be a CUDA tensor [num_pages, page_size, hk, d], bf16 or fp16"
-    n, page, hk, d = k_pages.shape
+    shape, dev = k_pages.shape, k_pages.device
+    n, page, hk, d = shape
     for x in (k_pages, v_pages):
         if x is not None:
-            assert x.shape == k_pages.shape and x.dtype == k_pages.dtype \
-                and x.device == k_pages.device, "v_pages must be like k_pages"
-            assert x.stride(3) == 1 and all(s % 8 == 0 and s > 0 for s in x.stride()[:3]) \
-                and x.data_ptr() % 16 == 0, \
+            assert x.shape == shape and x.dtype == k_pages.dtype and x.device == dev, \
+                "v_pages must be like k_pages"
+            assert x.data_ptr() % 16 == 0 and (x.is_contiguous() or (
+                x.stride(3) == 1 and all(s % 8 == 0 and s > 0 for s in x.stride()[:3]))), \
                 "pages need a contiguous head_dim and strides in multiples of 8 elements"
     assert n >= 1 and page >= 1 and page % 8 == 0, "page_size must be a multiple of 8"
     assert d in (64, 128), "kernel specialised to head_dim in (64, 128)"
     if weights is not None:
-        assert weights.shape == (n, page) and weights.dtype == torch.float32 \
-            and weights.is_contiguous() and weights.device == k_pages.device, \
+        assert weights.shape == shape[:2] and weights.dtype == torch.float32 \
+            and weights.device == dev and weights.is_contiguous(), \
             "weights must be fp32 [num_pages, page_size], contiguous"
-    assert block_table.dtype == torch.int32 and block_table.dim() == 2 \
-        and block_table.device == k_pages.device and block_table.shape[1] >= 1, \
-        "block_table must be int32 [b, max_pages]"
+    _check_table(block_table, dev, "block_table")
+    return n, page, hk, d, dev
 
 
-def _check_lens(lens, b, device, name="lens"):
-    assert lens.dtype == torch.int32 and lens.shape == (b,) and lens.device == device, \
+def _check_table(table, dev, name):
+    assert table.dtype == torch.int32 and table.dim() == 2 and table.device == dev \
+        and table.shape[1] >= 1, f"{name} must be int32 [b, pages] on the pool's device"
+
+
+def _check_lens(lens, b, dev, name="lens"):
+    assert lens.dtype == torch.int32 and lens.shape == (b,) and lens.device == dev, \
         f"{name} must be int32 [b] on the pool's device"
 
 
-def _page_strides(x):
-    return (ctypes.c_int64 * 3)(*x.stride()[:3])
+@functools.lru_cache(maxsize=256)
+def _attn_workspace(b, h, hk, d, max_pages, page, weights) -> int:
+    return max(lib().dsa_paged_attn_workspace_bytes(b, h, hk, d, max_pages, page, weights), 256)
 
 
 def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor | None,
@@ -68,43 +76,48 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor | N
     fp32 log of the softmax divisor [b, h]. With ``weights`` the slot of each visible row
     gains its attention weight summed over the heads, in place.
     """
-    assert q.is_cuda and q.dim() == 3, "q must be a CUDA tensor [b, h, d]"
-    _check_pool(k_pages, v_pages, weights, block_table)
-    b, h, d = q.shape
-    n, page, hk, _ = k_pages.shape
-    assert q.dtype == k_pages.dtype and q.device == k_pages.device and d == k_pages.shape[3], \
+    assert q.dim() == 3, "q must be [b, h, d]"
+    n, page, hk, d, dev = _check_pool(k_pages, v_pages, weights, block_table)
+    b, h, _ = q.shape
+    assert q.dtype == k_pages.dtype and q.device == dev and q.shape[2] == d, \
         "q must have the pool's type, device and head_dim"
     assert h % hk == 0 and 1 <= h // hk <= 128, \
         "n_heads must be a multiple of n_kv_heads, at most 128 to a group"
+    width = block_table.shape[1]
     assert block_table.shape[0] == b
-    _check_lens(lens, b, q.device)
+    _check_lens(lens, b, dev)
     scale = float(d ** -0.5 if softmax_scale is None else softmax_scale)
     assert window >= 0 and n_first >= 0 and scale > 0
     if sink is not None:
         assert sink.numel() == h, "sink must have n_heads entries"
-    if q.stride(2) != 1 or q.data_ptr() % 16 or any(
-            m > 1 and (s <= 0 or s % 8) for m, s in zip(q.shape, q.stride()[:2])):
-        q = q.contiguous()
+        sink = _sink_on(sink, dev)
+    strides = None
+    if not q.is_contiguous():
+        if q.stride(2) != 1 or any(m > 1 and (s <= 0 or s % 8)
+                                   for m, s in zip(q.shape, q.stride()[:2])):
+            q = q.contiguous()
+        else:
+            strides = (ctypes.c_int64 * 2)(*q.stride()[:2])
+    if q.data_ptr() % 16:
+        q, strides = q.clone(memory_format=torch.contiguous_format), None
     if out is None:
-        out = torch.empty(b, h, d, dtype=q.dtype, device=q.device)
+        out = torch.empty((b, h, d), dtype=q.dtype, device=dev)
     else:
-        assert out.shape == q.shape and out.dtype == q.dtype and out.device == q.device \
+        assert out.shape == q.shape and out.dtype == q.dtype and out.device == dev \
             and out.is_contiguous(), "out must be contiguous and like q"
-    lse = torch.empty(b, h, dtype=torch.float32, device=q.device) if return_lse else None
-    sink = _sink_on(sink, q.device)
+    lse = torch.empty((b, h), dtype=torch.float32, device=dev) if return_lse else None
     table, lens = block_table.contiguous(), lens.contiguous()
-    values = k_pages if v_pages is None else v_pages
-    nbytes = lib().dsa_paged_attn_workspace_bytes(b, h, hk, d, table.shape[1], page,
-                                                  0 if weights is None else 1)
-    ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=q.device)
-    stream = torch.cuda.current_stream(q.device).cuda_stream
-    with torch.cuda.device(q.device):
-        call("dsa_paged_attn_fwd", q.data_ptr(), (ctypes.c_int64 * 2)(*q.stride()[:2]),
-             k_pages.data_ptr(), _page_strides(k_pages), values.data_ptr(), _page_strides(values),
-             table.data_ptr(), lens.data_ptr(), _ptr(sink), out.data_ptr(), _ptr(lse),
-             _ptr(weights), DTYPES[q.dtype], b, h, hk, d, n, page, table.shape[1],
-             min(int(window), 1 << 28), min(int(n_first), 1 << 28), scale, ws.data_ptr(),
-             ws.numel(), stream)
+    nbytes = _attn_workspace(b, h, hk, d, width, page, 0 if weights is None else 1)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    k_strides = _strides(k_pages)
+    if v_pages is None:
+        values, v_strides = k_pages.data_ptr(), k_strides
+    else:
+        values, v_strides = v_pages.data_ptr(), _strides(v_pages)
+    _run("dsa_paged_attn_fwd", q.get_device(), q.data_ptr(), strides, k_pages.data_ptr(), k_strides,
+         values, v_strides, table.data_ptr(), lens.data_ptr(), _ptr(sink), out.data_ptr(), _ptr(lse),
+         _ptr(weights), DTYPES[q.dtype], b, h, hk, d, n, page, width, min(int(window), 1 << 28),
+         min(int(n_first), 1 << 28), scale, ws.data_ptr(), nbytes)
     return (out, lse) if return_lse else out
 
 
@@ -114,25 +127,24 @@ def cache_append(k: torch.Tensor, v: torch.Tensor | None, k_pages: torch.Tensor,
     """Writes k, v [b, t, hk, d] to rows start[b] .. start[b] + t - 1 of each sequence and
     sets their slots' ``weights`` to 0. ``start`` int32 [b]. Rows past the table's room or
     of pages that do not exist are not written (see ``_native.device_error``)."""
-    _check_pool(k_pages, v_pages, weights, block_table)
+    n, page, hk, d, dev = _check_pool(k_pages, v_pages, weights, block_table)
     assert (v is None) == (v_pages is None), "v and v_pages are both given or both None"
-    b, t, hk, d = k.shape
-    n, page = k_pages.shape[:2]
-    assert (hk, d) == tuple(k_pages.shape[2:]) and k.dtype == k_pages.dtype \
-        and k.device == k_pages.device, "k must be [b, t, hk, d] of the pool's type and device"
-    if v is not None:
-        assert v.shape == k.shape and v.dtype == k.dtype and v.device == k.device
+    assert k.dim() == 4 and k.shape[2:] == k_pages.shape[2:] and k.dtype == k_pages.dtype \
+        and k.device == dev, "k must be [b, t, hk, d] of the pool's type and device"
+    b, t = k.shape[:2]
     assert block_table.shape[0] == b
-    _check_lens(start, b, k.device, "start")
+    _check_lens(start, b, dev, "start")
     k = _strided(k)
-    v = None if v is None else _strided(v)
+    v_ptr = v_strides = None
+    if v is not None:
+        assert v.shape == k.shape and v.dtype == k.dtype and v.device == dev, "v must be like k"
+        v = _strided(v)
+        v_ptr, v_strides = v.data_ptr(), _strides(v)
     table, start = block_table.contiguous(), start.contiguous()
-    stream = torch.cuda.current_stream(k.device).cuda_stream
-    with torch.cuda.device(k.device):
-        call("dsa_cache_append", k.data_ptr(), _strides(k), _ptr(v),
-             None if v is None else _strides(v), k_pages.data_ptr(), _page_strides(k_pages),
-             _ptr(v_pages), None if v_pages is None else _page_strides(v_pages), _ptr(weights),
-             table.data_ptr(), start.data_ptr(), b, t, hk, d, n, page, table.shape[1], stream)
+    _run("dsa_cache_append", k.get_device(), k.data_ptr(), _strides(k), v_ptr, v_strides,
+         k_pages.data_ptr(), _strides(k_pages), _ptr(v_pages),
+         None if v_pages is None else _strides(v_pages), _ptr(weights), table.data_ptr(),
+         start.data_ptr(), b, t, hk, d, n, page, table.shape[1])
 
 
 def cache_evict(k_pages: torch.Tensor, v_pages: torch.Tensor | None, weights: torch.Tensor,
@@ -144,25 +156,22 @@ def cache_evict(k_pages: torch.Tensor, v_pages: torch.Tensor | None, weights: to
     0, 1, ... of the pages of ``dst_table`` [b, dst_pages] int32 (distinct pages that no
     sequence of the call uses); the old pages stay as they are. Returns the kept rows
     [b, budget] int32, filled up with -1, and the new lengths [b] int32."""
-    _check_pool(k_pages, v_pages, weights, block_table)
-    n, page, hk, d = k_pages.shape
-    b = block_table.shape[0]
+    n, page, hk, d, dev = _check_pool(k_pages, v_pages, weights, block_table)
+    b, width = block_table.shape
     assert weights is not None, "eviction goes by the weights"
-    _check_lens(lens, b, k_pages.device)
-    assert dst_table.dtype == torch.int32 and dst_table.dim() == 2 and dst_table.shape[0] == b \
-        and dst_table.device == k_pages.device, "dst_table must be int32 [b, dst_pages]"
+    _check_lens(lens, b, dev)
+    _check_table(dst_table, dev, "dst_table")
+    assert dst_table.shape[0] == b
     assert budget >= 1 and n_first >= 0 and n_recent >= 0 and n_first + n_recent <= budget, \
         "n_first + n_recent <= budget"
     assert budget <= dst_table.shape[1] * page, "dst_table has no room for budget rows"
     table, lens, dst = block_table.contiguous(), lens.contiguous(), dst_table.contiguous()
-    kept = torch.empty(b, budget, dtype=torch.int32, device=k_pages.device)
-    left = torch.empty(b, dtype=torch.int32, device=k_pages.device)
-    stream = torch.cuda.current_stream(k_pages.device).cuda_stream
-    with torch.cuda.device(k_pages.device):
-        call("dsa_cache_evict", k_pages.data_ptr(), _page_strides(k_pages), _ptr(v_pages),
-             None if v_pages is None else _page_strides(v_pages), weights.data_ptr(),
-             table.data_ptr(), lens.data_ptr(), dst.data_ptr(), kept.data_ptr(), left.data_ptr(),
-             b, hk, d, n, page, table.shape[1], dst.shape[1], budget, n_first, n_recent, stream)
+    kept = torch.empty((b, budget), dtype=torch.int32, device=dev)
+    left = torch.empty((b,), dtype=torch.int32, device=dev)
+    _run("dsa_cache_evict", k_pages.get_device(), k_pages.data_ptr(), _strides(k_pages),
+         _ptr(v_pages), None if v_pages is None else _strides(v_pages), weights.data_ptr(),
+         table.data_ptr(), lens.data_ptr(), dst.data_ptr(), kept.data_ptr(), left.data_ptr(), b, hk,
+         d, n, page, width, dst.shape[1], budget, n_first, n_recent)
     return kept, left
 
 

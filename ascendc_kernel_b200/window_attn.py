@@ -17,13 +17,21 @@ import ctypes
 import torch
 import torch.nn as nn
 
-from ._native import call, lib
+from ._native import bind, lib
+
+try:  # the current stream's raw handle without building a Stream object
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+except AttributeError:  # pragma: no cover - older torch
+    def _raw_stream(device: int) -> int:
+        return torch.cuda.current_stream(device).cuda_stream
 
 DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # DSA_DTYPE_*
 
 
 def _strided(x: torch.Tensor) -> torch.Tensor:
     """x itself when the kernels can step over its strides, else a contiguous copy."""
+    if x.is_contiguous() and x.data_ptr() % 16 == 0:
+        return x
     ok = x.stride(-1) == 1 and x.data_ptr() % 16 == 0 and all(
         n <= 1 or (s > 0 and s % 8 == 0) for n, s in zip(x.shape[:-1], x.stride()[:-1]))
     if ok:
@@ -32,8 +40,29 @@ def _strided(x: torch.Tensor) -> torch.Tensor:
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
+_I64x3 = ctypes.c_int64 * 3
+
+
 def _strides(x: torch.Tensor):
-    return (ctypes.c_int64 * 3)(*x.stride()[:3])
+    """The first three strides for the C ABI; None (contiguous) where they are that."""
+    return None if x.is_contiguous() else _I64x3(*x.stride()[:3])
+
+
+_entries = {}
+
+
+def _run(fn: str, dev: int, *args) -> None:
+    """Calls entry point `fn` on device `dev` with the current stream there as the last
+    argument. The entry points are bound once, and the device guard is entered only for a
+    device that is not the current one: the calls are a few microseconds long."""
+    entry = _entries.get(fn)
+    if entry is None:
+        entry = _entries[fn] = bind(fn)
+    if dev == torch.cuda.current_device():
+        entry(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            entry(*args, _raw_stream(dev))
 
 
 def _check(q, k, v, sink, window, n_first, kv_lens, softmax_scale):
@@ -60,8 +89,9 @@ def _check(q, k, v, sink, window, n_first, kv_lens, softmax_scale):
 
 
 def _sink_on(sink, device):
-    if sink is None:
-        return None
+    if sink is None or (sink.dtype == torch.float32 and sink.device == device
+                        and sink.is_contiguous()):
+        return sink
     return sink.detach().to(device=device, dtype=torch.float32).contiguous()
 
 
@@ -79,11 +109,9 @@ def _forward(q, k, v, sink, window, n_first, kv_lens, scale, out, want_lse):
     if out is None:
         out = torch.empty(b, m, h, d, dtype=q.dtype, device=q.device)
     lse = torch.empty(b, m, h, dtype=torch.float32, device=q.device) if want_lse else None
-    stream = torch.cuda.current_stream(q.device).cuda_stream
-    with torch.cuda.device(q.device):
-        call("dsa_window_attn_fwd", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
-             v.data_ptr(), _strides(v), _ptr(sink), _ptr(kv_lens), out.data_ptr(), _ptr(lse),
-             DTYPES[q.dtype], b, m, n, h, hk, d, window, n_first, scale, stream)
+    _run("dsa_window_attn_fwd", q.get_device(), q.data_ptr(), _strides(q), k.data_ptr(),
+         _strides(k), v.data_ptr(), _strides(v), _ptr(sink), _ptr(kv_lens), out.data_ptr(),
+         _ptr(lse), DTYPES[q.dtype], b, m, n, h, hk, d, window, n_first, scale)
     return out, lse
 
 
@@ -118,13 +146,11 @@ def window_attn_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
     nbytes = lib().dsa_window_attn_bwd_workspace_bytes(b, m, n, h, hk, d, window, n_first,
                                                        1 if v is None else 0)
     ws = torch.empty(max(nbytes, 256), dtype=torch.uint8, device=dev)
-    stream = torch.cuda.current_stream(dev).cuda_stream
-    with torch.cuda.device(dev):
-        call("dsa_window_attn_bwd", q.data_ptr(), _strides(q), k.data_ptr(), _strides(k),
-             values.data_ptr(), _strides(values), _ptr(sink), _ptr(kv_lens), out.data_ptr(),
-             lse.data_ptr(), dout.data_ptr(), _strides(dout), dq.data_ptr(), dk.data_ptr(),
-             _ptr(dv), _ptr(dsink), DTYPES[q.dtype], b, m, n, h, hk, d, window, n_first, scale,
-             ws.data_ptr(), ws.numel(), stream)
+    _run("dsa_window_attn_bwd", q.get_device(), q.data_ptr(), _strides(q), k.data_ptr(),
+         _strides(k), values.data_ptr(), _strides(values), _ptr(sink), _ptr(kv_lens),
+         out.data_ptr(), lse.data_ptr(), dout.data_ptr(), _strides(dout), dq.data_ptr(),
+         dk.data_ptr(), _ptr(dv), _ptr(dsink), DTYPES[q.dtype], b, m, n, h, hk, d, window,
+         n_first, scale, ws.data_ptr(), ws.numel())
     return dq, dk, dv, dsink
 
 
