@@ -78,7 +78,7 @@ struct DkvCfg {
   static constexpr int kOffStat = kOffS + kStages * kStageBytes;  // [stage][2][64] f32
   static constexpr int kOffStage = kOffStat + kStages * 2 * kStream * 4;  // [8 warps] 2 KB
   static constexpr int kOffBar = kOffStage + 8 * 2048;
-  static constexpr int kNumBars = 2 + 2 * kStages + 2 + 2 + 2 + 1 + 1 + 1;
+  static constexpr int kNumBars = 2 + 2 * kStages + 2 + 2 + 2 + 2 + 2 + 1 + 1 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
 };
@@ -157,9 +157,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint64_t* kv_empty = bars + 1;
   uint64_t* st_full = bars + 2;                // [kStages] rows and statistics (1 + 32 arrivals)
   uint64_t* st_empty = st_full + C::kStages;   // [kStages] products done and statistics read
-  uint64_t* s_full = st_empty + C::kStages;    // [2] S^T and dP^T of a tile in TMEM
-  uint64_t* p_full = s_full + 2;               // [2] P^T and dS^T written (128 arrivals)
-  uint64_t* o_done = p_full + 2;               // [2] products of a tile completed
+  uint64_t* s_full = st_empty + C::kStages;    // [2] S^T of a tile in TMEM
+  uint64_t* dp_full = s_full + 2;              // [2] dP^T of a tile in TMEM
+  uint64_t* p_full = dp_full + 2;              // [2] P^T written (128 arrivals)
+  uint64_t* ds_full = p_full + 2;              // [2] dS^T written (128 arrivals)
+  uint64_t* o_done = ds_full + 2;              // [2] products of a tile completed
   uint64_t* acc_full = o_done + 2;             // all products of the unit completed
   uint64_t* acc_empty = acc_full + 1;          // accumulators read (256 arrivals)
   uint64_t* drain_bar = acc_empty + 1;
@@ -179,12 +181,14 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
     }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&s_full[w], 1);
+      mbar_init(&dp_full[w], 1);
       mbar_init(&p_full[w], 128);
+      mbar_init(&ds_full[w], 128);
       mbar_init(&o_done[w], 1);
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 256);
-    mbar_init(drain_bar, 1);
+    mbar_init(drain_bar, 2);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_q);
@@ -274,9 +278,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       if (uses > 0) mbar_drain(kv_full, (uses - 1) & 1);
       for (int i = (gs > C::kStages ? gs - C::kStages : 0); i < gs; ++i)
         mbar_drain(&st_full[i % C::kStages], (i / C::kStages) & 1);
-    } else if (warp == 1) {
-      // ---------------------------------------------------------- MMA issuer
-      // the whole warp walks and waits; one elected lane issues
+    } else if (warp == 1 || warp == 2) {
+      // ---------------------------------------------------------- MMA issuers
+      // warp 1: S^T and dP^T, warp 2: the products over the rows. Each walks and waits as
+      // a whole, one elected lane issues. A tile's four products start one by one as their
+      // operands are there: P^T is formed while dP^T is computed, dV summed while dS^T is
+      // formed
       constexpr uint32_t idesc_s = make_idesc<T>(128, kStream, 0);
       constexpr uint32_t idesc_o = make_idesc<T>(128, D, 1);
       const uint64_t dk0 = make_smem_desc(smem_u32(smem + C::kOffK), 16u, 1024u, kLayoutSW128);
@@ -287,7 +294,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const uint32_t mn_lo = static_cast<uint32_t>(make_smem_desc(
           smem_u32(smem + C::kOffS), static_cast<uint32_t>(kHalfBox), 1024u, kLayoutSW128));
       int gs = 0, uses = 0;
-      int gp[2] = {0, 0};
       bool ok = true;
       auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
         return mbar_wait_warp(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
@@ -296,10 +302,11 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (elect_one()) umma_commit(b);
         __syncwarp();
       };
-      auto issue_s = [&](int i) -> bool {  // i: global tile number; buffer i & 1
+      // i: number of the streamed tile in the CTA; it uses buffer i & 1
+      auto issue_s = [&](int i) -> bool {
         const int w = i & 1, s = i % C::kStages;
         if (!wait_warp(&st_full[s], (i / C::kStages) & 1)) return false;
-        if (gp[w] >= 1 && !wait_warp(&o_done[w], (gp[w] - 1) & 1)) return false;
+        if (i >= 2 && !wait_warp(&o_done[w], ((i - 2) >> 1) & 1)) return false;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 128);
         const uint32_t qb = s_lo + static_cast<uint32_t>(s * (C::kStageBytes >> 4));
@@ -312,6 +319,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             umma_bf16(d, desc_from_words(k_lo + ao, hi), desc_from_words(qb + bo, hi), idesc_s,
                       k > 0 ? 1u : 0u);
           }
+          umma_commit(&s_full[w]);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
@@ -319,52 +327,54 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             umma_bf16(d + 64u, desc_from_words(v_lo + ao, hi), desc_from_words(ob + bo, hi), idesc_s,
                       k > 0 ? 1u : 0u);
           }
-          umma_commit(&s_full[w]);
+          umma_commit(&dp_full[w]);
         }
         __syncwarp();
         return true;
       };
       auto issue_o = [&](int i, bool fresh) -> bool {
         const int w = i & 1, s = i % C::kStages;
-        if (!wait_warp(&p_full[w], gp[w] & 1)) return false;
-        tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 128);
         const uint32_t qb = mn_lo + static_cast<uint32_t>(s * (C::kStageBytes >> 4));
         const uint32_t ob = qb + static_cast<uint32_t>(C::kStageBytes >> 5);
+        const uint32_t more = fresh ? 0u : 1u;
+        if (!wait_warp(&p_full[w], (i >> 1) & 1)) return false;
+        tc_fence_after();
         if (elect_one()) {
 #pragma unroll
-          for (int st = 0; st < kStream / 16; ++st) {
-            const uint32_t acc = (fresh && st == 0) ? 0u : 1u;
-            const uint32_t bo = static_cast<uint32_t>(st * 128);
+          for (int st = 0; st < kStream / 16; ++st)
             umma_bf16_tmem_a(tmem + 384u, d + static_cast<uint32_t>(st * 8),
-                             desc_from_words(ob + bo, hi), idesc_o, acc);
+                             desc_from_words(ob + static_cast<uint32_t>(st * 128), hi), idesc_o,
+                             st > 0 ? 1u : more);
+        }
+        __syncwarp();
+        if (!wait_warp(&ds_full[w], (i >> 1) & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int st = 0; st < kStream / 16; ++st)
             umma_bf16_tmem_a(tmem + 256u, d + 64u + static_cast<uint32_t>(st * 8),
-                             desc_from_words(qb + bo, hi), idesc_o, acc);
-          }
+                             desc_from_words(qb + static_cast<uint32_t>(st * 128), hi), idesc_o,
+                             st > 0 ? 1u : more);
           umma_commit(&o_done[w]);
           umma_commit(&st_empty[s]);
         }
         __syncwarp();
-        ++gp[w];
         return true;
       };
       for (int64_t x = blockIdx.x; ok && x < p.units; x += gridDim.x) {
         const Unit u = make_unit(p, x);
         const int nt = u.r1 - u.r0;
         if (nt <= 0) continue;
-        ok = wait_warp(kv_full, uses & 1);
-        ok = ok && issue_s(gs) && (nt < 2 || issue_s(gs + 1));
-        if (ok && nt <= 2) commit(kv_empty);
-        ok = ok && (uses == 0 || wait_warp(acc_empty, (uses - 1) & 1));
-        for (int i = 0; i < nt && ok; ++i) {
-          ok = issue_o(gs + i, i == 0);
-          if (ok && i + 2 < nt) {
-            ok = issue_s(gs + i + 2);
-            if (ok && i + 3 == nt) commit(kv_empty);  // the key tile is no longer read
-          }
+        if (warp == 1) {
+          ok = wait_warp(kv_full, uses & 1);
+          for (int i = 0; i < nt && ok; ++i) ok = issue_s(gs + i);
+          if (ok) commit(kv_empty);  // the key tile is no longer read
+        } else {
+          ok = uses == 0 || wait_warp(acc_empty, (uses - 1) & 1);
+          for (int i = 0; i < nt && ok; ++i) ok = issue_o(gs + i, i == 0);
+          if (ok) commit(acc_full);
         }
-        if (!ok) break;
-        commit(acc_full);
         gs += nt;
         ++uses;
       }
@@ -403,11 +413,6 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ok = mbar_wait_warp(&st_full[s], ((gs + i) / C::kStages) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         tc_fence_after();
-        uint32_t sv[2][32], dv[2][32];
-        tmem_ld_32x32b_x32_nowait(sp, sv[0]);
-        tmem_ld_32x32b_x32_nowait(sp + 64u, dv[0]);
-        tmem_ld_32x32b_x32_nowait(sp + 32u, sv[1]);
-        tmem_ld_32x32b_x32_nowait(sp + 96u, dv[1]);
         // the columns (rows of the streamed tile) that see this key: one range,
         // since rows are token-major
         const int r = u.r0 + i;
@@ -416,54 +421,82 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         const int tok_b = min(max(end - p0, 0), p.tt);
         const int dup = (r % p.hb) == 0 ? 0 : p.hb * p.gb - p.s.g;
         const int ca = max(tok_a * p.gb, dup), cb = tok_b * p.gb;
+        const uint32_t seen[2] = {bits_between(ca, cb), bits_between(ca - 32, cb - 32)};
+        const bool all = __all_sync(0xFFFFFFFFu, (seen[0] & seen[1]) == 0xFFFFFFFFu);
+        // two 16-bit weights of a word that their rows do not see become 0
+        auto keep = [&](uint32_t word, uint32_t bits, int k) -> uint32_t {
+          const uint32_t two = (bits >> (2 * k)) & 3u;
+          return word & ((two & 1u ? 0x0000FFFFu : 0u) | (two & 2u ? 0xFFFF0000u : 0u));
+        };
         const uint32_t stat4 = smem_u32(smem + C::kOffStat) + static_cast<uint32_t>(s * 2 * kStream * 4);
+        uint32_t sv[2][32];  // S^T, then P^T in fp32
+        tmem_ld_32x32b_x32_nowait(sp, sv[0]);
+        tmem_ld_32x32b_x32_nowait(sp + 32u, sv[1]);
         tmem_wait_ld_dep(sv[0]);
-        tmem_wait_ld_dep(dv[0]);
         tmem_wait_ld_dep(sv[1]);
-        tmem_wait_ld_dep(dv[1]);
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const uint32_t seen = bits_between(ca - 32 * q, cb - 32 * q);
-          const bool all = __all_sync(0xFFFFFFFFu, seen == 0xFFFFFFFFu);
-          uint32_t pk[16], dk[16];
+          uint32_t pk[16];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             const float4 nl = ld_shared_f4(stat4 + static_cast<uint32_t>((q * 8 + k) * 16));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int c = 4 * k + 2 * e;
+              float z0, z1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[q][c]), __uint_as_float(sv[q][c + 1])),
+                               scale2, e ? f2_pack(nl.z, nl.w) : f2_pack(nl.x, nl.y)),
+                        z0, z1);
+              z0 = ex2_approx(z0);
+              z1 = ex2_approx(z1);
+              sv[q][c] = __float_as_uint(z0);
+              sv[q][c + 1] = __float_as_uint(z1);
+              pk[c >> 1] = T::pack(z0, z1);
+            }
+          }
+          if (!all) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) pk[k] = keep(pk[k], seen[q], k);
+          }
+          tmem_st_x16_nowait(sp + static_cast<uint32_t>(q * 16), pk);
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&p_full[w]);
+        ok = mbar_wait_warp(&dp_full[w], gw & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t dv[2][32];
+        tmem_ld_32x32b_x32_nowait(sp + 64u, dv[0]);
+        tmem_ld_32x32b_x32_nowait(sp + 96u, dv[1]);
+        tmem_wait_ld_dep(dv[0]);
+        tmem_wait_ld_dep(dv[1]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          uint32_t dk[16];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
             const float4 nd = ld_shared_f4(stat4 + static_cast<uint32_t>((16 + q * 8 + k) * 16));
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int c = 4 * k + 2 * e;
-              const uint64_t l2 = e ? f2_pack(nl.z, nl.w) : f2_pack(nl.x, nl.y);
-              const uint64_t d2 = e ? f2_pack(nd.z, nd.w) : f2_pack(nd.x, nd.y);
-              float z0, z1, g0, g1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[q][c]), __uint_as_float(sv[q][c + 1])),
-                               scale2, l2),
-                        z0, z1);
-              const float e0 = ex2_approx(z0), e1 = ex2_approx(z1);
-              f2_unpack(f2_mul(f2_pack(e0, e1),
-                               f2_add(f2_pack(__uint_as_float(dv[q][c]),
-                                              __uint_as_float(dv[q][c + 1])),
-                                      d2)),
+              float g0, g1;
+              f2_unpack(f2_mul(f2_pack(__uint_as_float(sv[q][c]), __uint_as_float(sv[q][c + 1])),
+                               f2_add(f2_pack(__uint_as_float(dv[q][c]), __uint_as_float(dv[q][c + 1])),
+                                      e ? f2_pack(nd.z, nd.w) : f2_pack(nd.x, nd.y))),
                         g0, g1);
-              pk[c >> 1] = T::pack(e0, e1);
               dk[c >> 1] = T::pack(g0, g1);
             }
           }
           if (!all) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const uint32_t two = (seen >> (2 * k)) & 3u;
-              const uint32_t keep = (two & 1u ? 0x0000FFFFu : 0u) | (two & 2u ? 0xFFFF0000u : 0u);
-              pk[k] &= keep;
-              dk[k] &= keep;
-            }
+            for (int k = 0; k < 16; ++k) dk[k] = keep(dk[k], seen[q], k);
           }
-          tmem_st_x16_nowait(sp + static_cast<uint32_t>(q * 16), pk);
           tmem_st_x16_nowait(sp + 64u + static_cast<uint32_t>(q * 16), dk);
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&p_full[w]);
+        mbar_arrive(&ds_full[w]);
         ++gw;
       }
       if (!ok) break;
@@ -583,7 +616,7 @@ struct DqCfg {
   static constexpr int kOffKV = 4 * kTileBytes;
   static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;  // [8 warps] 2 KB, dq rows
   static constexpr int kOffBar = kOffStage + 8 * 2048;
-  static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 2 + 2 + 2 + 2 + 1;
+  static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 2 + 2 + 2 + 2 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
 };
@@ -614,8 +647,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   uint64_t* q_empty = q_full + 2;           // [2] last products of the tile's rows done -> TMA
   uint64_t* kv_full = q_empty + 2;          // [kSlots]
   uint64_t* kv_empty = kv_full + C::kSlots; // [kSlots]
-  uint64_t* s_full = kv_empty + C::kSlots;  // [2] S and dP of a chunk in TMEM
-  uint64_t* p_full = s_full + 2;            // [2] dS written (128 arrivals)
+  uint64_t* s_full = kv_empty + C::kSlots;  // [2] S of a chunk in TMEM
+  uint64_t* dp_full = s_full + 2;           // [2] dP of a chunk in TMEM
+  uint64_t* p_full = dp_full + 2;           // [2] dS written (128 arrivals)
   uint64_t* o_done = p_full + 2;            // [2] dq product of a chunk completed
   uint64_t* o_empty = o_done + 2;           // [2] dq read by the epilogue (128 arrivals)
   uint64_t* drain_bar = o_empty + 2;
@@ -630,6 +664,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       mbar_init(&q_full[w], 1);
       mbar_init(&q_empty[w], 1);
       mbar_init(&s_full[w], 1);
+      mbar_init(&dp_full[w], 1);
       mbar_init(&p_full[w], 128);
       mbar_init(&o_done[w], 1);
       mbar_init(&o_empty[w], 128);
@@ -757,6 +792,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             umma_bf16(d, desc_from_words(qa + ao, hi), desc_from_words(kb + bo, hi), idesc_s,
                       k > 0 ? 1u : 0u);
           }
+          umma_commit(&s_full[w]);
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4);
@@ -764,7 +800,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
             umma_bf16(d + 64u, desc_from_words(oa + ao, hi), desc_from_words(vb + bo, hi), idesc_s,
                       k > 0 ? 1u : 0u);
           }
-          umma_commit(&s_full[w]);
+          umma_commit(&dp_full[w]);
           if (end) umma_commit(&q_empty[w]);
         }
         __syncwarp();
@@ -868,44 +904,52 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         ok = mbar_wait_warp(&s_full[w], gc & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
         if (!ok) break;
         tc_fence_after();
-        uint32_t sv[kCB][32], dv[kCB][32];
+        const bool full = chunk_full<kCB>(p.s, it, it.t0(w), it.t1(w), c);
+        uint32_t seen[kCB];
+        uint32_t sv[kCB][32];  // S, then P in fp32, formed while dP is computed
 #pragma unroll
-        for (int i = 0; i < kCB; ++i) {
-          if (i < nb) {
-            tmem_ld_32x32b_x32_nowait(sp + static_cast<uint32_t>(i * kBlk), sv[i]);
-            tmem_ld_32x32b_x32_nowait(sp + 64u + static_cast<uint32_t>(i * kBlk), dv[i]);
-          }
-        }
+        for (int i = 0; i < kCB; ++i)
+          if (i < nb) tmem_ld_32x32b_x32_nowait(sp + static_cast<uint32_t>(i * kBlk), sv[i]);
 #pragma unroll
         for (int i = 0; i < kCB; ++i) {
           if (i < nb) {
             tmem_wait_ld_dep(sv[i]);
-            tmem_wait_ld_dep(dv[i]);
+            if (!full) {
+              seen[i] = seen_bits(p.s, it.r, c * kCB + i, pos, it.kv_len);
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (!((seen[i] >> k) & 1u)) sv[i][k] = 0xFF800000u;  // P = 0
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              float z0, z1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[i][2 * k]), __uint_as_float(sv[i][2 * k + 1])),
+                               scale2, l2),
+                        z0, z1);
+              sv[i][2 * k] = __float_as_uint(ex2_approx(z0));
+              sv[i][2 * k + 1] = __float_as_uint(ex2_approx(z1));
+            }
           }
         }
-        const bool full = chunk_full<kCB>(p.s, it, it.t0(w), it.t1(w), c);
+        ok = mbar_wait_warp(&dp_full[w], gc & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll
         for (int i = 0; i < kCB; ++i) {
           if (i < nb) {
+            uint32_t dv[32];
+            tmem_ld_32x32b_x32(sp + 64u + static_cast<uint32_t>(i * kBlk), dv);
             if (!full) {
-              const uint32_t seen = seen_bits(p.s, it.r, c * kCB + i, pos, it.kv_len);
 #pragma unroll
               for (int k = 0; k < 32; ++k)
-                if (!((seen >> k) & 1u)) {
-                  sv[i][k] = 0xFF800000u;  // P = 0
-                  dv[i][k] = 0u;
-                }
+                if (!((seen[i] >> k) & 1u)) dv[k] = 0u;  // of a key that may hold anything
             }
             uint32_t pk[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              float z0, z1, g0, g1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(sv[i][2 * k]), __uint_as_float(sv[i][2 * k + 1])),
-                               scale2, l2),
-                        z0, z1);
-              const uint64_t e2 = f2_pack(ex2_approx(z0), ex2_approx(z1));
-              const uint64_t g2 =
-                  f2_pack(__uint_as_float(dv[i][2 * k]), __uint_as_float(dv[i][2 * k + 1]));
+              float g0, g1;
+              const uint64_t e2 = f2_pack(__uint_as_float(sv[i][2 * k]), __uint_as_float(sv[i][2 * k + 1]));
+              const uint64_t g2 = f2_pack(__uint_as_float(dv[2 * k]), __uint_as_float(dv[2 * k + 1]));
               psum[k & 1] = f2_fma(e2, g2, psum[k & 1]);
               f2_unpack(f2_mul(e2, f2_add(g2, d2)), g0, g1);
               pk[k] = T::pack(g0, g1);
