@@ -47,11 +47,11 @@ struct FwdCfg {
   static constexpr int kHalves = D / 64;
   static constexpr int kTileBytes = kRows * D * 2;
   static constexpr int kSlotBytes = kCB * kBlk * D * 2;
-  static constexpr int kSlots = 8;  // 8 stages of one slot (K = V) or 4 of two (K, V)
+  static constexpr int kSlots = 6;  // 6 stages of one slot (K = V) or 3 of two (K, V)
   static constexpr int kOffQ = 0;
   static constexpr int kOffKV = 2 * kTileBytes;
-  static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;  // [8 warps] 2 KB, out rows
-  static constexpr int kOffBar = kOffStage + 8 * 2048;
+  static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;  // [2] tiles of results
+  static constexpr int kOffBar = kOffStage + 2 * kTileBytes;
   static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 4 + 4 + 4 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
@@ -62,7 +62,6 @@ struct FwdParams {
   TileGrid grid;
   float scale_log2;
   const float* sink;    // [h] or null
-  uint16_t* out;        // [batch, m, h, D]
   float* lse;           // [batch, m, h] or null
   int shared;           // K and V are one tensor
   unsigned int* err;
@@ -71,7 +70,8 @@ struct FwdParams {
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     window_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
-                      const __grid_constant__ CUtensorMap tm_v, const FwdParams p) {
+                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_out,
+                      const FwdParams p) {
   using C = FwdCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -115,6 +115,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tma_prefetch_desc(&tm_q);
     tma_prefetch_desc(&tm_k);
     tma_prefetch_desc(&tm_v);
+    tma_prefetch_desc(&tm_out);
   }
   if (warp == 1) {
     tmem_alloc(tmem_holder, kTmemCols);
@@ -325,7 +326,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t st = tmem + lane_off + static_cast<uint32_t>(w * 256);
     const uint32_t od = st + 128u;
-    const uint32_t stage = smem_u32(smem + C::kOffStage) + static_cast<uint32_t>((warp - 4) * 2048);
+    uint8_t* stage = smem + C::kOffStage + w * C::kTileBytes;
+    const uint32_t stage_row = smem_u32(stage) + static_cast<uint32_t>(row * 128);
+    const uint32_t bar = 1 + static_cast<uint32_t>(w);
+    const bool leader = quarter == 0 && lane == 0;  // issues the tile's stores
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int gc = 0;  // chunks processed (all items)
     bool ok = true;
@@ -430,9 +434,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&p_full[2 * w + buf]);
         ++gc;
       }
-      if (!ok) break;
-      // ---- epilogue: O / (l + sink term), both relative to the larger of the reference
-      // and the sink
+      // ---- epilogue. The previous item's rows have left the staging buffer; a warpgroup
+      // leaves together, since it meets at barriers
+      if (leader) bulk_wait_group_read<0>();
+      if (!named_bar_and(bar, 128, ok)) break;
+      if (last >= 0) {
+        // a wait that runs out here ends the loop at the next item's barrier
+        ok = mbar_wait_warp(&o_done[2 * w + ((gc - 1) & 1)], ((gc - 1) >> 1) & 1, abort_flag, p.err,
+                            DSA_DEVERR_WIN_WAIT);
+        tc_fence_after();
+      }
+      // O / (l + sink term), both relative to the larger of the reference and the sink
       const float sink2 =
           p.sink != nullptr && tok < p.grid.tt ? __ldg(p.sink + gh) * kLog2e : -INFINITY;
       const float top = fmaxf(m, sink2);
@@ -440,32 +452,46 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float mine = ex2_approx(m - ref);  // 0 when no key was seen
       const float total = fmaf(l, mine, ex2_approx(sink2 - ref));
       const float inv = total == 0.f ? 0.f : mine / total;
-      const int64_t orow = (static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + gh;
-      if (last >= 0) {
-        ok = mbar_wait_warp(&o_done[2 * w + ((gc - 1) & 1)], ((gc - 1) >> 1) & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
-        if (!ok) break;
-        tc_fence_after();
-      }
-      // the row is rounded as it is read, so that O is given back before the stores
-      uint32_t x[D / 32][16];
 #pragma unroll
-      for (int q = 0; q < D / 32; ++q) {
-        uint32_t ov[32];
-        if (last >= 0) tmem_ld_32x32b_x32(od + static_cast<uint32_t>(q * 32), ov);
+      for (int half = 0; half < C::kHalves; ++half) {
+        uint32_t ov[2][32];
+        if (last >= 0) {
+          tmem_ld_32x32b_x32_nowait(od + static_cast<uint32_t>(half * 64), ov[0]);
+          tmem_ld_32x32b_x32_nowait(od + static_cast<uint32_t>(half * 64 + 32), ov[1]);
+          tmem_wait_ld_dep(ov[0]);
+          tmem_wait_ld_dep(ov[1]);
+          if (half == C::kHalves - 1) {
+            tc_fence_before();
+            mbar_arrive(&o_empty[w]);
+          }
+        }
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
-          x[q][k] = last < 0 ? 0u
-                             : T::pack(__uint_as_float(ov[2 * k]) * inv, __uint_as_float(ov[2 * k + 1]) * inv);
-      }
-      if (last >= 0) {
-        tc_fence_before();
-        mbar_arrive(&o_empty[w]);
-      }
+        for (int j = 0; j < 8; ++j) {
+          uint32_t x[4];
 #pragma unroll
-      for (int q = 0; q < D / 32; ++q)
-        store_rows(stage, x[q], valid ? p.out + orow * D + q * 32 : nullptr, lane);
-      if (valid && p.lse != nullptr) p.lse[orow] = (ref + log2f(total)) * kLn2;
+          for (int u = 0; u < 4; ++u) {
+            const int k = (j & 3) * 8 + 2 * u;
+            x[u] = last < 0 ? 0u
+                            : T::pack(__uint_as_float(ov[j >> 2][k]) * inv,
+                                      __uint_as_float(ov[j >> 2][k + 1]) * inv);
+          }
+          st_shared_v4(stage_row + static_cast<uint32_t>(half * kBoxBytes) +
+                           ((static_cast<uint32_t>(j) ^ static_cast<uint32_t>(row & 7)) << 4),
+                       x[0], x[1], x[2], x[3]);
+        }
+      }
+      fence_proxy_async_smem();
+      named_bar_sync(bar, 128);
+      if (leader && it.t1(w) > it.t0(w)) {
+#pragma unroll
+        for (int half = 0; half < C::kHalves; ++half)
+          tma_store_4d(&tm_out, stage + half * kBoxBytes, half * 64, it.kvh * p.s.g, it.t0(w), it.b);
+        bulk_commit_group();
+      }
+      if (valid && p.lse != nullptr)
+        p.lse[(static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + gh] = (ref + log2f(total)) * kLn2;
     }
+    if (leader) bulk_wait_group<0>();
   }
 
   __syncwarp();
@@ -493,20 +519,27 @@ int launch_fwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   if (!tile_grid(s, batch, &p.grid)) return DSA_ERR_UNSUPPORTED;
   p.scale_log2 = scale * kLog2e;
   p.sink = sink;
-  p.out = static_cast<uint16_t*>(out);
   p.lse = lse;
   p.shared = x.v == x.k && same_strides(x.vs, x.ks);
   p.err = err;
-  CUtensorMap tm_q, tm_k, tm_v;
+  CUtensorMap tm_q, tm_k, tm_v, tm_out;
   st = map_rows_by_head(&tm_q, T::kFmt, x.q, x.qs, batch, s.m, s.h, D, s.g, p.grid.tt);
   if (st == DSA_OK) st = map_head_by_rows(&tm_k, T::kFmt, x.k, x.ks, batch, s.n, s.hk, D, kBlk);
   if (st == DSA_OK) st = map_head_by_rows(&tm_v, T::kFmt, x.v, x.vs, batch, s.n, s.hk, D, kBlk);
+  if (st == DSA_OK) {
+    Strides os;
+    os.h = D;
+    os.t = static_cast<int64_t>(s.h) * D;
+    os.b = os.t * s.m;
+    st = map_rows_by_head(&tm_out, T::kFmt, out, os, batch, s.m, s.h, D, s.g, p.grid.tt);
+  }
   if (st != DSA_OK) return st;
   auto kernel = window_fwd_kernel<T, D>;
   st = set_max_dynamic_smem(reinterpret_cast<const void*>(kernel), C::kSmemBytes);
   if (st != DSA_OK) return st;
   const int grid = p.grid.items < di.num_sms ? p.grid.items : di.num_sms;
-  kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmemBytes, stream>>>(tm_q, tm_k, tm_v, p);
+  kernel<<<static_cast<unsigned>(grid), kThreads, C::kSmemBytes, stream>>>(tm_q, tm_k, tm_v, tm_out,
+                                                                              p);
   return cuda_status(cudaGetLastError());
 }
 
