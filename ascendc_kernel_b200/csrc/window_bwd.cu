@@ -33,35 +33,51 @@ constexpr int kStream = 64;           // rows of a streamed tile (dkv)
 constexpr int kHalfBox = kStream * 128;  // one [64 rows x 64 columns] SW128 box
 
 // ------------------------------------------------------------------ row statistics
-// stat[row] = (-lse log2 e, -D); D / 8 threads a row, 16-byte loads.
-template <typename T, int D>
+// stat[row] = (-lse log2 e, -D); D / 8 threads a row, each with kStatRows rows' 16-byte
+// loads in flight (one row a thread reached 4.3 TB/s). Flat: dout is contiguous like out.
+constexpr int kStatRows = 4;
+
+template <typename T, int D, bool Flat>
 __global__ void __launch_bounds__(256) window_stat_kernel(const uint16_t* out, const uint16_t* dout,
                                                           Strides ds, const float* lse, float2* stat,
                                                           int64_t rows, int m, int h) {
   constexpr int kLanes = D / 8;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * (256 / kLanes) + threadIdx.x / kLanes;
+  constexpr int kStep = 256 / kLanes;  // rows of a block at once
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kStep * kStatRows) + threadIdx.x / kLanes;
   const int x = threadIdx.x % kLanes;
-  float sum = 0.f;
-  if (row < rows) {
-    const int64_t bt = row / h;
-    const int head = static_cast<int>(row - bt * h);
-    const int64_t b = bt / m;
-    const int64_t t = bt - b * m;
-    const uint4 a = *reinterpret_cast<const uint4*>(out + row * D + x * 8);
-    const uint4 g = *reinterpret_cast<const uint4*>(dout + b * ds.b + t * ds.t + head * ds.h + x * 8);
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w};
+  uint4 a[kStatRows], g[kStatRows];
+#pragma unroll
+  for (int r = 0; r < kStatRows; ++r) {
+    const int64_t row = row0 + r * kStep;
+    a[r] = g[r] = make_uint4(0u, 0u, 0u, 0u);
+    if (row < rows) {
+      int64_t at = row * D;
+      a[r] = __ldcs(reinterpret_cast<const uint4*>(out + at + x * 8));
+      if (!Flat) {
+        const int64_t bt = row / h;
+        const int64_t b = bt / m;
+        at = b * ds.b + (bt - b * m) * ds.t + (row - bt * h) * ds.h;
+      }
+      g[r] = *reinterpret_cast<const uint4*>(dout + at + x * 8);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kStatRows; ++r) {
+    const int64_t row = row0 + r * kStep;
+    const uint32_t aw[4] = {a[r].x, a[r].y, a[r].z, a[r].w}, gw[4] = {g[r].x, g[r].y, g[r].z, g[r].w};
+    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       sum = fmaf(T::lo(aw[i]), T::lo(gw[i]), sum);
       sum = fmaf(T::hi(aw[i]), T::hi(gw[i]), sum);
     }
-  }
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-  if (row < rows && x == 0) {
-    const float l = lse[row];
-    // a row that sees nothing has no weights: 2^(s - inf) = 0
-    stat[row] = make_float2(l == -INFINITY ? -INFINITY : -l * kLog2e, -sum);
+    for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    if (row < rows && x == 0) {
+      const float l = lse[row];
+      // a row that sees nothing has no weights: 2^(s - inf) = 0
+      stat[row] = make_float2(l == -INFINITY ? -INFINITY : -l * kLog2e, -sum);
+    }
   }
 }
 
@@ -565,16 +581,19 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
   }
 }
 
-// Sums the parts of the key tiles with several units, in the order of the parts;
-// a thread four columns of a key.
+// Sums the parts of the key tiles with several units, in a fixed order: eight lanes take
+// every eighth part of four columns of a key, then their sums are added in lane order.
+// (One thread for all parts took 25 us where the first tokens' tile had 75 of them.)
 template <typename T, int D>
 __global__ void __launch_bounds__(256) window_join_kernel(const DkvParams p, int64_t batch) {
   const bool two = p.split > 1;  // all key tiles have parts, else only the first ones
   const int tiles = two ? p.key_tiles : p.first_tiles;
   const int kinds = p.dv == nullptr ? 1 : 2;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int col = static_cast<int>(i % (D / 4)) * 4;
-  int64_t x = i / (D / 4);
+  // a warp: 8 parts x 16 columns of one key
+  const int lane = threadIdx.x & 31;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+  const int col = static_cast<int>(i % (D / 16)) * 16 + (lane & 3) * 4;
+  int64_t x = i / (D / 16);
   const int row = static_cast<int>(x % kRows);
   x /= kRows;
   const int kind = static_cast<int>(x % kinds);
@@ -591,7 +610,8 @@ __global__ void __launch_bounds__(256) window_join_kernel(const DkvParams p, int
                               : static_cast<int64_t>(p.first_tiles) * p.split_first +
                                     static_cast<int64_t>(kt - p.first_tiles) * p.split);
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < parts; ++s) {
+#pragma unroll 4
+  for (int s = lane >> 2; s < parts; s += 8) {
     const float4 v = *reinterpret_cast<const float4*>(
         p.parts + (((unit + s) * kinds + kind) * kRows + row) * D + col);
     sum.x += v.x;
@@ -599,6 +619,14 @@ __global__ void __launch_bounds__(256) window_join_kernel(const DkvParams p, int
     sum.z += v.z;
     sum.w += v.w;
   }
+#pragma unroll
+  for (int o = 16; o >= 4; o >>= 1) {
+    sum.x += __shfl_down_sync(0xFFFFFFFFu, sum.x, o);
+    sum.y += __shfl_down_sync(0xFFFFFFFFu, sum.y, o);
+    sum.z += __shfl_down_sync(0xFFFFFFFFu, sum.z, o);
+    sum.w += __shfl_down_sync(0xFFFFFFFFu, sum.w, o);
+  }
+  if (lane >= 4) return;
   const int64_t b = bh / p.s.hk;
   uint16_t* out = kind ? p.dv : p.dk;
   *reinterpret_cast<uint2*>(out + ((b * p.s.n + key) * p.s.hk + (bh - b * p.s.hk)) * D + col) =
@@ -1007,7 +1035,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 // ------------------------------------------------------------------ dsink
 // Column sums of sink_rows [rows, h] in two fixed-order steps: blocks of
 // kSinkRows rows, then the blocks. A block holds 32 heads x 8 row lanes.
-constexpr int kSinkRows = 512;
+constexpr int kSinkRows = 256;
 
 __global__ void __launch_bounds__(256) window_dsink_kernel(const float* in, float* out, int64_t rows,
                                                            int h, float sign) {
@@ -1017,8 +1045,10 @@ __global__ void __launch_bounds__(256) window_dsink_kernel(const float* in, floa
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * kSinkRows;
   const int64_t r1 = r0 + kSinkRows < rows ? r0 + kSinkRows : rows;
   float sum = 0.f;
-  if (head < h)
+  if (head < h) {
+#pragma unroll 8
     for (int64_t r = r0 + y; r < r1; r += 8) sum += in[r * h + head];
+  }
   part[y][threadIdx.x & 31] = sum;
   __syncthreads();
   if (y == 0 && head < h) {
@@ -1093,10 +1123,12 @@ int launch_bwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   float* sink_rows = reinterpret_cast<float*>(ws + b.off_rows);
   float* sink_sum = reinterpret_cast<float*>(ws + b.off_sum);
   if (rows > 0) {
-    window_stat_kernel<T, D>
-        <<<static_cast<unsigned>(div_up(rows, 256 / (D / 8))), 256, 0, stream>>>(
-            static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(dout), dos, lse, stat,
-            rows, s.m, s.h);
+    const bool flat = dos.h == D && dos.t == static_cast<int64_t>(s.h) * D &&
+                      (batch == 1 || dos.b == dos.t * s.m);
+    auto kernel = flat ? window_stat_kernel<T, D, true> : window_stat_kernel<T, D, false>;
+    kernel<<<static_cast<unsigned>(div_up(rows, 256 / (D / 8) * kStatRows)), 256, 0, stream>>>(
+        static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(dout), dos, lse, stat, rows,
+        s.m, s.h);
     st = cuda_status(cudaGetLastError());
     if (st != DSA_OK) return st;
   }
@@ -1136,8 +1168,8 @@ int launch_bwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
     if (st != DSA_OK) return st;
     const int tiles = b.split > 1 ? b.key_tiles : (b.split_first > 1 ? b.first_tiles : 0);
     if (tiles > 0) {
-      const int64_t work = batch * s.hk * tiles * (dv ? 2 : 1) * kRows * (D / 4);
-      window_join_kernel<T, D><<<static_cast<unsigned>(div_up(work, 256)), 256, 0, stream>>>(p, batch);
+      const int64_t warps = batch * s.hk * tiles * (dv ? 2 : 1) * kRows * (D / 16);
+      window_join_kernel<T, D><<<static_cast<unsigned>(div_up(warps, 8)), 256, 0, stream>>>(p, batch);
       st = cuda_status(cudaGetLastError());
       if (st != DSA_OK) return st;
     }
