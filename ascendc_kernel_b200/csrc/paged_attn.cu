@@ -17,12 +17,12 @@
 // Heads are the N side of the products (S^T = K Q^T, O^T += V^T P^T): a group of
 // 8 heads costs a few columns and not a 128-row tile, and a thread owns one KEY:
 // its visibility is one flag, its weights of all heads lie in its registers.
-//   warp 0      TMA: pages -> ring of 128-row slots (K, V; one slot a chunk when they
-//               are one tensor), in granules of 8, 16 or 32 rows that never cross a
-//               page; rows of q
-//   warp 1      tcgen05 issuer
+//   warps 0, 3  TMA: pages -> rings of 128-row slots, K and q by warp 0, V by warp 3 (one
+//               ring for both when they are one tensor), in granules of 8, 16 or 32
+//               rows that never cross a page
+//   warps 1, 2  tcgen05 issuers: S^T and O^T
 //   warps 4..11 softmax: warpgroup w takes the chunks of parity w, with its own
-//               accumulator, reference and sums; S^T products run up to three chunks ahead
+//               accumulator, reference and sums; S^T products run up to four chunks ahead
 // The reference of a head is the score of a warpgroup's first visible key of a
 // piece and moves (O and the sums are rescaled) only when a score exceeds it by more
 // than 2^14, so the common chunk needs one vote and no reduction over keys; the sums
@@ -56,7 +56,8 @@ struct Cfg {
   static constexpr int kSlotBytes = kKeys * D * 2;
   static constexpr int kSlots = (NM == 128 ? 3 : 5) * (128 / D);
   static constexpr int kSBufs = NM == 128 ? 2 : 4;  // S^T products that may run ahead
-  static constexpr int kLag = kSBufs - 1;           // O^T of chunk i - kLag after S^T of i
+  static constexpr int kSlotsK = kSlots / 2;        // of them K's; V has the others
+  static constexpr int kSlotsV = kSlots - kSlotsK;
   static constexpr int kQBytes = NM * D * 2;
   static constexpr int kPBytes = kKeys * (NM < 64 ? 64 : NM) * 2;  // [128 keys x 64 heads] boxes
   static constexpr int kOffQ = 0;
@@ -68,20 +69,11 @@ struct Cfg {
   static constexpr int kOffRef = kOffMax + 2 * 4 * NM * 4;    // [2][2: reference, step][NM]
   static constexpr int kOffMeta = kOffRef + 2 * 2 * NM * 4;   // [16 chunks][16] granule states
   static constexpr int kOffBar = kOffMeta + 16 * 16 * 4;
-  static constexpr int kNumBars = 2 + 2 * kSlots + kSBufs + 2 + 2 + 2 + 2 + 1;
+  static constexpr int kNumBars = 2 + 2 * kSlots + 2 * kSBufs + 2 + 2 + 2 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 48 + 1024;
   static constexpr int kColsO = kSBufs * NM;                  // TMEM: S^T buffers, then O^T
   static constexpr uint32_t kTmemCols = kColsO + 2 * NM <= 256 ? 256 : 512;
-
-  // V is loaded kLag chunks behind K, in the order in which the products use them, so a
-  // slot is given back soon after its data arrived. Slot of chunk i's V, of n chunks: the
-  // loads run K(0) .. K(kLag - 1), then K(i), V(i - kLag) in turn, then the last V.
-  static __device__ __forceinline__ int slot_v(bool shared, int i, int n) {
-    const int64_t x = shared ? i : 2 * static_cast<int64_t>(i) + kLag + 1;
-    const int64_t y = static_cast<int64_t>(n) + i;
-    return static_cast<int>((x < y ? x : y) % kSlots);
-  }
 };
 
 struct Params {
@@ -233,7 +225,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* kv_full = q_empty + 1;            // [kSlots]
   uint64_t* kv_empty = kv_full + C::kSlots;   // [kSlots]
   uint64_t* s_full = kv_empty + C::kSlots;    // [kSBufs] S^T of a chunk in TMEM
-  uint64_t* p_full = s_full + C::kSBufs;      // [2] P written (128 arrivals)
+  uint64_t* s_empty = s_full + C::kSBufs;     // [kSBufs] its scores are read (128 arrivals)
+  uint64_t* p_full = s_empty + C::kSBufs;     // [2] P written (128 arrivals)
   uint64_t* o_done = p_full + 2;              // [2] O^T product of a chunk completed
   uint64_t* o_empty = o_done + 2;             // [2] O^T read at a piece's end (128 arrivals)
   uint64_t* v_ready = o_empty + 2;            // [2] V of the warpgroup's chunk has arrived
@@ -255,14 +248,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&kv_full[s], 1);
       mbar_init(&kv_empty[s], 1);
     }
-    for (int i = 0; i < C::kSBufs; ++i) mbar_init(&s_full[i], 1);
+    for (int i = 0; i < C::kSBufs; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&s_empty[i], 128);
+    }
     for (int w = 0; w < 2; ++w) {
       mbar_init(&p_full[w], 128);
       mbar_init(&o_done[w], 1);
       mbar_init(&o_empty[w], 128);
       mbar_init(&v_ready[w], 1);
     }
-    mbar_init(drain_bar, 1);
+    mbar_init(drain_bar, 2);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&tm_q);
@@ -331,71 +327,49 @@ __global__ void __launch_bounds__(kThreads, 1)
   wk.kvh = walk_s[1];
   wk.c0 = walk_s[2];
   wk.left = walk_s[3];
-  const int chunks = wk.left;  // of the whole stretch
+  // slots of the ring that chunks take in turn: K's (or both), and V's behind them
+  const int ring_k = p.shared ? C::kSlots : C::kSlotsK;
 
   if (warp < 4) {
     win::set_max_regs_dec<kRegsAux>();
-    if (warp == 0) {
-      // ---------------------------------------------------------- producer
-      Ring<C::kSlots> at;
-      int gc = 0, loads = 0, pieces = 0;
+    if (warp == 0 || (warp == 3 && !p.shared)) {
+      // ---------------------------------------------------------- producers: K (and q), V
+      const bool is_v = warp == 3;
+      const CUtensorMap* tm = is_v ? &tm_v : &tm_k;
+      const int slot0 = is_v ? C::kSlotsK : 0, slots = is_v ? C::kSlotsV : ring_k;
+      Ring<0> at;
+      int gc = 0, pieces = 0;
       bool ok = true;
-      // a lane's granule of a chunk: its page (-1: none), first slot of it, kv head
-      struct Gran {
-        int page, slot, kvh;
-      };
-      Gran late[C::kLag];  // of the chunks whose V is not yet requested
-      auto load = [&](const CUtensorMap* tm, const Gran& g, bool mine, int gi, int bytes) -> bool {
-        if (!mbar_wait_warp(&kv_empty[at.slot], at.parity ^ 1u, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
-          return false;
-        if (lane == 0) mbar_arrive_expect_tx(&kv_full[at.slot], static_cast<uint32_t>(bytes));
-        __syncwarp();
-        if (mine && g.page >= 0) {
-          uint8_t* dst = smem + C::kOffKV + at.slot * C::kSlotBytes + gi * p.gran * 128;
-#pragma unroll
-          for (int half = 0; half < C::kHalves; ++half)
-            tma_load_4d(dst + half * kBox, tm, half * 64, g.slot, g.kvh, g.page, &kv_full[at.slot]);
-        }
-        at.next();
-        ++loads;
-        return true;
-      };
       // a lane per granule of the next `ahead` chunks: their pages are looked up while the
       // copies of the chunks before them are waited for
       const int ahead = 32 / gpc;
       const int sub = lane / gpc, gi = lane - sub * gpc;
-      const int gran_bytes = p.gran * D * 2;
-      // V of chunk gc - kLag: lanes keep their entry of every chunk (page -1 for a chunk
-      // of another lane group), so each copy is issued by the lane that looked it up
-      auto shift = [&](const Gran& g) {
-#pragma unroll
-        for (int i = C::kLag - 1; i > 0; --i) late[i] = late[i - 1];
-        late[0] = g;
-      };
       for (; ok && walk_take(p, wk); walk_next(wk), ++pieces) {
-        ok = mbar_wait_warp(q_empty, (pieces & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
-        if (!ok) break;
-        if (lane == 0) {
-          mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.g * D * 2));
+        if (!is_v) {
+          ok = mbar_wait_warp(q_empty, (pieces & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+          if (!ok) break;
+          if (lane == 0) {
+            mbar_arrive_expect_tx(q_full, static_cast<uint32_t>(p.g * D * 2));
 #pragma unroll
-          for (int half = 0; half < C::kHalves; ++half)
-            tma_load_3d(smem + C::kOffQ + half * NM * 128, &tm_q, half * 64, wk.kvh * p.g, wk.b,
-                        q_full);
+            for (int half = 0; half < C::kHalves; ++half)
+              tma_load_3d(smem + C::kOffQ + half * NM * 128, &tm_q, half * 64, wk.kvh * p.g, wk.b,
+                          q_full);
+          }
         }
-        int page = -1, slot = 0, next_page = -1, next_slot = 0;
+        int page = -1, row = 0, next_page = -1, next_row = 0;
         auto look = [&](int c) {
-          const int row = gran_row(p, wk.s, (c + sub) * gpc + gi);
-          const int i = row / p.page;
-          next_slot = row - i * p.page;
-          next_page = c + sub < wk.c1 && row < wk.s.len
+          const int r = gran_row(p, wk.s, (c + sub) * gpc + gi);
+          const int i = r / p.page;
+          next_row = r - i * p.page;
+          next_page = c + sub < wk.c1 && r < wk.s.len
                           ? __ldg(p.table + static_cast<int64_t>(wk.b) * p.max_pages + i)
                           : -2;  // nothing to read
         };
         look(wk.c0);
-        for (int c = wk.c0, turn = 0; ok && c < wk.c1; ++c, ++gc, turn = turn + 1 == ahead ? 0 : turn + 1) {
+        for (int c = wk.c0, turn = 0; c < wk.c1; ++c, ++gc, turn = turn + 1 == ahead ? 0 : turn + 1) {
           if (turn == 0) {
             page = next_page;
-            slot = next_slot;
+            row = next_row;
             if (page != -2 && (page < 0 || page >= p.num_pages)) {
               atomicOr(p.err, DSA_DEVERR_CACHE);
               page = -1;
@@ -403,38 +377,31 @@ __global__ void __launch_bounds__(kThreads, 1)
             look(c + ahead);
           }
           const bool mine = sub == turn;
-          const Gran g = {mine ? max(page, -1) : -1, slot, wk.kvh};
-          const uint32_t live = __ballot_sync(0xFFFFFFFFu, g.page >= 0);
-          if (mine) meta[(gc & 15) * 16 + gi] = g.page >= 0 ? 1 : 0;
+          const bool live = mine && page >= 0;
+          const int bytes = __popc(__ballot_sync(0xFFFFFFFFu, live)) * p.gran * D * 2;
+          const int s = slot0 + at.slot;
+          ok = mbar_wait_warp(&kv_empty[s], at.parity ^ 1u, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+          if (!ok) break;
+          // the granules' states: the ring of 16 is longer than any chunk is ahead
+          if (mine && !is_v) meta[(gc & 15) * 16 + gi] = live ? 1 : 0;
           __syncwarp();
-          ok = load(&tm_k, g, mine, gi, __popc(live) * gran_bytes);
-          if (ok && !p.shared) {
-            if (gc >= C::kLag) {
-              const Gran& v = late[C::kLag - 1];
-              const uint32_t l = __ballot_sync(0xFFFFFFFFu, v.page >= 0);
-              ok = load(&tm_v, v, true, gi, __popc(l) * gran_bytes);
-            }
-            shift(g);
-          }
-        }
-      }
-      if (ok && !p.shared) {
-        // the last chunks' V
-        const int rest = min(gc, C::kLag);
+          if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], static_cast<uint32_t>(bytes));
+          __syncwarp();
+          if (live) {
+            uint8_t* dst = smem + C::kOffKV + s * C::kSlotBytes + gi * p.gran * 128;
 #pragma unroll
-        for (int i = C::kLag - 1; i >= 0; --i) {
-          if (i < rest && ok) {
-            const uint32_t l = __ballot_sync(0xFFFFFFFFu, late[i].page >= 0);
-            ok = load(&tm_v, late[i], true, gi, __popc(l) * gran_bytes);
+            for (int half = 0; half < C::kHalves; ++half)
+              tma_load_4d(dst + half * kBox, tm, half * 64, row, wk.kvh, page, &kv_full[s]);
           }
+          at.next(slots);
         }
       }
       // copies in flight land before the CTA's shared memory goes away
-      for (int i = max(loads - C::kSlots, 0); i < loads; ++i)
-        mbar_drain(&kv_full[i % C::kSlots], static_cast<uint32_t>((i / C::kSlots) & 1));
-      if (pieces > 0) mbar_drain(q_full, (pieces - 1) & 1);
-    } else if (warp == 1) {
-      // ---------------------------------------------------------- MMA issuer
+      for (int i = max(gc - slots, 0); i < gc; ++i)
+        mbar_drain(&kv_full[slot0 + i % slots], static_cast<uint32_t>((i / slots) & 1));
+      if (!is_v && pieces > 0) mbar_drain(q_full, (pieces - 1) & 1);
+    } else if (warp == 1 || warp == 2) {
+      // ---------------------------------------------------------- MMA issuers: S^T, O^T
       // The whole warp walks and waits; one elected lane issues.
       const uint32_t idesc_s = win::make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(npad / 8) << 17);
       const uint32_t idesc_o = win::make_idesc<T>(128, 0, 1) | (1u << 15) |
@@ -447,33 +414,50 @@ __global__ void __launch_bounds__(kThreads, 1)
           smem_u32(smem + C::kOffKV), static_cast<uint32_t>(kBox), 1024u, kLayoutSW128));
       const uint32_t p_lo = static_cast<uint32_t>(make_smem_desc(
           smem_u32(smem + C::kOffP), static_cast<uint32_t>(kBox), 1024u, kLayoutSW128));
-      Ring<C::kSlots> at;       // the next slot in the order of the loads
-      Ring<C::kSlots> old;      // shared: the slot of chunk gc - kLag
+      Ring<0> at;
       int gc = 0, pieces = 0;
-      int gp[2] = {0, 0};       // O^T products issued per warpgroup
       int drained[2] = {0, 0};  // pieces of the warpgroup whose O^T was to be read
-      uint32_t fresh_bits = 0;  // bit k: chunk gc - 1 - k is its warpgroup's first of a piece
       bool ok = true;
       auto wait_warp = [&](uint64_t* b, uint32_t parity) -> bool {
         return mbar_wait_warp(b, parity, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
       };
-      auto wait_slot = [&]() -> bool {
-        return wait_warp(&kv_full[at.slot], at.parity);
-      };
-      auto issue_o = [&](int w, bool fresh) -> bool {
-        int s = old.slot;
-        if (p.shared) {
-          old.next();
-        } else {
-          if (!wait_slot()) return false;
-          s = at.slot;
-          at.next();
+      // S^T runs ahead of the softmax by up to kSBufs chunks
+      auto issue_s = [&](bool end) -> bool {
+        const int s = at.slot;
+        const uint32_t buf = static_cast<uint32_t>(gc) % C::kSBufs;
+        if (!wait_warp(&kv_full[s], at.parity) ||
+            !wait_warp(&s_empty[buf], ((static_cast<uint32_t>(gc) / C::kSBufs) & 1u) ^ 1u))
+          return false;
+        at.next(ring_k);
+        tc_fence_after();
+        const uint32_t ka = k_lo + static_cast<uint32_t>(s * (C::kSlotBytes >> 4));
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBox + (k & 3) * 32) >> 4);
+            const uint32_t bo = static_cast<uint32_t>(((k >> 2) * NM * 128 + (k & 3) * 32) >> 4);
+            umma_bf16(tmem + buf * NM, desc_from_words(ka + ao, hi), desc_from_words(q_lo + bo, hi),
+                      idesc_s, k > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[buf]);
+          if (!p.shared) umma_commit(&kv_empty[s]);
+          if (end) umma_commit(q_empty);
         }
-        if (lane == 0) mbar_arrive(&v_ready[w]);  // the softmax may clear its hidden rows
-        if (!wait_warp(&p_full[w], gp[w] & 1)) return false;
+        __syncwarp();
+        return true;
+      };
+      auto issue_o = [&](bool fresh) -> bool {
+        const int w = gc & 1;
+        const int s = p.shared ? at.slot : C::kSlotsK + at.slot;
+        // shared: the slot's data is there, since the chunk's P is made of its S^T
+        if (!p.shared && !wait_warp(&kv_full[s], at.parity)) return false;
+        if (elect_one()) mbar_arrive(&v_ready[w]);  // the softmax may clear its hidden rows
+        __syncwarp();
+        at.next(p.shared ? ring_k : C::kSlotsV);
+        if (!wait_warp(&p_full[w], (gc >> 1) & 1)) return false;
         if (fresh) {
-          if (drained[w] > 0 && !wait_warp(&o_empty[w], (drained[w] - 1) & 1)) return false;
-          ++drained[w];
+          const int d = w ? drained[1]++ : drained[0]++;
+          if (d > 0 && !wait_warp(&o_empty[w], (d - 1) & 1)) return false;
         }
         tc_fence_after();
         const uint32_t va = v_lo + static_cast<uint32_t>(s * (C::kSlotBytes >> 4));
@@ -489,41 +473,18 @@ __global__ void __launch_bounds__(kThreads, 1)
           umma_commit(&kv_empty[s]);
         }
         __syncwarp();
-        ++gp[w];
         return true;
       };
       for (; ok && walk_take(p, wk); walk_next(wk), ++pieces) {
-        ok = wait_warp(q_full, pieces & 1);
         const int n = wk.c1 - wk.c0;
-        for (int j = 0; ok && j < n; ++j, ++gc) {
-          // S^T runs ahead of the softmax: the buffer held S^T(gc - kSBufs), whose readers
-          // arrived before O^T(gc - kSBufs) was issued
-          ok = wait_slot();
-          if (!ok) break;
-          const int s = at.slot;
-          at.next();
-          tc_fence_after();
-          const uint32_t ka = k_lo + static_cast<uint32_t>(s * (C::kSlotBytes >> 4));
-          const uint32_t buf = static_cast<uint32_t>(gc) % C::kSBufs;
-          if (elect_one()) {
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k) {
-              const uint32_t ao = static_cast<uint32_t>(((k >> 2) * kBox + (k & 3) * 32) >> 4);
-              const uint32_t bo = static_cast<uint32_t>(((k >> 2) * NM * 128 + (k & 3) * 32) >> 4);
-              umma_bf16(tmem + buf * NM, desc_from_words(ka + ao, hi), desc_from_words(q_lo + bo, hi),
-                        idesc_s, k > 0 ? 1u : 0u);
-            }
-            umma_commit(&s_full[buf]);
-            if (!p.shared) umma_commit(&kv_empty[s]);
-            if (j == n - 1) umma_commit(q_empty);
-          }
-          __syncwarp();
-          if (gc >= C::kLag) ok = issue_o((gc - C::kLag) & 1, (fresh_bits >> (C::kLag - 1)) & 1u);
-          fresh_bits = (fresh_bits << 1) | (j < 2 ? 1u : 0u);
+        if (warp == 1) {
+          ok = wait_warp(q_full, pieces & 1);
+          for (int j = 0; ok && j < n; ++j, ++gc) ok = issue_s(j == n - 1);
+        } else {
+          // the first chunk of each warpgroup in the piece starts its sum anew
+          for (int j = 0; ok && j < n; ++j, ++gc) ok = issue_o(j < 2);
         }
       }
-      for (int i = max(gc - C::kLag, 0); ok && i < gc; ++i)
-        ok = issue_o(i & 1, (fresh_bits >> (gc - 1 - i)) & 1u);
       if (elect_one()) umma_commit(drain_bar);
       __syncwarp();
       mbar_drain(drain_bar, 0);
@@ -754,9 +715,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (!valid) {
-          // a hidden V row may hold anything, and 0 x NaN is NaN: it is cleared. The issuer,
-          // which waits for the slots in their order, says when V is there
-          const int sv = C::slot_v(p.shared, gc, chunks);
+          // a hidden V row may hold anything, and 0 x NaN is NaN: it is cleared. The issuer
+          // of O^T, which waits for V's slots in their order, says when it is there
+          const int sv = p.shared ? gc % C::kSlots : C::kSlotsK + gc % C::kSlotsV;
           mbar_wait(&v_ready[w], gw & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
           uint8_t* vr = smem + C::kOffKV + sv * C::kSlotBytes + key * 128;
 #pragma unroll
@@ -766,6 +727,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         fence_proxy_async_smem();
         tc_fence_before();
+        mbar_arrive(&s_empty[buf]);
         mbar_arrive(&p_full[w]);
         ++gw;
         fresh = false;
