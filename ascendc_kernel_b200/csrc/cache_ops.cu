@@ -368,6 +368,7 @@ __global__ void __launch_bounds__(kCopyThreads) evict_copy_kernel(const EvictPar
   __shared__ RowPlan plan;
   const int b = blockIdx.y;
   const int64_t r0 = static_cast<int64_t>(blockIdx.x) * p.copy.rows;
+  grid_dependency_wait();
   if (threadIdx.x < p.copy.rows) {
     const int left = p.new_lens[b];
     const int64_t row = r0 + threadIdx.x;
@@ -577,6 +578,6 @@ extern "C" int dsa_cache_evict(void* k_pages, const int64_t* kp_strides, void* v
   p.copy.src_head[1] = p.pool.vs[2];
   const int64_t blocks = (dst_pages * page_size + p.copy.rows - 1) / p.copy.rows;
   auto kernel = flat_rows(p.copy) ? evict_copy_kernel<true> : evict_copy_kernel<false>;
-  kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(batch)), kCopyThreads, 0, cs>>>(p);
-  return cuda_status(cudaGetLastError());
+  return launch_dependent(kernel, dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(batch)),
+                          dim3(kCopyThreads), 0, cs, p);
 }

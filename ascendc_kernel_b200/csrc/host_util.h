@@ -65,6 +65,25 @@ struct SideStream {
 };
 int thread_side_stream(SideStream* out, bool may_create);
 
+// Launches `kernel` so that it may start while the launch before it on `stream` still
+// drains: it must call grid_dependency_wait() before it touches anything that an earlier
+// launch reads or writes.
+template <typename... P, typename... A>
+inline int launch_dependent(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem,
+                            cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace dsa

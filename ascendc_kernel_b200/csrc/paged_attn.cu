@@ -321,6 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  grid_launch_dependents();
   const uint32_t tmem = *tmem_holder;
   Walk wk;
   wk.b = walk_s[0];
@@ -804,6 +805,7 @@ __global__ void __launch_bounds__(D) paged_join_kernel(const Params p) {
     u0 = line.owner(first);
     parts = (line.owner(first + n - 1) - u0 + 1) * 2;
   }
+  grid_dependency_wait();
   // piece u of (sequence, kv head) is number u + b hk + kvh
   const int64_t piece = (static_cast<int64_t>(u0) + static_cast<int64_t>(b) * p.hk + kvh) * 2;
   auto part = [&](int i) -> float2 {
@@ -862,6 +864,7 @@ __global__ void __launch_bounds__(kKeys) paged_weights_kernel(const Params p) {
   if (!row_seen(s, c * per + gi, row)) return;
   const int page = page_of(p, b, row);
   if (page < 0) return;
+  grid_dependency_wait();
   const int64_t cap = (static_cast<int64_t>(p.max_pages) * p.page + kKeys - 1) / kKeys + 2;
   const float* lse = p.lse2 + static_cast<int64_t>(b) * p.h;
   const float* z = p.scores + ((static_cast<int64_t>(b) * p.hk * cap + c) * kKeys + threadIdx.x) * p.g;
@@ -936,14 +939,13 @@ int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, con
            : p.g <= 64 ? launch_split<T, D, 64>(q, k, v, p, stream)
                        : launch_split<T, D, 128>(q, k, v, p, stream);
   if (st != DSA_OK) return st;
-  paged_join_kernel<T, D><<<static_cast<unsigned>(p.batch * p.h), D, 2 * (p.units + 1) * sizeof(float),
-                            stream>>>(p);
-  st = cuda_status(cudaGetLastError());
+  st = launch_dependent(paged_join_kernel<T, D>, dim3(static_cast<unsigned>(p.batch * p.h)), dim3(D),
+                        2 * (p.units + 1) * sizeof(float), stream, p);
   if (st != DSA_OK || p.weights == nullptr) return st;
-  paged_weights_kernel<<<dim3(static_cast<unsigned>(max_chunks(p.max_pages, p.page)),
-                              static_cast<unsigned>(p.batch)),
-                         kKeys, 0, stream>>>(p);
-  return cuda_status(cudaGetLastError());
+  return launch_dependent(paged_weights_kernel,
+                          dim3(static_cast<unsigned>(max_chunks(p.max_pages, p.page)),
+                               static_cast<unsigned>(p.batch)),
+                          dim3(kKeys), 0, stream, p);
 }
 
 // Pages [num_pages, page, heads, d]: a box of `rows` slots of one page and head.
