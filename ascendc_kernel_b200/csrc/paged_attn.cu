@@ -29,6 +29,16 @@
 // stay per thread until the piece ends. P is rounded to the operands' type
 // (relative 2^-8 at most for bf16, the size of the output's own rounding); sums are fp32.
 // TMEM: kSBufs S^T buffers of NM columns, then O^T of the two warpgroups.
+//
+// Measured (bf16, head_dim 128):
+//   64 sequences of up to 8192 rows, 32 heads on 8, with weights: 221 us for 1.21 GB;
+//   the split kernel 202 us, 6.0 TB/s (DRAM 76 % active), the weights 12, the join 8.
+//   8 sequences of up to 131,072 rows, 64 heads on one kv head (K is V): split 52 us,
+//   172 MB at 3.3 TB/s. Bound by the softmax: 8,192 exponentials a chunk, about 3,450
+//   cycles for a warpgroup with two of them in turn; DRAM 37 %.
+//   One sequence of 333 rows, 64 heads: split 9 us, join 4.4: the launches' and a
+//   chunk's latency.
+//   One copy warp for all rings and one issuer for S^T and O^T: 242, 71 and 41 us.
 #include "host_util.h"
 #include "window_common.cuh"
 #include "window_host.h"

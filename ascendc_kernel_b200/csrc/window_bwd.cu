@@ -17,6 +17,16 @@
 // over them (relative 2^-8 at most for bf16, the size of the gradients' own rounding);
 // every sum is fp32. D comes from the rounded out; the sink's gradient, an fp32
 // output, uses the unrounded D = sum_j P_j (dout.v_j) that the dq kernel sees.
+//
+// Measured (bf16, head_dim 128), in us:
+//   2 x 4096 tokens, 32 heads on 8, window 1024 + 4: dk/dv 368, dq 316, statistics 22,
+//   join 9; the five products the formulas need run at 440 TFLOP/s, the seven done at
+//   613. Tensor pipe 45 % (dk/dv) and 32 % (dq), issue slots 34 % and 27 %, DRAM below 8 %:
+//   bound by the chain S, dP -> P, dS -> products of a tile, of which two are in flight
+//   (TMEM is full: two accumulators and two pairs of S and dP), and by the 64-wide
+//   products, which read shared memory faster than they compute.
+//   2 x 2600 tokens, 64 heads on one kv head, window 128 + 4: dk/dv 200, dq 96, statistics
+//   31, join 12, dsink 6.
 #include "host_util.h"
 #include "window_common.cuh"
 #include "window_host.h"
@@ -34,7 +44,8 @@ constexpr int kHalfBox = kStream * 128;  // one [64 rows x 64 columns] SW128 box
 
 // ------------------------------------------------------------------ row statistics
 // stat[row] = (-lse log2 e, -D); D / 8 threads a row, each with kStatRows rows' 16-byte
-// loads in flight (one row a thread reached 4.3 TB/s). Flat: dout is contiguous like out.
+// loads in flight: 22 us for 2 x 4096 x 32 rows of 128, 5.9 TB/s (one row a thread: 31 us,
+// 4.3 TB/s). Flat: dout is contiguous like out.
 constexpr int kStatRows = 4;
 
 template <typename T, int D, bool Flat>

@@ -24,6 +24,16 @@
 // the size of the output's own rounding. The reference moves, and O is rescaled,
 // only when a row's maximum exceeds it by more than 2^8, so P stays within fp16.
 // TMEM per tile w: S/P buffers [256w, +64), [256w+64, +64), O [256w+128, +D).
+//
+// Measured (bf16, head_dim 128):
+//   8 x 2600 tokens, 64 heads on one kv head, window 128 + 4: 233 us, 2.9 TB/s of q and
+//   out (0.45 of a copy). An item has 5 chunks, so its start (q, the first scores)
+//   and its end (O to HBM) are most of it; the tensor pipe is active 27 % of the time.
+//   16,384 tokens, 32 heads on 8, window 4096 + 4: 1,090-1,110 us, 870 TFLOP/s (0.52 of a
+//   library GEMM's burst). Tensor pipe 44 %, exponentials 45 %, issue slots 45 %: no
+//   unit is full; the chain S -> maximum -> 2^x -> P -> O of a chunk is what a row's
+//   thread waits for, and two tiles (all that TMEM and registers hold) hide half of it.
+//   128-key chunks with one S buffer a tile, one issuer for both: 349 and 1,581 us.
 #include "host_util.h"
 #include "window_common.cuh"
 #include "window_host.h"

@@ -332,7 +332,9 @@ int dsa_chain_fwd(const void* x, const void* qr, const void* wq_b, const void* w
  *   lse = log(sum_j e^s_j + e^sink[h]),  out = sum_j e^(s_j - lse) v_j
  * (sink: [n_heads] fp32 logits or NULL). A row that sees no key and has no sink
  * gets out = 0, lse = -inf. k and v rows at or past kv_lens[b] may hold
- * anything. Products of the 16-bit operands are summed in fp32; the softmax
+ * anything; rows below it have to be finite: one that is not reaches every query
+ * row of the tiles that read it, also those that do not see it (a masked weight is
+ * 0, and 0 x NaN is NaN, as in the dense form). Products of the 16-bit operands are summed in fp32; the softmax
  * runs in fp32; its weights are rounded to the operands' type for the second
  * product and out once at the end.
  * dtype: DSA_DTYPE_*, of q, k, v and out. q_strides, k_strides, v_strides:
@@ -392,7 +394,9 @@ int dsa_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k,
  * The token sees rows j < lens[b], with window > 0 only j >= lens[b] - window or
  * j < n_first. out, lse [batch, n_heads] (fp32 or NULL), sink and the numerics as
  * dsa_window_attn_fwd. With weights, each visible row's slot gains sum_h e^(s_j -
- * lse_h) (one add per row and sequence; the other slots are untouched).
+ * lse_h) (one add per row and sequence; the other slots are untouched; where
+ * sequences share a page, the order of their adds, and with it the last bit, is not
+ * fixed). Hidden rows may hold anything, NaN included.
  * dtype: DSA_DTYPE_*. Strides in elements, host arrays or NULL for contiguous:
  * q_strides (batch, head), k_strides and v_strides (page, slot, head). Supported:
  * head_dim 64 or 128, n_heads / n_kv_heads <= 128, page_size a multiple of 8,
