@@ -463,9 +463,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint8_t* stage = smem + C::kOffQ + (2 * w + (n & 1)) * C::kTileBytes;
       const uint32_t stage_row = smem_u32(stage) + static_cast<uint32_t>(row * 128);
       if (!named_bar_and(bar, 128, ok)) break;
-      if (last >= 0) {
-        // a wait that runs out here ends the loop at the next item's barrier
-        ok = mbar_wait_warp(&o_done[2 * w + ((gc - 1) & 1)], ((gc - 1) >> 1) & 1, abort_flag, p.err,
+      {
+        // Without keys nothing but q's barrier says that the buffer's turn has come (and the
+        // producer could find q_empty two phases on). A wait that runs out here ends the
+        // loop at the next item's barrier.
+        const bool some = last >= 0;
+        const int x = some ? gc - 1 : n;
+        ok = mbar_wait_warp((some ? o_done : q_full) + 2 * w + (x & 1), (x >> 1) & 1, abort_flag, p.err,
                             DSA_DEVERR_WIN_WAIT);
         tc_fence_after();
       }

@@ -170,6 +170,18 @@ def test_key_tiles_split_over_their_rows(cuda_device):
         assert ((x.double() - r[name]).abs() <= (1 + 2.0 ** -4) * r[name + "_err"]).all(), name
 
 
+
+@pytest.mark.parametrize("lens", [[204, 0, 0], [0, 0, 0], [0, 204, 0]])
+def test_long_runs_of_rows_without_keys(cuda_device, lens):
+    """Several work items in a row on each SM see no key, after and before some that do."""
+    q, k, v, s, _ = inputs(3, 153, 204, 381, 3, 64, torch.bfloat16, True, False)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    _native.device_error(0)
+    out = window_attn(q, k, v, s, window=2, n_first=65, kv_lens=n)
+    assert _native.device_error(0) == 0
+    check_out(out, definition(q, k, v, s, 2, 65, n, 64 ** -0.5), torch.bfloat16)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_gradient_against_differences(cuda_device, dtype):
     """The directional derivative of sum(out * dout) from the gradients, against a central
