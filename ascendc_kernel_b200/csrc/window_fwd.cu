@@ -58,10 +58,11 @@ struct FwdCfg {
   static constexpr int kTileBytes = kRows * D * 2;
   static constexpr int kSlotBytes = kCB * kBlk * D * 2;
   static constexpr int kSlots = 6;  // 6 stages of one slot (K = V) or 3 of two (K, V)
-  static constexpr int kOffQ = 0;  // [2 tiles][2]: q of an item, then its results
-  static constexpr int kOffKV = 4 * kTileBytes;
-  static constexpr int kOffBar = kOffKV + kSlots * kSlotBytes;
-  static constexpr int kNumBars = 4 + 4 + 2 * kSlots + 4 + 4 + 4 + 2 + 1;
+  static constexpr int kOffQ = 0;
+  static constexpr int kOffKV = 2 * kTileBytes;
+  static constexpr int kOffStage = kOffKV + kSlots * kSlotBytes;  // [2] tiles of results
+  static constexpr int kOffBar = kOffStage + 2 * kTileBytes;
+  static constexpr int kNumBars = 2 + 2 + 2 * kSlots + 4 + 4 + 4 + 2 + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;
   static constexpr int kSmemBytes = kOffMisc + 16 + 1024;
 };
@@ -86,9 +87,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t* q_full = bars;                  // [2 tiles][2] TMA -> MMA
-  uint64_t* q_empty = q_full + 4;           // [2 tiles][2] the results there left -> TMA
-  uint64_t* kv_full = q_empty + 4;          // [stages]
+  uint64_t* q_full = bars;                  // [2] TMA -> MMA
+  uint64_t* q_empty = q_full + 2;           // [2] last S of the tile done -> TMA
+  uint64_t* kv_full = q_empty + 2;          // [stages]
   uint64_t* kv_empty = kv_full + C::kSlots; // [stages] both issuers
   uint64_t* s_full = kv_empty + C::kSlots;  // [2 tiles][2] S of a chunk in TMEM
   uint64_t* p_full = s_full + 4;            // [2 tiles][2] P written (128 arrivals)
@@ -105,9 +106,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int w = 0; w < 2; ++w) {
+      mbar_init(&q_full[w], 1);
+      mbar_init(&q_empty[w], 1);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&q_full[2 * w + i], 1);
-        mbar_init(&q_empty[2 * w + i], 1);
         mbar_init(&s_full[2 * w + i], 1);
         mbar_init(&p_full[2 * w + i], 128);
         mbar_init(&o_done[2 * w + i], 1);
@@ -142,8 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       Ring<0> at;
       int loads = 0;
-      int q_loads[2] = {0, 0};
-      int n = 0;  // items
+      int uses0 = 0, uses1 = 0;
       bool ok = true;
       auto load = [&](const Item<kCB>& it, int c) -> bool {
         if (!mbar_wait(&kv_empty[at.slot], at.parity ^ 1u, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
@@ -166,36 +166,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         ++loads;
         return true;
       };
-      // every item takes its turn at the buffers, also one whose tile has nothing to load
-      auto load_q = [&](const Item<kCB>& it, int w) -> bool {
-        const int buf = 2 * w + (n & 1);
-        if (!mbar_wait(&q_empty[buf], ((n >> 1) & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
+      auto load_q = [&](const Item<kCB>& it, int w, int& uses) -> bool {
+        if (it.last(w) < 0) return true;
+        if (!mbar_wait(&q_empty[w], (uses & 1) ^ 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT))
           return false;
-        ++q_loads[w];
-        if (it.last(w) < 0) {
-          mbar_arrive(&q_full[buf]);
-          return true;
-        }
-        uint8_t* qs = smem + C::kOffQ + buf * C::kTileBytes;
-        mbar_arrive_expect_tx(&q_full[buf], static_cast<uint32_t>(p.grid.tt * p.s.g * D * 2));
+        uint8_t* qs = smem + C::kOffQ + w * C::kTileBytes;
+        mbar_arrive_expect_tx(&q_full[w], static_cast<uint32_t>(p.grid.tt * p.s.g * D * 2));
 #pragma unroll
         for (int half = 0; half < C::kHalves; ++half)
           tma_load_4d(qs + half * kBoxBytes, &tm_q, half * 64, it.kvh * p.s.g, it.t0(w), it.b,
-                      &q_full[buf]);
+                      &q_full[w]);
+        ++uses;
         return true;
       };
-      for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid), ++n) {
+      for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid)) {
         const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
         if (it.chunks > 0) ok = load(it, 0);
-        ok = ok && load_q(it, 0) && load_q(it, 1);
+        ok = ok && load_q(it, 0, uses0) && load_q(it, 1, uses1);
         for (int c = 1; c < it.chunks && ok; ++c) ok = load(it, c);
       }
       // copies in flight land before the CTA's shared memory goes away
       for (int i = max(loads - stages, 0); i < loads; ++i)
         mbar_drain(&kv_full[i % stages], (i / stages) & 1);
-      for (int w = 0; w < 2; ++w)
-        for (int i = max(q_loads[w] - 2, 0); i < q_loads[w]; ++i)
-          mbar_drain(&q_full[2 * w + (i & 1)], (i >> 1) & 1);
+      if (uses0 > 0) mbar_drain(&q_full[0], (uses0 - 1) & 1);
+      if (uses1 > 0) mbar_drain(&q_full[1], (uses1 - 1) & 1);
     }
   } else if (warp == 1 || warp == 2) {
     // ------------------------------------------------------------ MMA issuers
@@ -226,8 +220,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         at.next(stages);
         return s;
       };
-      int gs = 0, go = 0, uses = 0;  // S and PV products issued, items with some
-      int n = 0;                     // items
+      int gs = 0, go = 0, uses = 0;  // S and PV products issued, items
       auto issue_s = [&](const Item<kCB>& it, int c, int slot) {
         if (!ok || !it.active(w, c)) return;
         // the buffer's P was read by the PV product before the last one
@@ -236,10 +229,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) return;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(w * 256 + (gs & 1) * 64);
-        const uint32_t qa = q_lo + static_cast<uint32_t>((2 * w + (n & 1)) * (C::kTileBytes >> 4));
+        const uint32_t qa = q_lo + static_cast<uint32_t>(w * (C::kTileBytes >> 4));
         const uint32_t kb = k_lo + static_cast<uint32_t>(slot * (stage_bytes >> 4));
         const uint32_t idesc_s =
             make_idesc<T>(128, 0, 0) | (static_cast<uint32_t>(it.blocks(c) * kBlk / 8) << 17);
+        const bool end = c == it.last(w);
         if (elect_one()) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
@@ -249,6 +243,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                       k > 0 ? 1u : 0u);
           }
           umma_commit(&s_full[buf]);
+          if (end) umma_commit(&q_empty[w]);
         }
         __syncwarp();
         ++gs;
@@ -302,22 +297,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (wrote) fence_proxy_async_smem();
         __syncwarp();
       };
-      for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid), ++n) {
+      for (ItemWalk wk(p.s, p.grid); ok && wk.item < p.grid.items; wk.next(p.s, p.grid)) {
         const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
-        ok = wait_warp(&q_full[2 * w + (n & 1)], (n >> 1) & 1);
-        if (it.chunks == 0) continue;
+        const int n = it.chunks;
+        if (n == 0) continue;
         // stages of chunks c, c + 1 and c + 2; the other issuer takes the same
         int s0 = take(), s1 = 0, s2 = 0;
-        if (it.last(w) >= 0) ++uses;
+        if (it.last(w) >= 0) ok = ok && wait_warp(&q_full[w], uses++ & 1);
         issue_s(it, 0, s0);
-        if (it.chunks > 1) {
+        if (n > 1) {
           s1 = take();
           issue_s(it, 1, s1);
         }
-        for (int c = 0; c < it.chunks && ok; ++c) {
+        for (int c = 0; c < n && ok; ++c) {
           if (p.s.kv_lens != nullptr) clear_tail(it, c, s0);
           issue_pv(it, c, s0);
-          if (c + 2 < it.chunks) {
+          if (c + 2 < n) {
             s2 = take();
             issue_s(it, c + 2, s2);
           }
@@ -341,21 +336,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lane_off = static_cast<uint32_t>(quarter * 32) << 16;
     const uint32_t st = tmem + lane_off + static_cast<uint32_t>(w * 256);
     const uint32_t od = st + 128u;
+    uint8_t* stage = smem + C::kOffStage + w * C::kTileBytes;
+    const uint32_t stage_row = smem_u32(stage) + static_cast<uint32_t>(row * 128);
     const uint32_t bar = 1 + static_cast<uint32_t>(w);
     const bool leader = quarter == 0 && lane == 0;  // issues the tile's stores
     const uint64_t scale2 = f2_pack(p.scale_log2, p.scale_log2);
     int gc = 0;  // chunks processed (all items)
-    int n = 0;   // items
     bool ok = true;
-    bool pending = false;  // the last item's buffer was not given back yet
-    auto give_back = [&]() {
-      if (pending && leader) {
-        bulk_wait_group_read<0>();
-        mbar_arrive(&q_empty[2 * w + ((n & 1) ^ 1)]);
-      }
-      pending = false;
-    };
-    for (ItemWalk wk(p.s, p.grid); wk.item < p.grid.items; wk.next(p.s, p.grid), ++n) {
+    for (ItemWalk wk(p.s, p.grid); wk.item < p.grid.items; wk.next(p.s, p.grid)) {
       const Item<kCB> it = make_item<kCB>(p.s, p.grid, wk);
       const int first = it.first(w), last = it.last(w);
       const int t = it.t0(w) + tok;
@@ -455,21 +443,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         mbar_arrive(&p_full[2 * w + buf]);
         ++gc;
-        give_back();
       }
-      // ---- epilogue. The results go where the item's q was: all its S are there. A
-      // warpgroup leaves together, since it meets at barriers
-      give_back();
-      uint8_t* stage = smem + C::kOffQ + (2 * w + (n & 1)) * C::kTileBytes;
-      const uint32_t stage_row = smem_u32(stage) + static_cast<uint32_t>(row * 128);
+      // ---- epilogue. The previous item's rows have left the staging buffer; a warpgroup
+      // leaves together, since it meets at barriers
+      if (leader) bulk_wait_group_read<0>();
       if (!named_bar_and(bar, 128, ok)) break;
-      {
-        // Without keys nothing but q's barrier says that the buffer's turn has come (and the
-        // producer could find q_empty two phases on). A wait that runs out here ends the
-        // loop at the next item's barrier.
-        const bool some = last >= 0;
-        const int x = some ? gc - 1 : n;
-        ok = mbar_wait_warp((some ? o_done : q_full) + 2 * w + (x & 1), (x >> 1) & 1, abort_flag, p.err,
+      if (last >= 0) {
+        // a wait that runs out here ends the loop at the next item's barrier
+        ok = mbar_wait_warp(&o_done[2 * w + ((gc - 1) & 1)], ((gc - 1) >> 1) & 1, abort_flag, p.err,
                             DSA_DEVERR_WIN_WAIT);
         tc_fence_after();
       }
@@ -517,7 +498,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           tma_store_4d(&tm_out, stage + half * kBoxBytes, half * 64, it.kvh * p.s.g, it.t0(w), it.b);
         bulk_commit_group();
       }
-      pending = true;
       if (valid && p.lse != nullptr)
         p.lse[(static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + gh] = (ref + log2f(total)) * kLn2;
     }
