@@ -863,7 +863,8 @@ __global__ void __launch_bounds__(D) paged_join_kernel(const Params p) {
 }
 
 // weights[slot of key] += sum over heads of 2^(z - lse): a thread a key, heads in order,
-// four at a time where the group's size and the scores' rows allow.
+// four at a time where the group's size and the scores' rows allow. lse is the join's
+// result, so it is read with ordinary loads: a read-only load is not held back by the wait.
 __global__ void __launch_bounds__(kKeys) paged_weights_kernel(const Params p) {
   const int b = blockIdx.y, c = blockIdx.x;
   const Seq s = make_seq(p, b);
@@ -886,14 +887,14 @@ __global__ void __launch_bounds__(kKeys) paged_weights_kernel(const Params p) {
     for (int i = 0; i < n4; ++i) {
       const int kvh = i / g4;
       const float4 a = *reinterpret_cast<const float4*>(z + kvh * step + (i - kvh * g4) * 4);
-      const float4 m = __ldg(reinterpret_cast<const float4*>(lse) + i);
+      const float4 m = reinterpret_cast<const float4*>(lse)[i];
       sum += (ex2_approx(a.x - m.x) + ex2_approx(a.y - m.y)) +
              (ex2_approx(a.z - m.z) + ex2_approx(a.w - m.w));
     }
   } else {
     for (int kvh = 0; kvh < p.hk; ++kvh)
       for (int k = 0; k < p.g; ++k)
-        sum += ex2_approx(z[kvh * step + k] - __ldg(lse + kvh * p.g + k));
+        sum += ex2_approx(z[kvh * step + k] - lse[kvh * p.g + k]);
   }
   // one add per slot; pages that sequences share get one from each
   atomicAdd(p.weights + static_cast<int64_t>(page) * p.page + row % p.page, sum);
