@@ -868,14 +868,17 @@ __global__ void __launch_bounds__(D) paged_join_kernel(const Params p) {
 __global__ void __launch_bounds__(kKeys) paged_weights_kernel(const Params p) {
   const int b = blockIdx.y, c = blockIdx.x;
   const Seq s = make_seq(p, b);
-  if (c >= s.chunks) return;
-  const int per = kKeys >> p.gshift;
-  const int gi = threadIdx.x >> p.gshift;
-  const int row = gran_row(p, s, c * per + gi) + (threadIdx.x & (p.gran - 1));
-  if (!row_seen(s, c * per + gi, row)) return;
-  const int page = page_of(p, b, row);
-  if (page < 0) return;
+  int row = 0, page = -1;
+  if (c < s.chunks) {
+    const int per = kKeys >> p.gshift;
+    const int gi = threadIdx.x >> p.gshift;
+    row = gran_row(p, s, c * per + gi) + (threadIdx.x & (p.gran - 1));
+    if (row_seen(s, c * per + gi, row)) page = page_of(p, b, row);
+  }
+  // every block waits, also those without a visible row: the launch after this one counts on
+  // the join being done once this grid is
   grid_dependency_wait();
+  if (page < 0) return;
   const int64_t cap = (static_cast<int64_t>(p.max_pages) * p.page + kKeys - 1) / kKeys + 2;
   const float* lse = p.lse2 + static_cast<int64_t>(b) * p.h;
   const float* z = p.scores + ((static_cast<int64_t>(b) * p.hk * cap + c) * kKeys + threadIdx.x) * p.g;

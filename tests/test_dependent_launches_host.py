@@ -5,6 +5,9 @@ Such a kernel's lifetime begins before the earlier launch has written its result
 non-coherent load (``__ldg``) promises that the data is read-only for that whole lifetime and
 is not ordered by the wait, so nothing that follows ``grid_dependency_wait()`` in the kernel's
 body may use one.
+
+A launch after it waits for its end alone, so that end must not come before the earlier
+launch's: every block waits, and none returns before.
 """
 
 import glob
@@ -43,3 +46,10 @@ def test_the_dependent_kernels_are_found():
 @pytest.mark.parametrize("name,body", dependent_kernels(), ids=lambda x: x if len(x) < 40 else "")
 def test_no_read_only_loads_after_the_wait(name, body):
     assert "__ldg" not in body.split("grid_dependency_wait()", 1)[1], name
+
+
+@pytest.mark.parametrize("name,body", dependent_kernels(), ids=lambda x: x if len(x) < 40 else "")
+def test_no_block_leaves_before_the_wait(name, body):
+    # returns of lambdas (`-> type {`) belong to the lambda
+    before = re.sub(r"->[^{;]*\{[^}]*\}", "", body.split("grid_dependency_wait()", 1)[0])
+    assert not re.search(r"\breturn\b", before), name
