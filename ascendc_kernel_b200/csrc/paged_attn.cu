@@ -778,7 +778,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         float sum = ld_shared_f32(wmax + key * 4);
 #pragma unroll
         for (int i = 1; i < 4; ++i) sum += ld_shared_f32(wmax + static_cast<uint32_t>((i * NM + key) * 4));
-        ml[key] = make_float2(-ld_shared_f32(nref + key * 4), sum);
+        // chunks of absent pages leave no reference: the join must not take their 0 for one
+        ml[key] = make_float2(unset ? kNone : -ld_shared_f32(nref + key * 4), sum);
       }
       named_bar_sync(bar, 128);  // the next piece writes the references and maxima
     }

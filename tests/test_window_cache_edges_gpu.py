@@ -1,0 +1,59 @@
+"""Windowed attention and the paged cache at the ends of their ranges: chunks whose pages are
+absent under very low scores.
+
+Bounds as in test_paged_cache_gpu.py; where scores are about -100, their fp32 sums (64 terms,
+each addition off by at most 2^-23 of 800, times the scale of 1/8) are good to 8e-4, so the
+fp32 part is 1e-3 of the magnitudes.
+"""
+
+import math
+
+import pytest
+import torch
+
+from ascendc_kernel_b200 import _native
+from ascendc_kernel_b200.paged_cache import paged_attn
+
+pytestmark = pytest.mark.gpu
+
+DEVERR_CACHE = 0x0040
+
+
+# rows, page, first and last + 1 page that is absent: the first chunk of 128 rows, one between
+# others, the last one, all but one; chunks of their own block and blocks of several chunks
+@pytest.mark.parametrize("rows,page,gone", [
+    (300, 16, (0, 8)), (300, 16, (8, 16)), (300, 16, (16, 19)), (300, 16, (0, 16)),
+    (60000, 64, (2, 4)), (60000, 64, (101, 460)),
+])
+@pytest.mark.parametrize("weighted", [False, True])
+def test_absent_chunks_under_low_scores(cuda_device, rows, page, gone, weighted):
+    """Rows without a page count as hidden, also where they fill whole chunks and every score
+    lies far below 0."""
+    h, d, dtype = 4, 64, torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(7)
+    width = -(-rows // page)
+    k = torch.randn(width, page, 1, d, generator=g, device="cuda").to(dtype) * 0.25
+    v = torch.randn(width, page, 1, d, generator=g, device="cuda").to(dtype)
+    k[..., 0] = -100.0
+    q = torch.randn(1, h, d, generator=g, device="cuda").to(dtype)
+    q[..., 0] = 8.0
+    table = torch.arange(width, dtype=torch.int32, device="cuda")[None].contiguous()
+    table[0, gone[0]:gone[1]] = -1
+    n = torch.full((1,), rows, dtype=torch.int32, device="cuda")
+    weights = torch.zeros(width, page, device="cuda") if weighted else None
+    out, lse = paged_attn(q, k, v, table, n, weights=weights, return_lse=True)
+    assert _native.device_error(0) == DEVERR_CACHE
+    live = torch.ones(width, page, dtype=torch.bool, device="cuda")
+    live[gone[0]:gone[1]] = False
+    live.view(-1)[rows:] = False
+    kk, vv = k[live][:, 0].double(), v[live][:, 0].double()
+    s = (q[0].double() @ kk.T) * d ** -0.5
+    p = torch.softmax(s, 1)
+    mag = p @ vv.abs()
+    want = p @ vv
+    assert s.max() < -90 and len(kk) > 0
+    assert ((out[0].double() - want).abs() <= 2.0 ** -8 * (want.abs() + mag) + 1e-3 * mag).all()
+    assert ((lse[0].double() - torch.logsumexp(s, 1)).abs() <= 1e-3).all()
+    if weighted:
+        assert not weights[~live].any()
+        assert ((weights[live].double() - p.sum(0)).abs() <= 1e-3 * p.sum(0)).all()
