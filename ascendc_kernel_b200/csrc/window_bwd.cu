@@ -5,7 +5,8 @@
 //   dq = scale sum_j dS_j k_j      dk_j = scale sum_rows dS_j q      dv_j = sum_rows P_j dout
 //   dsink_h = -sum_rows e^(sink_h - lse) D       (v the same tensor as k: dk + dv in one)
 //
-// Deterministic without atomics, in up to five launches:
+// Deterministic without atomics (but maxima, whose order does not matter), in up to five
+// launches:
 //   window_stat_kernel  per row -lse log2(e) and -D, HBM bound (out and dout read once)
 //   window_dkv_kernel   a key tile stays, the rows that see it stream by (4 products)
 //   window_join_kernel  sums the fp32 parts of key tiles whose rows were split
@@ -17,6 +18,16 @@
 // over them (relative 2^-8 at most for bf16, the size of the gradients' own rounding);
 // every sum is fp32. D comes from the rounded out; the sink's gradient, an fp32
 // output, uses the unrounded D = sum_j P_j (dout.v_j) that the dq kernel sees.
+//
+// fp16 is normal from 2^-14 to 2^16 only, where P has 1 / keys and dS the upstream gradient's
+// size in it. Both are scaled by powers of two before they are rounded and the sums scaled back
+// in fp32: P by 2^14, dP - D by the power of two that brings its bound below 1,
+//   |dP - D| <= |dout| |v| + |D|
+// (dk: this key's |v| and the largest |dout| and |D| of the kv head's rows; dq: this row's
+// |dout| and D and the largest |v|). The scale belongs to the accumulator's row, so it leaves
+// the sum. |dS| stays below 2^14, and no dS is off by more than 2^-38 of the bound. It costs
+// 3 % of the gradients' time in the first case below and 9 % in the second (752 against 728
+// and 394 against 362 us); unscaled, dk of an upstream gradient of 1e-5 was lost.
 //
 // Measured (bf16, head_dim 128), in us:
 //   2 x 4096 tokens, 32 heads on 8, window 1024 + 4: dk/dv 368, dq 316, statistics 22,
@@ -42,25 +53,58 @@ constexpr int kCB = 2;                // key blocks of a chunk (dq), 64 keys
 constexpr int kStream = 64;           // rows of a streamed tile (dkv)
 constexpr int kHalfBox = kStream * 128;  // one [64 rows x 64 columns] SW128 box
 
+// ------------------------------------------------------------------ scales (fp16)
+constexpr float kPUp = 14.f;                // P is rounded as 2^kPUp P
+constexpr float kPDown = 1.f / 16384.f;
+
+// Largest norms and magnitudes of one (batch, kv head) as bits of non-negative floats, whose
+// order is the values' (a maximum does not depend on the order of its atomics).
+struct Peak {
+  uint32_t dout, d, v;
+};
+__device__ __forceinline__ void raise(uint32_t* peak, uint32_t bits) {
+  if (bits > *static_cast<volatile uint32_t*>(peak)) atomicMax(peak, bits);
+}
+
+// The power of two f that brings bound f to [1/2, 1); 1 where the bound is 0 or not finite.
+__device__ __forceinline__ float power_below(float bound) {
+  const uint32_t e = __float_as_uint(bound) >> 23;  // bound >= 0 or NaN
+  return e >= 27u && e < 250u ? __uint_as_float((253u - e) << 23) : 1.f;
+}
+// What a sum of dS 2^kPUp f is scaled by.
+__device__ __forceinline__ float scale_down(float scale, float f) {
+  return scale * (kPDown * __uint_as_float((254u << 23) - __float_as_uint(f)));  // 1 / f
+}
+
 // ------------------------------------------------------------------ row statistics
 // stat[row] = (-lse log2 e, -D); D / 8 threads a row, each with kStatRows rows' 16-byte
 // loads in flight: 22 us for 2 x 4096 x 32 rows of 128, 5.9 TB/s (one row a thread: 31 us,
-// 4.3 TB/s). Flat: dout is contiguous like out.
+// 4.3 TB/s). Flat: dout is contiguous like out. With fp16 also norm[row] = |dout| and the
+// peaks of the rows that see something.
 constexpr int kStatRows = 4;
 
 template <typename T, int D, bool Flat>
 __global__ void __launch_bounds__(256) window_stat_kernel(const uint16_t* out, const uint16_t* dout,
                                                           Strides ds, const float* lse, float2* stat,
-                                                          int64_t rows, int m, int h) {
+                                                          float* norm, Peak* peaks, int64_t rows,
+                                                          int m, int h, int g) {
   constexpr int kLanes = D / 8;
   constexpr int kStep = 256 / kLanes;  // rows of a block at once
+  // fp16: maxima of the block's (token, kv head) groups of rows, which then raise the peaks:
+  // an atomic a row took 75 us more
+  __shared__ uint32_t top[T::kNarrow ? 2 : 1][T::kNarrow ? kStep * kStatRows + 1 : 1];
+  const int64_t group0 = static_cast<int64_t>(blockIdx.x) * (kStep * kStatRows) / g;
+  if constexpr (T::kNarrow) {
+    for (int i = threadIdx.x; i <= kStep * kStatRows; i += 256) top[0][i] = top[1][i] = 0u;
+    __syncthreads();
+  }
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * (kStep * kStatRows) + threadIdx.x / kLanes;
   const int x = threadIdx.x % kLanes;
-  uint4 a[kStatRows], g[kStatRows];
+  uint4 a[kStatRows], up[kStatRows];
 #pragma unroll
   for (int r = 0; r < kStatRows; ++r) {
     const int64_t row = row0 + r * kStep;
-    a[r] = g[r] = make_uint4(0u, 0u, 0u, 0u);
+    a[r] = up[r] = make_uint4(0u, 0u, 0u, 0u);
     if (row < rows) {
       int64_t at = row * D;
       a[r] = __ldcs(reinterpret_cast<const uint4*>(out + at + x * 8));
@@ -69,13 +113,14 @@ __global__ void __launch_bounds__(256) window_stat_kernel(const uint16_t* out, c
         const int64_t b = bt / m;
         at = b * ds.b + (bt - b * m) * ds.t + (row - bt * h) * ds.h;
       }
-      g[r] = *reinterpret_cast<const uint4*>(dout + at + x * 8);
+      up[r] = *reinterpret_cast<const uint4*>(dout + at + x * 8);
     }
   }
 #pragma unroll
   for (int r = 0; r < kStatRows; ++r) {
     const int64_t row = row0 + r * kStep;
-    const uint32_t aw[4] = {a[r].x, a[r].y, a[r].z, a[r].w}, gw[4] = {g[r].x, g[r].y, g[r].z, g[r].w};
+    const uint32_t aw[4] = {a[r].x, a[r].y, a[r].z, a[r].w};
+    const uint32_t gw[4] = {up[r].x, up[r].y, up[r].z, up[r].w};
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -84,10 +129,41 @@ __global__ void __launch_bounds__(256) window_stat_kernel(const uint16_t* out, c
     }
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+    float sq = 0.f;
+    if constexpr (T::kNarrow) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sq = fmaf(T::lo(gw[i]), T::lo(gw[i]), sq);
+        sq = fmaf(T::hi(gw[i]), T::hi(gw[i]), sq);
+      }
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) sq += __shfl_xor_sync(0xFFFFFFFFu, sq, o);
+    }
     if (row < rows && x == 0) {
       const float l = lse[row];
+      if constexpr (T::kNarrow) {
+        const float size = sqrtf(sq);
+        norm[row] = size;
+        if (l != -INFINITY) {
+          const int i = static_cast<int>(row - group0 * g) / g;
+          atomicMax(&top[0][i], __float_as_uint(size));
+          atomicMax(&top[1][i], __float_as_uint(fabsf(sum)));
+        }
+      }
       // a row that sees nothing has no weights: 2^(s - inf) = 0
       stat[row] = make_float2(l == -INFINITY ? -INFINITY : -l * kLog2e, -sum);
+    }
+  }
+  if constexpr (T::kNarrow) {
+    __syncthreads();
+    const int hk = h / g;
+    for (int i = threadIdx.x; i <= kStep * kStatRows; i += 256) {
+      if ((top[0][i] | top[1][i]) != 0u) {
+        const int64_t bt = (group0 + i) / hk;
+        Peak* peak = peaks + (bt / m) * hk + (group0 + i - bt * hk);
+        raise(&peak->dout, top[0][i]);
+        raise(&peak->d, top[1][i]);
+      }
     }
   }
 }
@@ -170,18 +246,20 @@ __device__ __forceinline__ Unit make_unit(const DkvParams& p, int64_t unit) {
   return u;
 }
 
+// peaks (fp16 only): of the rows when the kernel starts; the keys' norms are added. A
+// parameter of its own: inside DkvParams it cost the bf16 kernel 12 bytes of spills and 1 %.
 template <typename T, int D>
 __global__ void __launch_bounds__(kBwdThreads, 1)
     window_dkv_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_do,
                       const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
-                      const DkvParams p) {
+                      const DkvParams p, Peak* peaks) {
   using C = DkvCfg<D>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
   uint64_t* kv_full = bars;
-  uint64_t* kv_empty = bars + 1;
+  uint64_t* kv_empty = bars + 1;               // products done (and with fp16, the norms taken)
   uint64_t* st_full = bars + 2;                // [kStages] rows and statistics (1 + 32 arrivals)
   uint64_t* st_empty = st_full + C::kStages;   // [kStages] products done and statistics read
   uint64_t* s_full = st_empty + C::kStages;    // [2] S^T of a tile in TMEM
@@ -201,7 +279,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    mbar_init(kv_empty, 1);
+    mbar_init(kv_empty, T::kNarrow ? 1 + 256 : 1);
     for (int s = 0; s < C::kStages; ++s) {
       mbar_init(&st_full[s], 33);
       mbar_init(&st_empty[s], 1);
@@ -295,7 +373,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           float* ss = stat_s + s * 2 * kStream;
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            ss[lane + 32 * i] = st[i].x;
+            ss[lane + 32 * i] = T::kNarrow ? st[i].x + kPUp : st[i].x;
             ss[kStream + lane + 32 * i] = st[i].y;
           }
           mbar_arrive(&st_full[s]);
@@ -430,6 +508,41 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       int end = p.s.n;
       if (key >= p.s.n_first && far < end) end = static_cast<int>(far);
       if (key >= u.kv_len) end = key;
+      float up = 1.f;  // the key's scale of dS (fp16)
+      if constexpr (T::kNarrow) {
+        if (nt > 0) {
+          ok = mbar_wait_warp(kv_full, uses & 1, abort_flag, p.err, DSA_DEVERR_WIN_WAIT);
+          if (!ok) break;
+          float sq = 0.f;
+#pragma unroll
+          for (int half = 0; half < C::kHalves; ++half) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              // 16-byte pieces in an order that keeps the lanes on different banks
+              const float4 x = ld_shared_f4(smem_u32(smem + C::kOffV + half * kBoxBytes + row * 128) +
+                                            ((static_cast<uint32_t>(j) ^ static_cast<uint32_t>(row & 7)) << 4));
+              const uint32_t vw[4] = {__float_as_uint(x.x), __float_as_uint(x.y),
+                                      __float_as_uint(x.z), __float_as_uint(x.w)};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                sq = fmaf(T::lo(vw[i]), T::lo(vw[i]), sq);
+                sq = fmaf(T::hi(vw[i]), T::hi(vw[i]), sq);
+              }
+            }
+          }
+          mbar_arrive(kv_empty);
+          const float size = sqrtf(sq);
+          Peak* peak = peaks + (static_cast<int64_t>(u.b) * p.s.hk + u.kvh);
+          const uint32_t most =
+              __reduce_max_sync(0xFFFFFFFFu, key < u.kv_len ? __float_as_uint(size) : 0u);
+          if (w == 0 && lane == 0) raise(&peak->v, most);
+          up = power_below(__uint_as_float(peak->dout) * size + __uint_as_float(peak->d));
+        }
+      }
+      auto scaled = [&](uint64_t g2) -> uint64_t {
+        if constexpr (T::kNarrow) return f2_mul(g2, f2_pack(up, up));
+        return g2;
+      };
       for (int i = 0; i < nt; ++i) {
         if (((gs + i) & 1) != w) continue;
         const int s = (gs + i) % C::kStages;
@@ -509,8 +622,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               const int c = 4 * k + 2 * e;
               float g0, g1;
               f2_unpack(f2_mul(f2_pack(__uint_as_float(sv[q][c]), __uint_as_float(sv[q][c + 1])),
-                               f2_add(f2_pack(__uint_as_float(dv[q][c]), __uint_as_float(dv[q][c + 1])),
-                                      e ? f2_pack(nd.z, nd.w) : f2_pack(nd.x, nd.y))),
+                               scaled(f2_add(f2_pack(__uint_as_float(dv[q][c]),
+                                                     __uint_as_float(dv[q][c + 1])),
+                                             e ? f2_pack(nd.z, nd.w) : f2_pack(nd.x, nd.y)))),
                         g0, g1);
               dk[c >> 1] = T::pack(g0, g1);
             }
@@ -544,11 +658,12 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
           tmem_ld_32x32b_x32(tmem + lane_off + 256u + static_cast<uint32_t>(c0 + q * 32), a);
           tmem_ld_32x32b_x32(tmem + lane_off + 384u + static_cast<uint32_t>(c0 + q * 32), b);
         }
+        const float down = T::kNarrow ? scale_down(p.scale, up) : p.scale;
         float fk[32], fv[32];
 #pragma unroll
         for (int k = 0; k < 32; ++k) {
-          fk[k] = live ? __uint_as_float(a[k]) * p.scale : 0.f;
-          fv[k] = live ? __uint_as_float(b[k]) : 0.f;
+          fk[k] = live ? __uint_as_float(a[k]) * down : 0.f;
+          fv[k] = live ? __uint_as_float(b[k]) * (T::kNarrow ? kPDown : 1.f) : 0.f;
           if (p.dv == nullptr) fk[k] += fv[k];
         }
         if (u.parts > 1) {
@@ -666,8 +781,11 @@ struct DqParams {
   float scale, scale_log2;
   const float2* stat;   // [batch, m, h]
   const float* sink;    // [h] or null
+  const Peak* peaks;    // [batch, hk], fp16 only
   uint16_t* dq;         // [batch, m, h, D]
-  float* sink_rows;     // [batch, m, h]: e^(sink - lse) sum_j P_j dP_j, with sink
+  // [batch, m, h]: with fp16 a row's |dout| when the kernel starts; then, with sink,
+  // e^(sink - lse) sum_j P_j dP_j
+  float* sink_rows;
   int shared;
   unsigned int* err;
 };
@@ -935,7 +1053,13 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
       const int pos = min(t, it.t1(w) - 1) + p.s.n - p.s.m;
       const int64_t orow = (static_cast<int64_t>(it.b) * p.s.m + t) * p.s.h + it.kvh * p.s.g + head;
       const float2 st = valid ? __ldg(p.stat + orow) : make_float2(-INFINITY, 0.f);
-      const uint64_t l2 = f2_pack(st.x, st.x), d2 = f2_pack(st.y, st.y);
+      const float nl = T::kNarrow ? st.x + kPUp : st.x;
+      const uint64_t l2 = f2_pack(nl, nl), d2 = f2_pack(st.y, st.y);
+      float up = 1.f;  // the row's scale of dS (fp16)
+      if constexpr (T::kNarrow) {
+        const Peak* peak = p.peaks + (static_cast<int64_t>(it.b) * p.s.hk + it.kvh);
+        if (valid) up = power_below(p.sink_rows[orow] * __uint_as_float(__ldg(&peak->v)) + fabsf(st.y));
+      }
       uint64_t psum[2] = {0ull, 0ull};  // sum_j P_j dP_j
       for (int c = first; c <= last; ++c) {
         if (!it.active(w, c)) continue;
@@ -990,7 +1114,9 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
               const uint64_t e2 = f2_pack(__uint_as_float(sv[i][2 * k]), __uint_as_float(sv[i][2 * k + 1]));
               const uint64_t g2 = f2_pack(__uint_as_float(dv[2 * k]), __uint_as_float(dv[2 * k + 1]));
               psum[k & 1] = f2_fma(e2, g2, psum[k & 1]);
-              f2_unpack(f2_mul(e2, f2_add(g2, d2)), g0, g1);
+              uint64_t ds2 = f2_add(g2, d2);
+              if constexpr (T::kNarrow) ds2 = f2_mul(ds2, f2_pack(up, up));
+              f2_unpack(f2_mul(e2, ds2), g0, g1);
               pk[k] = T::pack(g0, g1);
             }
             tmem_st_x16_nowait(sp + static_cast<uint32_t>(i * 16), pk);
@@ -1007,6 +1133,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         if (!ok) break;
         tc_fence_after();
       }
+      const float down = T::kNarrow ? scale_down(p.scale, up) : p.scale;
 #pragma unroll 1
       for (int q = 0; q < D / 32; ++q) {
         uint32_t ov[32], x[16];
@@ -1014,8 +1141,8 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
 #pragma unroll
         for (int k = 0; k < 16; ++k)
           x[k] = last < 0 ? 0u
-                          : T::pack(__uint_as_float(ov[2 * k]) * p.scale,
-                                    __uint_as_float(ov[2 * k + 1]) * p.scale);
+                          : T::pack(__uint_as_float(ov[2 * k]) * down,
+                                    __uint_as_float(ov[2 * k + 1]) * down);
         if (last >= 0 && q == D / 32 - 1) {
           tc_fence_before();
           mbar_arrive(&o_empty[w]);
@@ -1028,7 +1155,7 @@ __global__ void __launch_bounds__(kBwdThreads, 1)
         f2_unpack(psum[1], b0, b1);
         // the sink's own weight e^(sink - lse): 0 where the sink is -inf
         const float weight = ex2_approx(fmaf(__ldg(p.sink + it.kvh * p.s.g + head), kLog2e, st.x));
-        const float sum = (a0 + a1) + (b0 + b1);
+        const float sum = ((a0 + a1) + (b0 + b1)) * (T::kNarrow ? kPDown : 1.f);
         p.sink_rows[orow] = st.x == -INFINITY ? 0.f : weight * sum;
       }
     }
@@ -1074,7 +1201,7 @@ struct BwdPlan {
   int gb, hb, tt;
   int key_tiles, first_tiles, split_first, split, units_per_head;
   int64_t units;
-  size_t off_stat, off_rows, off_sum, off_parts, bytes;
+  size_t off_stat, off_rows, off_sum, off_peaks, off_parts, bytes;
 };
 
 inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -1110,7 +1237,8 @@ inline BwdPlan plan_bwd(const Shape& s, int64_t batch, int d, bool shared) {
   b.off_stat = 0;
   b.off_rows = pad(rows * sizeof(float2));
   b.off_sum = b.off_rows + pad(rows * sizeof(float));
-  b.off_parts = b.off_sum + pad(static_cast<size_t>(div_up(batch * s.m, kSinkRows)) * s.h * sizeof(float));
+  b.off_peaks = b.off_sum + pad(static_cast<size_t>(div_up(batch * s.m, kSinkRows)) * s.h * sizeof(float));
+  b.off_parts = b.off_peaks + pad(static_cast<size_t>(batch) * s.hk * sizeof(Peak));
   const bool parts = b.split > 1 || (b.first_tiles > 0 && b.split_first > 1);
   b.bytes = b.off_parts +
             (parts ? static_cast<size_t>(b.units) * (shared ? 1 : 2) * kRows * d * sizeof(float) : 0);
@@ -1133,13 +1261,18 @@ int launch_bwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   float2* stat = reinterpret_cast<float2*>(ws + b.off_stat);
   float* sink_rows = reinterpret_cast<float*>(ws + b.off_rows);
   float* sink_sum = reinterpret_cast<float*>(ws + b.off_sum);
+  Peak* peaks = reinterpret_cast<Peak*>(ws + b.off_peaks);
   if (rows > 0) {
+    if (T::kNarrow) {
+      st = cuda_status(cudaMemsetAsync(peaks, 0, static_cast<size_t>(batch) * s.hk * sizeof(Peak), stream));
+      if (st != DSA_OK) return st;
+    }
     const bool flat = dos.h == D && dos.t == static_cast<int64_t>(s.h) * D &&
                       (batch == 1 || dos.b == dos.t * s.m);
     auto kernel = flat ? window_stat_kernel<T, D, true> : window_stat_kernel<T, D, false>;
     kernel<<<static_cast<unsigned>(div_up(rows, 256 / (D / 8) * kStatRows)), 256, 0, stream>>>(
-        static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(dout), dos, lse, stat, rows,
-        s.m, s.h);
+        static_cast<const uint16_t*>(out), static_cast<const uint16_t*>(dout), dos, lse, stat,
+        sink_rows, peaks, rows, s.m, s.h, s.g);
     st = cuda_status(cudaGetLastError());
     if (st != DSA_OK) return st;
   }
@@ -1174,7 +1307,7 @@ int launch_bwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
     if (st != DSA_OK) return st;
     const int64_t grid = p.units < di.num_sms ? p.units : di.num_sms;
     kernel<<<static_cast<unsigned>(grid), kBwdThreads, DkvCfg<D>::kSmemBytes, stream>>>(
-        tm_q, tm_do, tm_k, tm_v, p);
+        tm_q, tm_do, tm_k, tm_v, p, peaks);
     st = cuda_status(cudaGetLastError());
     if (st != DSA_OK) return st;
     const int tiles = b.split > 1 ? b.key_tiles : (b.split_first > 1 ? b.first_tiles : 0);
@@ -1195,6 +1328,7 @@ int launch_bwd(const Tensors& x, const Shape& s, int64_t batch, float scale, con
   p.scale = scale;
   p.scale_log2 = scale * kLog2e;
   p.stat = stat;
+  p.peaks = peaks;
   p.sink = dsink != nullptr ? sink : nullptr;
   p.dq = static_cast<uint16_t*>(dq);
   p.sink_rows = sink_rows;

@@ -28,15 +28,18 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kBoxBytes = kRows * 128;  // one [128 rows x 64 columns] SW128 box
 
 // 16-bit operand types: element format of tcgen05 kind::f16 and the rounding
-// of two fp32 values into a packed pair (low half first).
+// of two fp32 values into a packed pair (low half first). kNarrow: the exponent's range is
+// smaller than fp32's, so values far from 1 have to be scaled before they are rounded.
 struct Bf16 {
   static constexpr uint32_t kFmt = 1;
+  static constexpr bool kNarrow = false;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
   static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
   static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 };
 struct Fp16 {
   static constexpr uint32_t kFmt = 0;
+  static constexpr bool kNarrow = true;
   static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

@@ -362,9 +362,10 @@ int dsa_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k,
  *   -sum over batch and rows of e^(sink[h] - lse) sum_j P_j (dout.v_j)
  * dq like q, dk and dv like k and v (contiguous, the type of q; rows at or past
  * kv_lens[b] get 0); dv NULL when v is k: dk receives the sum of both. dsink
- * [n_heads] fp32 or NULL. Deterministic: no atomics, sums in a fixed order in
- * fp32; P and dS are rounded to the operands' type for the products that sum over
- * them. workspace: dsa_window_attn_bwd_workspace_bytes(...) bytes (shared_kv:
+ * [n_heads] fp32 or NULL. Deterministic: sums in a fixed order in fp32, no atomics
+ * but maxima; P and dS are rounded to the operands' type for the products that sum over
+ * them, in fp16 after scaling by powers of two (2^14 for P; for dS so that |dout| |v| + |D|
+ * stands for 2^14), which keeps small gradients and those whose dS passes 65504. workspace: dsa_window_attn_bwd_workspace_bytes(...) bytes (shared_kv:
  * dv is NULL; 0 for arguments the call refuses), 256-byte aligned. */
 size_t dsa_window_attn_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t n, int n_heads,
                                            int n_kv_heads, int head_dim, int64_t window,
