@@ -248,13 +248,17 @@ class PagedKVCache:
         width = -(-budget // self.page_size)
         after = [min(n, budget) for n in self.host_lens]
         need = [-(-n // self.page_size) for n in after]
-        flat, fresh = self._take(sum(need)), []
+        taken, fresh, at = self._take(sum(need)), [], 0
         for n in need:
-            fresh.append(flat[:n])
-            del flat[:n]
-        kept, left = cache_evict(self.k_pages, self.v_pages, self.weights, self.block_table,
-                                 self.lens, self._upload(fresh, width), budget=budget,
-                                 n_first=n_first, n_recent=n_recent)
+            fresh.append(taken[at:at + n])
+            at += n
+        try:
+            kept, left = cache_evict(self.k_pages, self.v_pages, self.weights, self.block_table,
+                                     self.lens, self._upload(fresh, width), budget=budget,
+                                     n_first=n_first, n_recent=n_recent)
+        except Exception:
+            self.free += taken[::-1]  # as _take found them
+            raise
         self.host_lens = after
         for old in self.pages:
             self.free += old
