@@ -178,8 +178,10 @@ def cache_evict(k_pages: torch.Tensor, v_pages: torch.Tensor | None, weights: to
 class PagedKVCache:
     """A pool of pages with the tables, lengths and free pages of a batch of sequences.
 
-    Page numbers and lengths are kept on the host as well, so no call waits for the GPU;
-    the pool is used on the caller's current stream, in call order. ``shared`` holds one
+    Page numbers and lengths are kept on the host as well and go up from pinned memory, so no
+    call waits for the GPU (the first ones may, while that memory is allocated); the pool is
+    used on the caller's current stream, in call order. All sequences advance together: an
+    ``append`` adds as many rows to each. ``shared`` holds one
     tensor that serves as keys and values; ``track_weights`` holds the attention each row
     gathers (needed for :meth:`evict`).
     """
@@ -210,9 +212,11 @@ class PagedKVCache:
         del self.free[len(self.free) - count:]
         return taken
 
-    def _upload(self, rows: list[list[int]], width: int) -> torch.Tensor:
-        flat = torch.tensor([r + [-1] * (width - len(r)) for r in rows], dtype=torch.int32)
-        return flat.to(self.block_table.device)
+    def _table(self, rows: list[list[int]], width: int) -> torch.Tensor:
+        """The rows' page numbers on the host, in pinned memory where the pool is on a GPU: a
+        copy from there need not be waited for (torch keeps the memory until it is done)."""
+        return torch.tensor([r + [-1] * (width - len(r)) for r in rows], dtype=torch.int32,
+                            pin_memory=self.block_table.is_cuda)
 
     def append(self, k: torch.Tensor, v: torch.Tensor | None = None) -> None:
         """Adds the next rows k, v [batch, t, hk, d] of every sequence."""
@@ -228,7 +232,7 @@ class PagedKVCache:
                 if n > 0:
                     self.pages[i] += taken[:n]
                     del taken[:n]
-            self.block_table.copy_(self._upload(self.pages, self.max_pages))
+            self.block_table.copy_(self._table(self.pages, self.max_pages), non_blocking=True)
         cache_append(k, v, self.k_pages, self.v_pages, self.block_table, self.lens, self.weights)
         self.lens += t
         self.host_lens = [n + t for n in self.host_lens]
@@ -253,9 +257,10 @@ class PagedKVCache:
             fresh.append(taken[at:at + n])
             at += n
         try:
+            dst = self._table(fresh, width).to(self.block_table.device, non_blocking=True)
             kept, left = cache_evict(self.k_pages, self.v_pages, self.weights, self.block_table,
-                                     self.lens, self._upload(fresh, width), budget=budget,
-                                     n_first=n_first, n_recent=n_recent)
+                                     self.lens, dst, budget=budget, n_first=n_first,
+                                     n_recent=n_recent)
         except Exception:
             self.free += taken[::-1]  # as _take found them
             raise
@@ -263,6 +268,6 @@ class PagedKVCache:
         for old in self.pages:
             self.free += old
         self.pages = fresh
-        self.block_table.copy_(self._upload(self.pages, self.max_pages))
+        self.block_table.copy_(self._table(self.pages, self.max_pages), non_blocking=True)
         self.lens.copy_(left)
         return kept

@@ -1,5 +1,5 @@
 """Windowed attention and the paged cache at the ends of their ranges: chunks whose pages are
-absent under very low scores.
+absent under very low scores, a pool whose calls must not wait for the GPU.
 
 Bounds as in test_paged_cache_gpu.py; where scores are about -100, their fp32 sums (64 terms,
 each addition off by at most 2^-23 of 800, times the scale of 1/8) are good to 8e-4, so the
@@ -12,7 +12,7 @@ import pytest
 import torch
 
 from ascendc_kernel_b200 import _native
-from ascendc_kernel_b200.paged_cache import paged_attn
+from ascendc_kernel_b200.paged_cache import PagedKVCache, paged_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,37 @@ def test_absent_chunks_under_low_scores(cuda_device, rows, page, gone, weighted)
     if weighted:
         assert not weights[~live].any()
         assert ((weights[live].double() - p.sum(0)).abs() <= 1e-3 * p.sum(0)).all()
+
+
+def test_pool_calls_do_not_wait(cuda_device):
+    """Appends that take pages and evictions while the stream is busy: torch reports a call that
+    would wait, and the tables that they send arrive whole."""
+    b, page, d = 2, 16, 64
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn(b, 60, 1, d, generator=g, device="cuda").to(torch.bfloat16)
+    q = torch.randn(b, 4, d, generator=g, device="cuda").to(torch.bfloat16)
+
+    def steps(c):
+        for t in (60, 40, 1, 30):
+            c.append(x[:, :t].contiguous())
+            c.attend(q)
+            c.evict(50, 2, 4)
+            c.append(x[:, t - 1:t].contiguous())
+        return c.attend(q), c.lens.clone()
+
+    def pool():
+        return PagedKVCache(b, 40, page, 200, 1, d, shared=True, track_weights=True)
+
+    want, lens = steps(pool())
+    busy = pool()
+    torch.cuda.synchronize()
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        torch.cuda._sleep(20_000_000)  # about 10 ms: every upload below is pending at once
+        got, left = steps(busy)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(got, want) and torch.equal(left, lens)
+    assert busy.lens.tolist() == busy.host_lens
+    for i, pages in enumerate(busy.pages):
+        assert busy.block_table[i].tolist() == pages + [-1] * (busy.max_pages - len(pages))
