@@ -161,12 +161,16 @@ class _WindowAttn(torch.autograd.Function):
                             None, True)
         ctx.save_for_backward(q, k, v, sink, kv_lens, out, lse)
         ctx.args = (window, n_first, scale)
-        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
-    def backward(ctx, dout, _):
+    def backward(ctx, dout, dlse):
+        if dlse is not None:
+            raise RuntimeError("the lse of window_attn has no gradient: detach it in the loss")
+        if dout is None:
+            return (None,) * 8
         q, k, v, sink, kv_lens, out, lse = ctx.saved_tensors
         window, n_first, scale = ctx.args
         dq, dk, dv, dsink = window_attn_bwd(dout, q, k, v, sink, out, lse, window=window,
@@ -190,7 +194,8 @@ def window_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None,
     that see nothing and have no sink are 0. Returns out like q, and with ``return_lse``
     also the fp32 log of the softmax divisor [b, m, h].
 
-    Differentiable in q, k, v and sink (``out`` must then be None).
+    out is differentiable in q, k, v and sink (the ``out`` argument must then be None). lse is
+    not: a backward pass that reaches it raises RuntimeError.
     """
     scale = float(q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale)
     _check(q, k, v, sink, window, n_first, kv_lens, scale)

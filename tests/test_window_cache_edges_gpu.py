@@ -1,5 +1,6 @@
 """Windowed attention and the paged cache at the ends of their ranges: chunks whose pages are
-absent under very low scores, a pool whose calls must not wait for the GPU.
+absent under very low scores, a pool whose calls must not wait for the GPU, losses that
+use what has no gradient.
 
 Bounds as in test_paged_cache_gpu.py; where scores are about -100, their fp32 sums (64 terms,
 each addition off by at most 2^-23 of 800, times the scale of 1/8) are good to 8e-4, so the
@@ -13,6 +14,7 @@ import torch
 
 from ascendc_kernel_b200 import _native
 from ascendc_kernel_b200.paged_cache import PagedKVCache, paged_attn
+from ascendc_kernel_b200.window_attn import window_attn
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +93,20 @@ def test_pool_calls_do_not_wait(cuda_device):
     assert busy.lens.tolist() == busy.host_lens
     for i, pages in enumerate(busy.pages):
         assert busy.block_table[i].tolist() == pages + [-1] * (busy.max_pages - len(pages))
+
+
+def test_a_loss_with_lse_is_refused(cuda_device):
+    """lse has no gradient: a loss that uses it must not get one without its share."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    q, k = (torch.randn(1, 20, h, 64, generator=g, device="cuda").to(torch.bfloat16)
+            .requires_grad_(True) for h in (4, 2))
+    sink = torch.randn(4, generator=g, device="cuda").requires_grad_(True)
+    out, lse = window_attn(q, k, None, sink, window=9, return_lse=True)
+    for loss in (out.float().sum() + lse.square().sum(), lse.sum()):
+        with pytest.raises(RuntimeError, match="lse"):
+            torch.autograd.grad(loss, (q, k, sink), retain_graph=True)
+    # without it, and with it detached, nothing changes
+    want = torch.autograd.grad(window_attn(q, k, None, sink, window=9).float().sum(), (q, k, sink))
+    for loss in (out.float().sum(), out.float().sum() + lse.detach().sum()):
+        for a, b in zip(torch.autograd.grad(loss, (q, k, sink), retain_graph=True), want):
+            assert torch.equal(a, b)
