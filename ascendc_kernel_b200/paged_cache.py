@@ -57,6 +57,19 @@ def _check_lens(lens, b, dev, name="lens"):
         f"{name} must be int32 [b] on the pool's device"
 
 
+class _NoGradient(torch.autograd.Function):
+    """x, whose gradient is asked for in vain: better an error than a loss without its share."""
+
+    @staticmethod
+    def forward(ctx, x, *sources):
+        return x.view_as(x)
+
+    @staticmethod
+    def backward(ctx, dx):
+        raise RuntimeError("paged_attn has no gradient: train with window_attn, or call it "
+                           "under torch.no_grad()")
+
+
 @functools.lru_cache(maxsize=256)
 def _attn_workspace(b, h, hk, d, max_pages, page, weights) -> int:
     return max(lib().dsa_paged_attn_workspace_bytes(b, h, hk, d, max_pages, page, weights), 256)
@@ -74,9 +87,11 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor | N
     them; sink [h] fp32 logits or None; softmax_scale defaults to d ** -0.5. Returns out
     like q (0 where nothing is visible and there is no sink) and with ``return_lse`` the
     fp32 log of the softmax divisor [b, h]. With ``weights`` the slot of each visible row
-    gains its attention weight summed over the heads, in place.
+    gains its attention weight summed over the heads, in place. Not differentiable: a
+    backward pass that reaches the results of a call with gradients raises RuntimeError.
     """
     assert q.dim() == 3, "q must be [b, h, d]"
+    given = (q, k_pages, v_pages, sink)
     n, page, hk, d, dev = _check_pool(k_pages, v_pages, weights, block_table)
     b, h, _ = q.shape
     assert q.dtype == k_pages.dtype and q.device == dev and q.shape[2] == d, \
@@ -118,6 +133,11 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor | N
          values, v_strides, table.data_ptr(), lens.data_ptr(), _ptr(sink), out.data_ptr(), _ptr(lse),
          _ptr(weights), DTYPES[q.dtype], b, h, hk, d, n, page, width, min(int(window), 1 << 28),
          min(int(n_first), 1 << 28), scale, ws.data_ptr(), nbytes)
+    if torch.is_grad_enabled():
+        sources = [x for x in given if x is not None and x.requires_grad]
+        if sources:
+            out = _NoGradient.apply(out, *sources)
+            lse = _NoGradient.apply(lse, *sources) if return_lse else None
     return (out, lse) if return_lse else out
 
 

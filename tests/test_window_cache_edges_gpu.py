@@ -110,3 +110,33 @@ def test_a_loss_with_lse_is_refused(cuda_device):
     for loss in (out.float().sum(), out.float().sum() + lse.detach().sum()):
         for a, b in zip(torch.autograd.grad(loss, (q, k, sink), retain_graph=True), want):
             assert torch.equal(a, b)
+
+
+def test_a_loss_over_the_cache_is_refused(cuda_device):
+    """Single-token attention has no gradient: neither q's nor the sink's graph ends silently."""
+    g = torch.Generator(device="cuda").manual_seed(8)
+    k = torch.randn(3, 16, 1, 64, generator=g, device="cuda").to(torch.bfloat16)
+    table = torch.arange(3, dtype=torch.int32, device="cuda")[None].contiguous()
+    n = torch.full((1,), 40, dtype=torch.int32, device="cuda")
+    q = torch.randn(1, 4, 64, generator=g, device="cuda").to(torch.bfloat16)
+    sink = torch.randn(4, generator=g, device="cuda")
+    want, want_lse = paged_attn(q, k, None, table, n, sink, return_lse=True)
+    assert not want.requires_grad and not want_lse.requires_grad
+    for leaf in ("q", "sink", "noncontiguous q", "fp64 sink"):
+        a, s = q.clone(), sink.clone()
+        x = s if "sink" in leaf else a
+        x.requires_grad_(True)
+        if leaf == "fp64 sink":
+            s = s.double()
+        if leaf == "noncontiguous q":
+            a = a.transpose(1, 2).contiguous().transpose(1, 2)
+        buffer = torch.empty_like(q)
+        for kw in (dict(), dict(out=buffer)):
+            out, lse = paged_attn(a, k, None, table, n, s, return_lse=True, **kw)
+            assert torch.equal(out, want) and torch.equal(lse, want_lse)
+            for y in (out, lse):
+                with pytest.raises(RuntimeError, match="no gradient"):
+                    (x.float().sum() + y.float().sum()).backward()
+            with torch.no_grad():
+                assert not paged_attn(a, k, None, table, n, s, **kw).requires_grad
+        assert torch.equal(buffer, want)
