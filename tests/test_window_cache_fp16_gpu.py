@@ -1,4 +1,4 @@
-"""fp16 windowed attention with the bounds that its arithmetic gives.
+"""fp16 windowed and paged attention with the bounds that its arithmetic gives.
 
 u = 2^-11 is the unit roundoff of fp16; below 2^-14 its step is 2^-24, so a rounding is off by
 2^-25 at most there. Forward: a weight P is rounded relative to a reference that is a score
@@ -18,7 +18,10 @@ import pytest
 import torch
 
 from ascendc_kernel_b200 import _native
+from ascendc_kernel_b200.paged_cache import paged_attn
 from ascendc_kernel_b200.window_attn import window_attn, window_attn_bwd
+from tests import test_paged_cache_gpu as paged_tests
+from tests import test_window_attn_gpu as window_tests
 
 pytestmark = pytest.mark.gpu
 
@@ -127,3 +130,53 @@ def test_gradients_where_ds_passes_fp16(cuda_device, d):
     for name, x in zip(("dq", "dk", "dv"), got):
         within(x[0], want[name], bound[name], name)
     assert _native.device_error(0) == 0
+
+
+@pytest.mark.parametrize("rows,h,hk,d", [(5000, 8, 2, 64), (9000, 64, 1, 128), (30000, 8, 2, 64),
+                                         (30000, 128, 1, 64)])
+def test_long_paged_rows(cuda_device, rows, h, hk, d):
+    page = 64
+    g = torch.Generator(device="cuda").manual_seed(3)
+    width = -(-rows // page)
+    k = torch.randn(width, page, hk, d, generator=g, device="cuda").half()
+    v = torch.randn(width, page, hk, d, generator=g, device="cuda").half()
+    q = torch.randn(1, h, d, generator=g, device="cuda").half()
+    table = torch.arange(width, dtype=torch.int32, device="cuda")[None].contiguous()
+    n = torch.full((1,), rows, dtype=torch.int32, device="cuda")
+    out = paged_attn(q, k, v, table, n)
+    kk, vv = (x.reshape(-1, hk, d)[:rows].double().transpose(0, 1).repeat_interleave(h // hk, 0)
+              for x in (k, v))
+    p = torch.softmax((kk @ q[0].double()[:, :, None])[..., 0] * d ** -0.5, -1)[:, None]
+    want, mag = (p @ vv)[:, 0], (p @ vv.abs())[:, 0]
+    bound = U * (want.abs() + mag) + F32 * mag + STEP * (vv.abs().sum(1) + 1)
+    within(out[0], want, bound, "out")
+    assert _native.device_error(0) == 0
+
+
+@pytest.fixture
+def step(monkeypatch):
+    """The other files' bounds with 2^-25 a key for fp16 in place of their 2^-17: where their
+    reference lies 2^8 below the maximum, the divisor is that much larger too, and the
+    gradients' P and dS are scaled. In the long cases 2^-17 a key allows anything."""
+    monkeypatch.setitem(window_tests.TINY, torch.float16, STEP)
+    monkeypatch.setitem(paged_tests.TINY, torch.float16, STEP)
+
+
+@pytest.mark.parametrize("shape", window_tests.SHAPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sink,shared,ragged", [(True, True, False), (False, False, True),
+                                                (True, False, True), (False, True, False)])
+def test_window_shapes(cuda_device, step, shape, d, sink, shared, ragged):
+    window_tests.test_forward_and_gradients(cuda_device, shape, d, torch.float16, sink, shared,
+                                            ragged)
+
+
+def test_window_score_range(cuda_device, step):
+    window_tests.test_large_and_small_scores(cuda_device)
+
+
+@pytest.mark.parametrize("case", paged_tests.CASES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sink,shared", [(True, True), (False, False)])
+def test_paged_cases(cuda_device, step, case, d, sink, shared):
+    paged_tests.test_paged_attention(cuda_device, case, d, torch.float16, sink, shared)
