@@ -87,7 +87,8 @@ def paged_attn(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor | N
     them; sink [h] fp32 logits or None; softmax_scale defaults to d ** -0.5. Returns out
     like q (0 where nothing is visible and there is no sink) and with ``return_lse`` the
     fp32 log of the softmax divisor [b, h]. With ``weights`` the slot of each visible row
-    gains its attention weight summed over the heads, in place. Not differentiable: a
+    gains its attention weight summed over the heads, in place. The softmax's weights are
+    rounded to q's type before they meet v, everything else is fp32. Not differentiable: a
     backward pass that reaches the results of a call with gradients raises RuntimeError.
     """
     assert q.dim() == 3, "q must be [b, h, d]"

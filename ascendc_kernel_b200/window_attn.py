@@ -194,6 +194,15 @@ def window_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor | None = None,
     that see nothing and have no sink are 0. Returns out like q, and with ``return_lse``
     also the fp32 log of the softmax divisor [b, m, h].
 
+    Positions are the same in every sequence: ``kv_lens`` hides keys and moves no query. It
+    is for prompts padded on the right (m = n). The next chunk of sequences whose prefixes
+    differ in length has a position of its own in each: give each length a call, with k and
+    v cut to it (n = kv_lens[b]).
+
+    The softmax's weights are rounded to q's type before they meet v (its maxima, sums and
+    products are fp32), in the backward pass dS too: an error of the size of the results'
+    own rounding.
+
     out is differentiable in q, k, v and sink (the ``out`` argument must then be None). lse is
     not: a backward pass that reaches it raises RuntimeError.
     """

@@ -326,7 +326,10 @@ int dsa_chain_fwd(const void* x, const void* qr, const void* wq_b, const void* w
  *   q   [batch, m, n_heads, head_dim], out like q (contiguous)
  *   k,v [batch, n, n_kv_heads, head_dim]; v may be k (one tensor for both)
  * Query t stands at position p = t + n - m and sees key j when j <= p,
- * j < kv_lens[b] (NULL: n) and (j > p - window or j < n_first). With s_j =
+ * j < kv_lens[b] (NULL: n) and (j > p - window or j < n_first). The positions are
+ * the same in every batch entry: kv_lens hides keys and moves no query, so it suits
+ * prompts padded on the right (m = n); a chunk after prefixes of different lengths
+ * takes a call per length, with n = that length. With s_j =
  * softmax_scale q.k_j over the keys it sees (n_heads / n_kv_heads query heads
  * share a kv head):
  *   lse = log(sum_j e^s_j + e^sink[h]),  out = sum_j e^(s_j - lse) v_j
@@ -334,9 +337,10 @@ int dsa_chain_fwd(const void* x, const void* qr, const void* wq_b, const void* w
  * gets out = 0, lse = -inf. k and v rows at or past kv_lens[b] may hold
  * anything; rows below it have to be finite: one that is not reaches every query
  * row of the tiles that read it, also those that do not see it (a masked weight is
- * 0, and 0 x NaN is NaN, as in the dense form). Products of the 16-bit operands are summed in fp32; the softmax
- * runs in fp32; its weights are rounded to the operands' type for the second
- * product and out once at the end.
+ * 0, and 0 x NaN is NaN, as in the dense form). Products of the 16-bit operands are
+ * summed in fp32; the softmax runs in fp32; its weights are rounded to the operands'
+ * type for the second product (relative 2^-8 for bf16; for fp16 2^-11, and 2^-25 of the
+ * row's largest weight below 2^-14 of it) and out once at the end.
  * dtype: DSA_DTYPE_*, of q, k, v and out. q_strides, k_strides, v_strides:
  * strides in elements of (batch, token, head), host arrays, NULL for
  * contiguous; head_dim is contiguous. lse [batch, m, n_heads] fp32 or NULL.
@@ -403,7 +407,9 @@ int dsa_window_attn_bwd(const void* q, const int64_t* q_strides, const void* k,
  * head_dim 64 or 128, n_heads / n_kv_heads <= 128, page_size a multiple of 8,
  * max_pages * page_size <= 2^28, batch <= 65535. workspace:
  * dsa_paged_attn_workspace_bytes(...) bytes (want_weights: weights is given),
- * 256-byte aligned. No counterpart in the reference. */
+ * 256-byte aligned. With weights it holds every score that the table has room for, 4
+ * bytes x batch x n_heads x max_pages x page_size, whatever the lengths and the window:
+ * keep the table as narrow as the longest sequence. No counterpart in the reference. */
 size_t dsa_paged_attn_workspace_bytes(int64_t batch, int n_heads, int n_kv_heads, int head_dim,
                                       int64_t max_pages, int64_t page_size, int want_weights);
 int dsa_paged_attn_fwd(const void* q, const int64_t* q_strides, const void* k_pages,
@@ -439,8 +445,8 @@ int dsa_cache_append(const void* k, const int64_t* k_strides, const void* v,
  * old pages are left as they are. The pages of dst_table must be distinct and belong to
  * no sequence of the call; entries past the kept rows may name none (-1). A kept row
  * whose dst_table entry names no page is not copied (DSA_DEVERR_CACHE); the same for
- * rows of block_table entries that name none (their weights rank below all others). Requires n_first + n_recent <= budget <=
- * dst_pages * page_size, max_pages * page_size <= 2^28, batch <= 65535. Exact and
+ * rows of block_table entries that name none (their weights rank below all others).
+ * Requires n_first + n_recent <= budget <= dst_pages * page_size, max_pages * page_size <= 2^28, batch <= 65535. Exact and
  * deterministic. No counterpart in the reference. */
 int dsa_cache_evict(void* k_pages, const int64_t* kp_strides, void* v_pages,
                     const int64_t* vp_strides, float* weights, const int* block_table,

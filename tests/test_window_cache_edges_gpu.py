@@ -1,6 +1,6 @@
 """Windowed attention and the paged cache at the ends of their ranges: chunks whose pages are
 absent under very low scores, a pool whose calls must not wait for the GPU, losses that
-use what has no gradient.
+use what has no gradient, chunks after prefixes of different lengths.
 
 Bounds as in test_paged_cache_gpu.py; where scores are about -100, their fp32 sums (64 terms,
 each addition off by at most 2^-23 of 800, times the scale of 1/8) are good to 8e-4, so the
@@ -140,3 +140,29 @@ def test_a_loss_over_the_cache_is_refused(cuda_device):
             with torch.no_grad():
                 assert not paged_attn(a, k, None, table, n, s, **kw).requires_grad
         assert torch.equal(buffer, want)
+
+
+def test_a_chunk_after_prefixes_of_different_lengths(cuda_device):
+    """kv_lens hides keys and moves no query: of a padded batch, a chunk's queries stand where
+    the padded length puts them. A call per length, on keys cut to it, is the chunk of that
+    sequence's own whole prompt."""
+    m, h, hk, d, n, lens = 40, 6, 2, 64, 300, [300, 137, 45, 40]
+    g = torch.Generator(device="cuda").manual_seed(9)
+    whole = torch.randn(4, n, h, d, generator=g, device="cuda").to(torch.bfloat16)
+    k, v = (torch.randn(4, n, hk, d, generator=g, device="cuda").to(torch.bfloat16)
+            for _ in range(2))
+    kw = dict(window=60, n_first=3)
+    full = window_attn(whole, k, v, kv_lens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
+                       **kw)  # whole prompts, padded on the right
+    for i, x in enumerate(lens):
+        rows = slice(x - m, x)
+        got = window_attn(whole[i:i + 1, rows], k[i:i + 1, :x], v[i:i + 1, :x], **kw)
+        # the rounding of the softmax's weights depends on how the keys are cut into blocks:
+        # both sides are within u (|out| + sum P |v|) of the definition
+        scale = v[i, :x].abs().max().double()
+        assert ((got[0].double() - full[i, rows].double()).abs() <= 2 * 2.0 ** -8 * 2 * scale).all()
+    # the padded form is another thing: the second sequence's queries stand past its keys
+    n_i = torch.tensor([lens[1]], dtype=torch.int32, device="cuda")
+    far = window_attn(whole[1:2, :m], k[1:2], v[1:2], kv_lens=n_i, **kw)
+    want = window_attn(whole[1:2, :1], k[1:2, :3], v[1:2, :3], window=3)
+    assert ((far[0, 0].double() - want[0, 0].double()).abs() <= 2.0 ** -6 * v.abs().max()).all()
