@@ -106,8 +106,8 @@ __device__ __forceinline__ void copy_rows(const RowCopy& c, const RowPlan& plan)
   }
 }
 
-// Rows of a block: few enough that the call fills the GPU's thread slots about twice,
-// one at least.
+// Rows of a block: few enough that the call fills the thread slots of a full GPU (148 SMs of 8
+// blocks) about twice, one at least.
 inline int rows_per_block(int64_t rows) {
   const int64_t r = rows / (2 * 148 * 8);
   return static_cast<int>(r < 1 ? 1 : (r > kCopyRows ? kCopyRows : r));

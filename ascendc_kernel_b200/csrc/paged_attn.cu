@@ -27,7 +27,8 @@
 // piece and moves (O and the sums are rescaled) only when a score exceeds it by more
 // than 2^14, so the common chunk needs one vote and no reduction over keys; the sums
 // stay per thread until the piece ends. P is rounded to the operands' type
-// (relative 2^-8 at most for bf16, the size of the output's own rounding); sums are fp32.
+// (relative 2^-8 at most for bf16, 2^-11 for fp16 and below its normal range 2^-25 of the row's
+// largest P: the size of the output's own rounding); sums are fp32.
 // TMEM: kSBufs S^T buffers of NM columns, then O^T of the two warpgroups.
 //
 // Measured (bf16, head_dim 128):
@@ -915,7 +916,9 @@ inline int64_t max_chunks(int64_t max_pages, int64_t page) {
   return (max_pages * page + kKeys - 1) / kKeys + 2;
 }
 
-// One CTA per SM of a full GPU, fewer when the batch cannot have that many chunks.
+// One CTA per SM of a full GPU (148, also on a part of one: the pieces and with them the bits
+// stay the same, and no CTA waits for another), fewer when the batch cannot have that many
+// chunks.
 inline Plan plan_paged(int64_t batch, int h, int hk, int d, int64_t max_pages, int64_t page,
                        bool weights) {
   Plan pl;

@@ -34,8 +34,9 @@
 //   join 9; the five products the formulas need run at 440 TFLOP/s, the seven done at
 //   613. Tensor pipe 45 % (dk/dv) and 32 % (dq), issue slots 34 % and 27 %, DRAM below 8 %:
 //   bound by the chain S, dP -> P, dS -> products of a tile, of which two are in flight
-//   (TMEM is full: two accumulators and two pairs of S and dP), and by the 64-wide
-//   products, which read shared memory faster than they compute.
+//   (dk/dv fills TMEM with two accumulators and two pairs of S and dP; dq has one pair a tile,
+//   so that its next scores wait for the product of this chunk), and by the 64-wide products,
+//   which read shared memory faster than they compute.
 //   2 x 2600 tokens, 64 heads on one kv head, window 128 + 4: dk/dv 200, dq 96, statistics
 //   31, join 12, dsink 6.
 #include "host_util.h"
@@ -1207,7 +1208,8 @@ struct BwdPlan {
 inline int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Key tiles are split over their rows so that no unit is much longer than an equal
-// share of a third of an SM (kUnits = 3 x 148), and none is shorter than 16
+// share of a third of an SM (kUnits = 3 x 148; the number is fixed, so that a sum's parts are
+// the same on every device), and none is shorter than 16
 // streamed tiles, below which the fp32 parts cost more than the balance gives.
 inline BwdPlan plan_bwd(const Shape& s, int64_t batch, int d, bool shared) {
   constexpr int64_t kUnits = 3 * 148;

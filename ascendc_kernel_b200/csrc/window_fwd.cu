@@ -20,15 +20,17 @@
 // when the softmax gets to them. One issuer for both tiles was the bottleneck: its
 // waits and commits took 2,000 of the 3,400 cycles of a chunk.
 // P is rounded to the operands' 16-bit type for the second product (its sum is
-// taken before the rounding, in fp32): a relative 2^-8 (2^-11 for fp16) a term at most,
-// the size of the output's own rounding. The reference moves, and O is rescaled,
+// taken before the rounding, in fp32): a relative 2^-8 (2^-11 for fp16, below its normal range
+// 2^-25 of the row's largest P) a term at most, the size of the output's own rounding. The
+// reference moves, and O is rescaled,
 // only when a row's maximum exceeds it by more than 2^8, so P stays within fp16.
 // TMEM per tile w: S/P buffers [256w, +64), [256w+64, +64), O [256w+128, +D).
 //
 // Measured (bf16, head_dim 128):
 //   8 x 2600 tokens, 64 heads on one kv head, window 128 + 4: 233 us, 2.9 TB/s of q and
-//   out (0.45 of a copy). An item has 5 chunks, so its start (q, the first scores)
-//   and its end (O to HBM) are most of it; the tensor pipe is active 27 % of the time.
+//   out (0.45 of a copy). An item is 4 tokens: 131 keys of the window and 4 first ones, 6
+//   blocks, 3 chunks; with its start (q, the first scores) and its end (O to HBM) it takes
+//   6.5 us where its bytes take 3.0; the tensor pipe is active 27 % of the time.
 //   16,384 tokens, 32 heads on 8, window 4096 + 4: 1,090-1,110 us, 870 TFLOP/s (0.52 of a
 //   library GEMM's burst). Tensor pipe 44 %, exponentials 45 %, issue slots 45 %: no
 //   unit is full; the chain S -> maximum -> 2^x -> P -> O of a chunk is what a row's
