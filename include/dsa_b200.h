@@ -369,8 +369,9 @@ int dsa_window_attn_fwd(const void* q, const int64_t* q_strides, const void* k,
  * [n_heads] fp32 or NULL. Deterministic: sums in a fixed order in fp32, no atomics
  * but maxima; P and dS are rounded to the operands' type for the products that sum over
  * them, in fp16 after scaling by powers of two (2^14 for P; for dS so that |dout| |v| + |D|
- * stands for 2^14), which keeps small gradients and those whose dS passes 65504. workspace: dsa_window_attn_bwd_workspace_bytes(...) bytes (shared_kv:
- * dv is NULL; 0 for arguments the call refuses), 256-byte aligned. */
+ * stands for 2^14), which keeps small gradients and those whose dS passes 65504.
+ * workspace: dsa_window_attn_bwd_workspace_bytes(...) bytes (shared_kv: dv is NULL; 0 for
+ * arguments the call refuses), 256-byte aligned. */
 size_t dsa_window_attn_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t n, int n_heads,
                                            int n_kv_heads, int head_dim, int64_t window,
                                            int64_t n_first, int shared_kv);
